@@ -115,6 +115,23 @@ SIGNATURES = {
                                      c_float, c_float, _P, _P, c_int, _P, c_int64, c_int, c_int64, c_int64, _P, _P]),
     "sage_adam_step_signal": (c_int, [_P, _P, _P, _P, c_int64, c_float, c_float, c_float, c_float,
                                       c_float, c_float, _P, _P, c_int, _P, _P]),
+    "sage_rms_norm_fwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int64, c_int, c_float, _P, c_int64,
+                                  _P, c_int64, _P]),
+    "sage_rms_norm_int8": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int64, c_int, c_float, c_int, _P,
+                                   c_int64, c_int64, _P, _P, c_int64, _P]),
+    "sage_dequantize_rows": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int, _P, c_int64, _P]),
+    "sage_rms_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "sage_rms_norm_bwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, _P, c_int64, c_int64, c_int64, c_int, c_float,
+                                  _P, c_int64, _P, _P, c_size_t, _P]),
+    "sage_pad_rows": (c_int, [_P, c_int64, c_int64, c_int64, _P, c_int64, _P]),
+    "sage_int8_linear": (c_int, [_P, c_int64, _P, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P]),
+    "sage_int8_gated_linear": (c_int, [_P, c_int64, _P, _P, c_int64, _P, _P, c_int64, _P, c_int, c_int64, c_int64,
+                                       c_int64, c_int, _P, c_int64, _P]),
+    "sage_gated_linear_fwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int, c_int64, c_int64, c_int64, c_int,
+                                      _P, c_int64, _P, _P]),
+    "sage_gated_linear_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "sage_gated_linear_bwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int64,
+                                      c_int64, c_int, _P, c_int64, _P, _P, c_size_t, _P]),
 }
 
 _lib = None

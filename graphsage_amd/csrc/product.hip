@@ -1,0 +1,718 @@
+// Products of the feed-forward block on the matrix cores: the 8-bit product with token and channel
+// scales, the gated projections h = act(x Wg^T) * (x Wu^T), and the products of their backward pass.
+//
+// All of them are C[m, n] = sum_k A[m, k] B[n, k] with both operands' rows contiguous in k, and one
+// kernel body serves every type because it works on 16-byte pieces of rows: a lane's operand of an
+// MFMA is 16 bytes of one row whatever the type (16 int8, 8 bf16 / fp16, 4 fp32), and the order in
+// which the k of a product are summed over lanes is free as long as A and B agree on it.
+#include "common.h"
+
+#include <type_traits>
+
+namespace sage {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(1))) const void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+
+// ------------------------------------------------------------------------------- types
+// Frag: 16 bytes of a row.  mma: 16 x 16 outputs, all k of the two 64-byte row pieces held by the wave.
+template <typename T>
+struct Mma;
+template <>
+struct Mma<int8_t> {
+  using Acc = i32x4;
+  __device__ static Acc mma(const i32x4& a, const i32x4& b, const Acc& c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<__bf16> {
+  using Acc = f32x4;
+  __device__ static Acc mma(const i32x4& a, const i32x4& b, const Acc& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<_Float16> {
+  using Acc = f32x4;
+  __device__ static Acc mma(const i32x4& a, const i32x4& b, const Acc& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {
+  using Acc = f32x4;
+  // four products of one k a lane: lane group q supplies k = 4 q + e of the 16 that the piece holds
+  __device__ static Acc mma(const i32x4& a, const i32x4& b, Acc c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// ------------------------------------------------------------------------------- epilogues
+// kExact: full-precision exponential and division (fp32 outputs); else the hardware's, which are
+// within a few 2^-24 and vanish in a 16-bit rounding.
+template <bool kExact>
+__device__ inline float sigmoid(float g) {
+  if constexpr (kExact) return 1.f / (1.f + expf(-g));
+  else return __builtin_amdgcn_rcpf(1.f + __expf(-g));
+}
+template <bool kExact>
+__device__ inline float act_value(float g, int act) {
+  if (act == SAGE_ACT_SILU) return g * sigmoid<kExact>(g);
+  if (act == SAGE_ACT_GELU) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+  return g < 0.f ? 0.f : g;
+}
+template <bool kExact>
+__device__ inline float act_slope(float g, int act) {
+  if (act == SAGE_ACT_SILU) {
+    const float p = sigmoid<kExact>(g);
+    return p * (1.f + g * (1.f - p));
+  }
+  if (act == SAGE_ACT_GELU) {
+    const float density = 0.39894228040143268f * (kExact ? expf(-0.5f * g * g) : __expf(-0.5f * g * g));
+    return 0.5f * (1.f + erff(g * 0.70710678118654752f)) + g * density;
+  }
+  return g > 0.f ? 1.f : 0.f;
+}
+
+struct Product {
+  const char* a;        // A rows (bytes)
+  const char* b0;       // B rows
+  const char* b1;       // second B of a gated product
+  int64_t lda, ldb0, ldb1;   // row strides in bytes
+  int64_t m, n;         // outputs (n: of each B)
+  int64_t kbytes;       // row length in bytes, a multiple of 16
+  void* out;
+  int64_t ldo;          // in elements
+  int out_dtype;
+  int act;
+  const float* sa;      // int8: scales of A's and B's rows
+  const float* sb0;
+  const float* sb1;
+  const float* bias;
+  float* saved;         // gated, training: pre-activations [2, m, n] in fp32
+};
+
+template <int n, typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Run {
+  T v[n];
+};
+
+template <int n, typename T>
+__device__ inline void store_run(T* p, int64_t left, const float (&v)[n]) {
+  if (left >= n) {
+    Run<n, T> r;
+#pragma unroll
+    for (int i = 0; i < n; ++i) r.v[i] = static_cast<T>(v[i]);
+    *reinterpret_cast<Run<n, T>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      if (i < left) p[i] = static_cast<T>(v[i]);
+  }
+}
+template <int n>
+__device__ inline void store_out(const Product& p, int64_t row, int64_t col, const float (&v)[n]) {
+  const int64_t at = row * p.ldo + col, left = p.n - col;
+  if (p.out_dtype == SAGE_BF16) store_run<n>(static_cast<__bf16*>(p.out) + at, left, v);
+  else if (p.out_dtype == SAGE_F16) store_run<n>(static_cast<_Float16*>(p.out) + at, left, v);
+  else store_run<n>(static_cast<float*>(p.out) + at, left, v);
+}
+
+// n consecutive columns of one row, from the sums of one B
+template <typename T, int n, typename S>
+__device__ inline void finish(const Product& p, int64_t row, int64_t col, const S (&c)[n]) {
+  if (row >= p.m || col >= p.n) return;
+  float v[n];
+  if constexpr (std::is_same<T, int8_t>::value) {
+    const float sa = p.sa[row];
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const int64_t at = col + i < p.n ? col + i : p.n - 1;
+      v[i] = static_cast<float>(c[i]) * (sa * p.sb0[at]) + (p.bias != nullptr ? p.bias[at] : 0.f);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = c[i];
+  }
+  store_out<n>(p, row, col, v);
+}
+
+// the same from the sums of both Bs
+template <typename T, int n, typename S>
+__device__ inline void finish_gated(const Product& p, int64_t row, int64_t col, const S (&cg)[n], const S (&cu)[n]) {
+  if (row >= p.m || col >= p.n) return;
+  float g[n], u[n], v[n];
+  if constexpr (std::is_same<T, int8_t>::value) {
+    const float sa = p.sa[row];
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const int64_t at = col + i < p.n ? col + i : p.n - 1;
+      g[i] = static_cast<float>(cg[i]) * (sa * p.sb0[at]);
+      u[i] = static_cast<float>(cu[i]) * (sa * p.sb1[at]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      g[i] = cg[i];
+      u[i] = cu[i];
+    }
+    if (p.saved != nullptr) {
+      store_run<n>(p.saved + row * p.n + col, p.n - col, g);
+      store_run<n>(p.saved + (p.m + row) * p.n + col, p.n - col, u);
+    }
+  }
+  if (p.out_dtype == SAGE_F32) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = act_value<true>(g[i], p.act) * u[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = act_value<false>(g[i], p.act) * u[i];
+  }
+  store_out<n>(p, row, col, v);
+}
+
+// 16 zero bytes that lanes read whose piece lies behind the row's end
+__device__ const i32x4 kZeroPiece = {0, 0, 0, 0};
+
+// ------------------------------------------------------------------------------- tiles
+// BM x BN outputs a block (gated: BN / 2 of each B), waves WM x WN, K-steps of 128 bytes.  Both
+// tiles go straight from memory to LDS (global_load_lds, 16 bytes a lane, no registers), one step
+// ahead of the MFMAs, in two buffers that are separate arrays so that the compiler's waits for one
+// do not cover the other.
+//
+// LDS rows are 128 bytes; piece c of row r lies at c ^ ((r >> 1) & 7), so that the 16 rows of an MFMA
+// operand fall on all 64 banks.  The order of B's rows in LDS is chosen so that a lane ends with 16
+// (gated: 8) consecutive columns of its row of C: slot 16 j + i of a wave's 64 holds column
+// 16 (i / 4) + 4 j + i % 4.
+template <int BM, int BN, int WM, int WN, bool kGated>
+struct TileShape {
+  static constexpr int kThreads = WM * WN * kWave;
+  static constexpr int kRowsM = BM / WM;             // rows of C a wave computes
+  static constexpr int kColsN = BN / WN;             // slots of B
+  static_assert(kColsN == 64, "the column order is written for 64 slots a wave");
+  static constexpr int kMI = kRowsM / 16, kNI = kColsN / 16;
+  static constexpr int kLoadA = BM * 128 / 16 / kThreads, kLoadB = BN * 128 / 16 / kThreads;
+  static constexpr int kColsOut = kGated ? BN / 2 : BN;
+};
+
+// column (within the block's) that B slot s holds, and which B
+template <bool kGated>
+__device__ inline int slot_column(int s, int* which) {
+  const int wn = s >> 6, j = (s >> 4) & 3, i = s & 15;
+  if constexpr (kGated) {
+    *which = j >> 1;
+    return wn * 32 + (i >> 2) * 8 + (j & 1) * 4 + (i & 3);
+  }
+  *which = 0;
+  return wn * 64 + (i >> 2) * 16 + j * 4 + (i & 3);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool kGated>
+__global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tiles_m, int tiles_n) {
+  using S = TileShape<BM, BN, WM, WN, kGated>;
+  using Acc = typename Mma<T>::Acc;
+  __shared__ __attribute__((aligned(1024))) char a_lds0[BM * 128];
+  __shared__ __attribute__((aligned(1024))) char b_lds0[BN * 128];
+  __shared__ __attribute__((aligned(1024))) char a_lds1[BM * 128];
+  __shared__ __attribute__((aligned(1024))) char b_lds1[BN * 128];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  // tiles: each XCD (blockIdx modulo 8) takes a contiguous run of them, and a run goes down groups of
+  // 8 tile rows, so that an XCD's L2 holds the operands that its blocks share
+  const int total = tiles_m * tiles_n;
+  int tile = blockIdx.x;
+  {
+    const int per = total / 8, rest = total % 8, xcd = tile % 8, at = tile / 8;
+    tile = xcd * per + (xcd < rest ? xcd : rest) + at;
+  }
+  constexpr int kGroup = 8;
+  const int group = tile / (kGroup * tiles_n);
+  const int first_m = group * kGroup;
+  const int rows_g = tiles_m - first_m < kGroup ? tiles_m - first_m : kGroup;
+  const int in_g = tile - group * kGroup * tiles_n;
+  const int tm = first_m + in_g % rows_g, tn = in_g / rows_g;
+  const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * S::kColsOut;
+
+  // a lane's pieces: row (of 8 a wave and load) and piece of the row, permuted as LDS holds them
+  const int piece_row = lane >> 3;
+  const char* ga[S::kLoadA];
+  const char* gb[S::kLoadB];
+  int ka[S::kLoadA], kb[S::kLoadB];
+  constexpr int kRowsLoad = S::kThreads / 8;        // rows a load of the whole block fills
+#pragma unroll
+  for (int j = 0; j < S::kLoadA; ++j) {
+    const int r = j * kRowsLoad + wave * 8 + piece_row;
+    ka[j] = ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    const int64_t row = m0 + r < p.m ? m0 + r : p.m - 1;     // rows behind the last: their outputs are not stored
+    ga[j] = p.a + row * p.lda + ka[j];
+  }
+#pragma unroll
+  for (int j = 0; j < S::kLoadB; ++j) {
+    const int r = j * kRowsLoad + wave * 8 + piece_row;
+    kb[j] = ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    int which;
+    const int64_t col = n0 + slot_column<kGated>(r, &which);
+    const int64_t row = col < p.n ? col : p.n - 1;
+    gb[j] = (which ? p.b1 + row * p.ldb1 : p.b0 + row * p.ldb0) + kb[j];
+  }
+  const char* zero = reinterpret_cast<const char*>(&kZeroPiece);
+  auto fetch = [&](char* a_lds, char* b_lds, int64_t k0) {
+    const int64_t left = p.kbytes - k0;
+    if (left >= 128) {
+#pragma unroll
+      for (int j = 0; j < S::kLoadA; ++j)
+        __builtin_amdgcn_global_load_lds((gptr_t)(ga[j] + k0), (lptr_t)(a_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
+#pragma unroll
+      for (int j = 0; j < S::kLoadB; ++j)
+        __builtin_amdgcn_global_load_lds((gptr_t)(gb[j] + k0), (lptr_t)(b_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < S::kLoadA; ++j)
+        __builtin_amdgcn_global_load_lds((gptr_t)(ka[j] < left ? ga[j] + k0 : zero),
+                                         (lptr_t)(a_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
+#pragma unroll
+      for (int j = 0; j < S::kLoadB; ++j)
+        __builtin_amdgcn_global_load_lds((gptr_t)(kb[j] < left ? gb[j] + k0 : zero),
+                                         (lptr_t)(b_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
+    }
+  };
+
+  Acc acc[S::kMI][S::kNI];
+#pragma unroll
+  for (int i = 0; i < S::kMI; ++i)
+#pragma unroll
+    for (int j = 0; j < S::kNI; ++j) acc[i][j] = Acc{};
+  const int wm = wave / WN, wn = wave % WN;
+  const int l15 = lane & 15, q = lane >> 4, swz = (l15 >> 1) & 7;
+  const int a_row = (wm * S::kRowsM + l15) * 128, b_row = (wn * 64 + l15) * 128;
+  auto multiply = [&](const char* a_lds, const char* b_lds) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int piece = ((h * 4 + q) ^ swz) * 16;
+      i32x4 a[S::kMI], b[S::kNI];
+#pragma unroll
+      for (int j = 0; j < S::kNI; ++j) b[j] = *reinterpret_cast<const i32x4*>(b_lds + b_row + j * 2048 + piece);
+#pragma unroll
+      for (int i = 0; i < S::kMI; ++i) a[i] = *reinterpret_cast<const i32x4*>(a_lds + a_row + i * 2048 + piece);
+#pragma unroll
+      for (int i = 0; i < S::kMI; ++i)
+#pragma unroll
+        for (int j = 0; j < S::kNI; ++j) acc[i][j] = Mma<T>::mma(b[j], a[i], acc[i][j]);
+    }
+  };
+
+  const int64_t steps = (p.kbytes + 127) / 128;
+  fetch(a_lds0, b_lds0, 0);
+  __syncthreads();
+  for (int64_t s = 0; s < steps; s += 2) {
+    if (s + 1 < steps) fetch(a_lds1, b_lds1, (s + 1) * 128);
+    multiply(a_lds0, b_lds0);
+    __syncthreads();
+    if (s + 1 >= steps) break;
+    if (s + 2 < steps) fetch(a_lds0, b_lds0, (s + 2) * 128);
+    multiply(a_lds1, b_lds1);
+    __syncthreads();
+  }
+
+  // C^T layout of the MFMA (B's rows are its first operand): lane l holds row l & 15, and of slot
+  // group j columns 4 (l >> 4) + 0..3, which the slot order makes consecutive over j
+  using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
+#pragma unroll
+  for (int i = 0; i < S::kMI; ++i) {
+    const int64_t row = m0 + wm * S::kRowsM + i * 16 + l15;
+    if constexpr (kGated) {
+      E g[8], u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        g[e] = acc[i][e >> 2][e & 3];
+        u[e] = acc[i][2 + (e >> 2)][e & 3];
+      }
+      finish_gated<T, 8>(p, row, n0 + wn * 32 + q * 8, g, u);
+    } else {
+      E c[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) c[e] = acc[i][e >> 2][e & 3];
+      finish<T, 16>(p, row, n0 + wn * 64 + q * 16, c);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- few rows
+// Up to 16 * MT rows of A against the whole of B: B is read once, straight into the registers that
+// the MFMAs take, so the kernel is as fast as B's bytes arrive.  A block owns 16 columns (gated: 16 of
+// each B); its waves take k in runs of 256 bytes in turn and add their sums in LDS, in wave order.
+constexpr int kFewWaves = 8;
+
+template <typename T, int MT, bool kGated>
+__global__ void __launch_bounds__(kFewWaves* kWave) few_rows_kernel(Product p) {
+  using Acc = typename Mma<T>::Acc;
+  constexpr int NB = kGated ? 2 : 1;
+  __shared__ Acc lds[kFewWaves][MT * NB][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int l15 = lane & 15, q = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
+  const int64_t col = n0 + l15 < p.n ? n0 + l15 : p.n - 1;
+  const char* b[NB];
+  b[0] = p.b0 + col * p.ldb0 + q * 16;
+  if constexpr (kGated) b[1] = p.b1 + col * p.ldb1 + q * 16;
+  const char* a[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t row = m0 + i * 16 + l15 < p.m ? m0 + i * 16 + l15 : p.m - 1;
+    a[i] = p.a + row * p.lda + q * 16;
+  }
+  Acc acc[MT][NB];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = Acc{};
+  const i32x4 none = {0, 0, 0, 0};
+  // four pieces of 64 bytes a turn: 256 contiguous bytes of a row, all loads before the first product
+  for (int64_t k = wave * 256; k < p.kbytes; k += kFewWaves * 256) {
+    i32x4 bv[4][NB], av[4][MT];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool in = k + u * 64 + q * 16 < p.kbytes;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) bv[u][j] = in ? *reinterpret_cast<const i32x4*>(b[j] + k + u * 64) : none;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) av[u][i] = in ? *reinterpret_cast<const i32x4*>(a[i] + k + u * 64) : none;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = Mma<T>::mma(bv[u][j], av[u][i], acc[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) lds[wave][i * NB + j][lane] = acc[i][j];
+  __syncthreads();
+  using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
+  for (int i = wave; i < MT; i += kFewWaves) {
+    Acc sum[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      sum[j] = lds[0][i * NB + j][lane];
+#pragma unroll
+      for (int w = 1; w < kFewWaves; ++w) sum[j] += lds[w][i * NB + j][lane];
+    }
+    const int64_t row = m0 + i * 16 + l15, at = n0 + q * 4;
+    E c[4], d[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c[e] = sum[0][e];
+      d[e] = sum[NB - 1][e];
+    }
+    if constexpr (kGated) finish_gated<T, 4>(p, row, at, c, d);
+    else finish<T, 4>(p, row, at, c);
+  }
+}
+
+// ------------------------------------------------------------------------------- launch
+template <typename T, bool kGated>
+int launch_product(const Product& p, hipStream_t stream, const char* what) {
+  const int64_t cus = 256;
+  if (p.m <= 64) {
+    const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), 1);
+    if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
+    else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
+    else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
+  } else {
+    const int64_t big = cdiv(p.m, 256) * cdiv(p.n, kGated ? 128 : 256);
+    if (big >= cus) {
+      const int64_t tm = cdiv(p.m, 256), tn = cdiv(p.n, kGated ? 128 : 256);
+      SAGE_REQUIRE(tm * tn < (int64_t{1} << 31), SAGE_ELIMIT, "%s: too many output tiles", what);
+      hipLaunchKernelGGL((tile_kernel<T, 256, 256, 2, 4, kGated>), dim3(static_cast<unsigned>(tm * tn)), dim3(512), 0, stream, p,
+                         static_cast<int>(tm), static_cast<int>(tn));
+    } else {
+      const int64_t tm = cdiv(p.m, 128), tn = cdiv(p.n, kGated ? 64 : 128);
+      SAGE_REQUIRE(tm * tn < (int64_t{1} << 31), SAGE_ELIMIT, "%s: too many output tiles", what);
+      hipLaunchKernelGGL((tile_kernel<T, 128, 128, 2, 2, kGated>), dim3(static_cast<unsigned>(tm * tn)), dim3(256), 0, stream, p,
+                         static_cast<int>(tm), static_cast<int>(tn));
+    }
+  }
+  SAGE_CHECK_LAUNCH(what);
+  return SAGE_OK;
+}
+
+inline int size_of(int dtype) { return dtype == SAGE_F32 ? 4 : 2; }
+inline bool known_dtype(int d) { return d == SAGE_F32 || d == SAGE_BF16 || d == SAGE_F16; }
+inline bool known_act(int a) { return a == SAGE_ACT_SILU || a == SAGE_ACT_GELU || a == SAGE_ACT_RELU; }
+inline bool rows16(const void* p, int64_t ld_bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld_bytes & 15) == 0 && ld_bytes >= 0;
+}
+
+template <bool kGated>
+int product_by_type(const Product& p, int dtype, hipStream_t stream, const char* what) {
+  if (dtype == SAGE_F32) return launch_product<float, kGated>(p, stream, what);
+  if (dtype == SAGE_BF16) return launch_product<__bf16, kGated>(p, stream, what);
+  return launch_product<_Float16, kGated>(p, stream, what);
+}
+
+// ------------------------------------------------------------------------------- backward pass
+// dg = dh * u * act'(g), du = dh * act(g) for a 64 x 64 piece, each rounded once to the operands' type
+// (the matrix cores take no wider one), written as rows [m, 2 h] for dx and, turned over in LDS, as
+// rows [2 h, m] for the weights' gradients.  Columns between a row's end and its stride are zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) gate_bwd_kernel(const T* dh, int64_t ld_dh, const float* saved, int act, int64_t m,
+                                                       int64_t h, T* rows, int64_t ld_rows, T* cols, int64_t ld_cols) {
+  __shared__ T lds[2][64][65];
+  constexpr bool kExact = std::is_same<T, float>::value;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 64, h0 = static_cast<int64_t>(blockIdx.x) * 64;
+  const int c = threadIdx.x & 63, r0 = threadIdx.x >> 6;
+#pragma unroll 4
+  for (int r = r0; r < 64; r += 4) {
+    const int64_t row = m0 + r, col = h0 + c;
+    T dg = static_cast<T>(0.f), du = static_cast<T>(0.f);
+    if (row < m && col < h) {
+      const float g = saved[row * h + col], u = saved[(m + row) * h + col];
+      const float d = static_cast<float>(dh[row * ld_dh + col]);
+      dg = static_cast<T>(d * u * act_slope<kExact>(g, act));
+      du = static_cast<T>(d * act_value<kExact>(g, act));
+      if (rows != nullptr) {
+        rows[row * ld_rows + col] = dg;
+        rows[row * ld_rows + h + col] = du;
+      }
+    }
+    lds[0][r][c] = dg;
+    lds[1][r][c] = du;
+  }
+  // the padding behind column 2 h of a row
+  if (rows != nullptr && blockIdx.x == gridDim.x - 1 && c < ld_rows - 2 * h)
+    for (int r = r0; r < 64; r += 4)
+      if (m0 + r < m) rows[(m0 + r) * ld_rows + 2 * h + c] = static_cast<T>(0.f);
+  if (cols == nullptr) return;
+  __syncthreads();
+#pragma unroll 4
+  for (int r = r0; r < 64; r += 4) {
+    const int64_t col = h0 + r, row = m0 + c;     // zeros where row >= m
+    if (col < h && row < ld_cols) {
+      cols[col * ld_cols + row] = lds[0][c][r];
+      cols[(h + col) * ld_cols + row] = lds[1][c][r];
+    }
+  }
+}
+
+// out[c, at + r] = in[r, c], zeros for rows between `rows` and `padded`
+template <typename T>
+__global__ void __launch_bounds__(256) transpose_kernel(const T* in, int64_t ld_in, int64_t rows, int64_t cols, T* out,
+                                                        int64_t ld_out, int64_t at, int64_t padded) {
+  __shared__ T lds[64][65];
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, c0 = static_cast<int64_t>(blockIdx.x) * 64;
+  const int x = threadIdx.x & 63, y0 = threadIdx.x >> 6;
+#pragma unroll 4
+  for (int y = y0; y < 64; y += 4)
+    lds[y][x] = r0 + y < rows && c0 + x < cols ? in[(r0 + y) * ld_in + c0 + x] : static_cast<T>(0.f);
+  __syncthreads();
+#pragma unroll 4
+  for (int y = y0; y < 64; y += 4)
+    if (c0 + y < cols && r0 + x < padded) out[(c0 + y) * ld_out + at + r0 + x] = lds[x][y];
+}
+
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint8_t* in, int64_t ld_in, int64_t row_bytes, uint8_t* out,
+                                                       int64_t ld_out, int64_t pieces, int64_t total) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / pieces, at = (i - row * pieces) * 16;
+  const uint8_t* p = in + row * ld_in + at;
+  struct __attribute__((packed, aligned(1))) P {
+    uint8_t v[16];
+  } k;
+  if (at + 16 <= row_bytes) {
+    k = *reinterpret_cast<const P*>(p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) k.v[e] = at + e < row_bytes ? p[e] : 0;
+  }
+  *reinterpret_cast<i32x4*>(out + row * ld_out + at) = __builtin_bit_cast(i32x4, k);
+}
+
+struct BwdLayout {
+  int64_t ld_rows, ld_cols, ld_w;          // in elements
+  size_t rows, cols, xt, wt, bytes;        // offsets
+};
+inline BwdLayout bwd_layout(int64_t m, int64_t h, int64_t k, int dtype) {
+  const int64_t piece = 16 / size_of(dtype);
+  BwdLayout l;
+  l.ld_rows = static_cast<int64_t>(align_up(static_cast<size_t>(2 * h), static_cast<size_t>(piece)));
+  l.ld_cols = static_cast<int64_t>(align_up(static_cast<size_t>(m), static_cast<size_t>(piece)));
+  l.ld_w = l.ld_rows;
+  size_t off = 0;
+  auto take = [&](int64_t elements) {
+    const size_t at = off;
+    off = align_up(off + static_cast<size_t>(elements) * size_of(dtype), 256);
+    return at;
+  };
+  l.rows = take(m * l.ld_rows);
+  l.cols = take(2 * h * l.ld_cols);
+  l.xt = take(k * l.ld_cols);
+  l.wt = take(k * l.ld_w);
+  l.bytes = off;
+  return l;
+}
+
+template <typename T>
+int gated_bwd(const void* dh, int64_t ld_dh, const void* x, int64_t ld_x, const void* wg, int64_t ld_g, const void* wu,
+              int64_t ld_u, const float* saved, int act, int64_t m, int64_t h, int64_t k, int dtype, void* dx,
+              int64_t ld_dx, void* dw, char* ws, hipStream_t st, const char* what) {
+  const BwdLayout l = bwd_layout(m, h, k, dtype);
+  T* rows = reinterpret_cast<T*>(ws + l.rows);
+  T* cols = reinterpret_cast<T*>(ws + l.cols);
+  T* xt = reinterpret_cast<T*>(ws + l.xt);
+  T* wt = reinterpret_cast<T*>(ws + l.wt);
+  auto grid64 = [](int64_t c, int64_t r) { return dim3(static_cast<unsigned>(cdiv(c, 64)), static_cast<unsigned>(cdiv(r, 64))); };
+  hipLaunchKernelGGL((gate_bwd_kernel<T>), grid64(h, m), dim3(256), 0, st, static_cast<const T*>(dh), ld_dh, saved, act, m, h,
+                     dx != nullptr ? rows : nullptr, l.ld_rows, dw != nullptr ? cols : nullptr, l.ld_cols);
+  SAGE_CHECK_LAUNCH(what);
+  if (dx != nullptr) {
+    // [k, 2 h]: the rows of B for dx[m, k] = sum over both halves of dgu[m, :] w[:, k]
+    hipLaunchKernelGGL((transpose_kernel<T>), grid64(k, h), dim3(256), 0, st, static_cast<const T*>(wg), ld_g, h, k, wt, l.ld_w,
+                       int64_t{0}, h);
+    SAGE_CHECK_LAUNCH(what);
+    hipLaunchKernelGGL((transpose_kernel<T>), grid64(k, l.ld_w - h), dim3(256), 0, st, static_cast<const T*>(wu), ld_u, h, k, wt,
+                       l.ld_w, h, l.ld_w - h);
+    SAGE_CHECK_LAUNCH(what);
+    Product p{};
+    p.a = reinterpret_cast<const char*>(rows); p.lda = l.ld_rows * sizeof(T);
+    p.b0 = reinterpret_cast<const char*>(wt); p.ldb0 = l.ld_w * sizeof(T);
+    p.m = m; p.n = k; p.kbytes = l.ld_rows * sizeof(T);
+    p.out = dx; p.ldo = ld_dx; p.out_dtype = dtype;
+    const int rc = launch_product<T, false>(p, st, what);
+    if (rc != SAGE_OK) return rc;
+  }
+  if (dw != nullptr) {
+    hipLaunchKernelGGL((transpose_kernel<T>), grid64(k, l.ld_cols), dim3(256), 0, st, static_cast<const T*>(x), ld_x, m, k, xt,
+                       l.ld_cols, int64_t{0}, l.ld_cols);
+    SAGE_CHECK_LAUNCH(what);
+    Product p{};
+    p.a = reinterpret_cast<const char*>(cols); p.lda = l.ld_cols * sizeof(T);
+    p.b0 = reinterpret_cast<const char*>(xt); p.ldb0 = l.ld_cols * sizeof(T);
+    p.m = 2 * h; p.n = k; p.kbytes = l.ld_cols * sizeof(T);
+    p.out = dw; p.ldo = k; p.out_dtype = dtype;
+    return launch_product<T, false>(p, st, what);
+  }
+  return SAGE_OK;
+}
+
+}  // namespace
+}  // namespace sage
+
+using namespace sage;
+
+extern "C" int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows, sage_i64 row_bytes, void* out,
+                             sage_i64 ld_out_bytes, void* stream) {
+  SAGE_REQUIRE(rows >= 0 && row_bytes > 0, SAGE_EINVAL, "sage_pad_rows: bad shape [%ld, %ld]", (long)rows, (long)row_bytes);
+  if (rows == 0) return SAGE_OK;
+  SAGE_REQUIRE(in != nullptr && out != nullptr, SAGE_EINVAL, "sage_pad_rows: NULL pointer");
+  SAGE_REQUIRE(rows16(out, ld_out_bytes) && ld_out_bytes >= row_bytes && ld_in_bytes >= 0, SAGE_EINVAL,
+               "sage_pad_rows: output rows start on 16 bytes and hold the input's");
+  const int64_t pieces = cdiv(row_bytes, 16), total = rows * pieces;
+  SAGE_REQUIRE(cdiv(total, 256) < (int64_t{1} << 31), SAGE_ELIMIT, "sage_pad_rows: %ld rows of %ld bytes", (long)rows, (long)row_bytes);
+  hipLaunchKernelGGL(pad_rows_kernel, dim3(static_cast<unsigned>(cdiv(total, 256))), dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const uint8_t*>(in), ld_in_bytes, row_bytes, static_cast<uint8_t*>(out), ld_out_bytes, pieces, total);
+  SAGE_CHECK_LAUNCH("sage_pad_rows");
+  return SAGE_OK;
+}
+
+#define SAGE_INT8_CHECKS(what)                                                                                          \
+  SAGE_REQUIRE(known_dtype(out_dtype), SAGE_EINVAL, what ": unknown output dtype %d", out_dtype);                       \
+  SAGE_REQUIRE(m >= 0 && n > 0 && k > 0, SAGE_EINVAL, what ": bad shape m %ld n %ld k %ld", (long)m, (long)n, (long)k); \
+  SAGE_REQUIRE(k <= SAGE_INT8_MAX_K, SAGE_ELIMIT, what ": k = %ld: a sum of k products could leave 32 bits", (long)k)
+
+extern "C" int sage_int8_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w, sage_i64 ld_w,
+                                const float* w_scale, const float* bias, sage_i64 m, sage_i64 n, sage_i64 k, int out_dtype,
+                                void* out, sage_i64 ld_out, void* stream) {
+  SAGE_INT8_CHECKS("sage_int8_linear");
+  if (m == 0) return SAGE_OK;
+  SAGE_REQUIRE(x && x_scale && w && w_scale && out, SAGE_EINVAL, "sage_int8_linear: NULL pointer");
+  SAGE_REQUIRE(k % 16 == 0 && rows16(x, ld_x) && rows16(w, ld_w) && ld_out >= n, SAGE_EINVAL,
+               "sage_int8_linear: rows are whole pieces of 16 bytes (sage_pad_rows) and outputs do not overlap");
+  Product p{};
+  p.a = reinterpret_cast<const char*>(x); p.lda = ld_x;
+  p.b0 = reinterpret_cast<const char*>(w); p.ldb0 = ld_w;
+  p.m = m; p.n = n; p.kbytes = k;
+  p.out = out; p.ldo = ld_out; p.out_dtype = out_dtype;
+  p.sa = x_scale; p.sb0 = w_scale; p.bias = bias;
+  return launch_product<int8_t, false>(p, static_cast<hipStream_t>(stream), "sage_int8_linear");
+}
+
+extern "C" int sage_int8_gated_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w_gate, sage_i64 ld_g,
+                                      const float* gate_scale, const int8_t* w_up, sage_i64 ld_u, const float* up_scale,
+                                      int activation, sage_i64 m, sage_i64 n, sage_i64 k, int out_dtype, void* out,
+                                      sage_i64 ld_out, void* stream) {
+  SAGE_INT8_CHECKS("sage_int8_gated_linear");
+  SAGE_REQUIRE(known_act(activation), SAGE_EINVAL, "sage_int8_gated_linear: unknown activation %d", activation);
+  if (m == 0) return SAGE_OK;
+  SAGE_REQUIRE(x && x_scale && w_gate && gate_scale && w_up && up_scale && out, SAGE_EINVAL, "sage_int8_gated_linear: NULL pointer");
+  SAGE_REQUIRE(k % 16 == 0 && rows16(x, ld_x) && rows16(w_gate, ld_g) && rows16(w_up, ld_u) && ld_out >= n, SAGE_EINVAL,
+               "sage_int8_gated_linear: rows are whole pieces of 16 bytes (sage_pad_rows) and outputs do not overlap");
+  Product p{};
+  p.a = reinterpret_cast<const char*>(x); p.lda = ld_x;
+  p.b0 = reinterpret_cast<const char*>(w_gate); p.ldb0 = ld_g;
+  p.b1 = reinterpret_cast<const char*>(w_up); p.ldb1 = ld_u;
+  p.m = m; p.n = n; p.kbytes = k;
+  p.out = out; p.ldo = ld_out; p.out_dtype = out_dtype; p.act = activation;
+  p.sa = x_scale; p.sb0 = gate_scale; p.sb1 = up_scale;
+  return launch_product<int8_t, true>(p, static_cast<hipStream_t>(stream), "sage_int8_gated_linear");
+}
+
+extern "C" int sage_gated_linear_fwd(const void* x, sage_i64 ld_x, const void* w_gate, sage_i64 ld_g, const void* w_up,
+                                     sage_i64 ld_u, int activation, sage_i64 m, sage_i64 h, sage_i64 k, int dtype, void* out,
+                                     sage_i64 ld_out, float* saved, void* stream) {
+  SAGE_REQUIRE(known_dtype(dtype), SAGE_EINVAL, "sage_gated_linear_fwd: unknown dtype %d", dtype);
+  SAGE_REQUIRE(known_act(activation), SAGE_EINVAL, "sage_gated_linear_fwd: unknown activation %d", activation);
+  SAGE_REQUIRE(m >= 0 && h > 0 && k > 0, SAGE_EINVAL, "sage_gated_linear_fwd: bad shape m %ld h %ld k %ld", (long)m, (long)h, (long)k);
+  if (m == 0) return SAGE_OK;
+  SAGE_REQUIRE(x && w_gate && w_up && out, SAGE_EINVAL, "sage_gated_linear_fwd: NULL pointer");
+  const int size = size_of(dtype);
+  SAGE_REQUIRE(k * size % 16 == 0 && rows16(x, ld_x * size) && rows16(w_gate, ld_g * size) && rows16(w_up, ld_u * size) && ld_out >= h,
+               SAGE_EINVAL, "sage_gated_linear_fwd: rows are whole pieces of 16 bytes (sage_pad_rows) and outputs do not overlap");
+  Product p{};
+  p.a = static_cast<const char*>(x); p.lda = ld_x * size;
+  p.b0 = static_cast<const char*>(w_gate); p.ldb0 = ld_g * size;
+  p.b1 = static_cast<const char*>(w_up); p.ldb1 = ld_u * size;
+  p.m = m; p.n = h; p.kbytes = k * size;
+  p.out = out; p.ldo = ld_out; p.out_dtype = dtype; p.act = activation; p.saved = saved;
+  return product_by_type<true>(p, dtype, static_cast<hipStream_t>(stream), "sage_gated_linear_fwd");
+}
+
+extern "C" size_t sage_gated_linear_bwd_workspace_bytes(sage_i64 m, sage_i64 h, sage_i64 k, int dtype) {
+  if (m <= 0 || h <= 0 || k <= 0 || !known_dtype(dtype)) return 0;
+  return bwd_layout(m, h, k, dtype).bytes;
+}
+
+extern "C" int sage_gated_linear_bwd(const void* dh, sage_i64 ld_dh, const void* x, sage_i64 ld_x, const void* w_gate,
+                                     sage_i64 ld_g, const void* w_up, sage_i64 ld_u, const float* saved, int activation,
+                                     sage_i64 m, sage_i64 h, sage_i64 k, int dtype, void* dx, sage_i64 ld_dx, void* dw,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  SAGE_REQUIRE(known_dtype(dtype), SAGE_EINVAL, "sage_gated_linear_bwd: unknown dtype %d", dtype);
+  SAGE_REQUIRE(known_act(activation), SAGE_EINVAL, "sage_gated_linear_bwd: unknown activation %d", activation);
+  SAGE_REQUIRE(m > 0 && h > 0 && k > 0, SAGE_EINVAL, "sage_gated_linear_bwd: bad shape m %ld h %ld k %ld", (long)m, (long)h, (long)k);
+  SAGE_REQUIRE(dh && x && w_gate && w_up && saved && (dx || dw), SAGE_EINVAL, "sage_gated_linear_bwd: NULL pointer");
+  SAGE_REQUIRE(ld_dh >= 0 && ld_x >= 0 && ld_g >= 0 && ld_u >= 0 && (dx == nullptr || ld_dx >= k), SAGE_EINVAL,
+               "sage_gated_linear_bwd: row stride below the width");
+  SAGE_REQUIRE(cdiv(m, 64) < 65536 && cdiv(2 * h, 64) < 65536, SAGE_ELIMIT, "sage_gated_linear_bwd: m %ld h %ld", (long)m, (long)h);
+  SAGE_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
+                   workspace_bytes >= sage_gated_linear_bwd_workspace_bytes(m, h, k, dtype),
+               SAGE_EWORKSPACE, "sage_gated_linear_bwd: workspace of %zu bytes", workspace_bytes);
+  char* ws = static_cast<char*>(workspace);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const char* what = "sage_gated_linear_bwd";
+  if (dtype == SAGE_F32)
+    return gated_bwd<float>(dh, ld_dh, x, ld_x, w_gate, ld_g, w_up, ld_u, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
+  if (dtype == SAGE_BF16)
+    return gated_bwd<__bf16>(dh, ld_dh, x, ld_x, w_gate, ld_g, w_up, ld_u, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
+  return gated_bwd<_Float16>(dh, ld_dh, x, ld_x, w_gate, ld_g, w_up, ld_u, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
+}

@@ -1326,3 +1326,286 @@ def lstm_pad_grad_bcast(g, num_features, j0, j1, dw):
     rc = lib.sage_lstm_pad_grad_bcast(gp, ld_g, dw.size(0), F, int(j0), int(j1), dp, ld_d, _stream())
     _lib.check(rc, "sage_lstm_pad_grad_bcast")
     return dw
+
+
+# ------------------------------------------------------------------------------- feed-forward block
+# Norm with the residual's addition, 8-bit and gated products: fp32, bf16 and fp16 rows.  Each call
+# runs on the current stream of its tensors' device, whichever device is the current one.
+ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
+
+
+def _call(name, device, *args):
+    lib = _lib.load()
+    if device.index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def _row_matrix(t, name, dtype=None, shape=None, device=None, output=False):
+    """2-D device matrix with contiguous rows -> (pointer, row stride in elements)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name}: expected a CUDA (HIP) tensor; graphsage_amd has no CPU path")
+    if t.dim() != 2:
+        raise RuntimeError(f"{name}: expected a 2-D tensor, got shape {tuple(t.shape)}")
+    if dtype is None:
+        if t.dtype not in ROW_DTYPES:
+            raise RuntimeError(f"{name}: expected fp32, bf16 or fp16, got {t.dtype}")
+    elif t.dtype != dtype:
+        raise RuntimeError(f"{name}: expected dtype {dtype}, got {t.dtype}")
+    rows, cols = t.shape
+    if shape is not None and (rows, cols) != shape:
+        raise RuntimeError(f"{name}: expected shape {list(shape)}, got {[rows, cols]}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name}: on {t.device}, the other operands on {device}")
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1:
+        raise RuntimeError(f"{name}: expected contiguous rows, got strides {t.stride()}")
+    if rows <= 1:
+        ld = max(ld, cols)
+    if output and ld < cols:
+        raise RuntimeError(f"{name}: the rows of an output must not overlap")
+    return t.data_ptr(), ld
+
+
+def _vector(t, name, n, device, dtypes=(torch.float32,)):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name}: expected a CUDA (HIP) tensor; graphsage_amd has no CPU path")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name}: expected dtype {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+        raise RuntimeError(f"{name}: expected {n} contiguous elements, got shape {tuple(t.shape)}")
+    if t.device != device:
+        raise RuntimeError(f"{name}: on {t.device}, the other operands on {device}")
+    return t.data_ptr()
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise RuntimeError(f"activation {name!r}: one of {sorted(ACTIVATIONS)}")
+    return ACTIVATIONS[name]
+
+
+def _norm_inputs(x, weight, residual, what):
+    px, ldx = _row_matrix(x, f"{what}: x")
+    shape, dev = tuple(x.shape), x.device
+    if shape[1] == 0:
+        raise RuntimeError(f"{what}: rows of no elements")
+    pr, ldr = (None, 0) if residual is None else _row_matrix(residual, f"{what}: residual", x.dtype, shape, dev)
+    pw = None if weight is None else _vector(weight, f"{what}: weight", shape[1], dev, (x.dtype, torch.float32))
+    wd = ROW_DTYPES[x.dtype if weight is None else weight.dtype]
+    return px, ldx, pr, ldr, pw, wd, shape, dev
+
+
+def _output(out, name, shape, dtype, device):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return out
+
+
+def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out=None, sum_out=None):
+    """s = x + residual; y = s / sqrt(mean(s^2) + eps) * weight over each row of x [rows, dim]
+    (fp32 / bf16 / fp16; weight in x's dtype or fp32).  Returns (y, s); without a residual s is x
+    itself.  sum_out may be `residual` (the residual stream updated in place)."""
+    px, ldx, pr, ldr, pw, wd, shape, dev = _norm_inputs(x, weight, residual, "rms_norm_fwd")
+    if weight is None:
+        raise RuntimeError("rms_norm_fwd: weight: tensor required")
+    y = _output(out, "out", shape, x.dtype, dev)
+    py, ldy = _row_matrix(y, "rms_norm_fwd: out", x.dtype, shape, dev, output=True)
+    ps, lds, s = None, 0, x
+    if residual is not None:
+        s = _output(sum_out, "sum_out", shape, x.dtype, dev)
+        ps, lds = _row_matrix(s, "rms_norm_fwd: sum_out", x.dtype, shape, dev, output=True)
+    elif sum_out is not None:
+        raise RuntimeError("rms_norm_fwd: sum_out without a residual")
+    _call("sage_rms_norm_fwd", dev, px, ldx, pr, ldr, pw, wd, shape[0], shape[1], ROW_DTYPES[x.dtype], eps,
+          py, ldy, ps, lds)
+    return y, s
+
+
+def _int8_rows(x, weight, residual, eps, normalise, padded, sum_out, what):
+    px, ldx, pr, ldr, pw, wd, shape, dev = _norm_inputs(x, weight, residual, what)
+    rows, dim = shape
+    wide = (dim + 15) // 16 * 16
+    q = torch.empty((rows, wide), dtype=torch.int8, device=dev)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    ps, lds, s = None, 0, x
+    if residual is not None:
+        s = _output(sum_out, "sum_out", shape, x.dtype, dev)
+        ps, lds = _row_matrix(s, f"{what}: sum_out", x.dtype, shape, dev, output=True)
+    elif sum_out is not None:
+        raise RuntimeError(f"{what}: sum_out without a residual")
+    _call("sage_rms_norm_int8", dev, px, ldx, pr, ldr, pw, wd, rows, dim, ROW_DTYPES[x.dtype], eps, normalise,
+          q.data_ptr(), wide, wide, scale.data_ptr(), ps, lds)
+    return (q if padded or wide == dim else q[:, :dim]), scale, s
+
+
+def rms_norm_int8(x, weight, residual=None, eps=1e-6, padded=False, sum_out=None):
+    """rms_norm_fwd with an 8-bit output: (q int8 [rows, dim], scale fp32 [rows], s), y = q * scale.
+    A row of zeros has scale 0; a row with an infinity or NaN has scale NaN.  padded: q's rows keep
+    the zeros that fill them to whole pieces of 16 bytes ([rows, dim rounded up to 16]), so that an
+    8-bit product with weights padded alike takes them as they are."""
+    if weight is None:
+        raise RuntimeError("rms_norm_int8: weight: tensor required")
+    return _int8_rows(x, weight, residual, eps, 1, padded, sum_out, "rms_norm_int8")
+
+
+def quantize_rows(x, padded=False):
+    """(q int8, scale fp32 [rows]) with x ~ q * scale: each row by its largest magnitude over 127."""
+    return _int8_rows(x, None, None, 0.0, 0, padded, None, "quantize_rows")[:2]
+
+
+def dequantize_rows(q, scale, dtype=torch.float32, out=None):
+    """q * scale[:, None] in `dtype` (rounded once)."""
+    pq, ldq = _row_matrix(q, "dequantize_rows: q", torch.int8)
+    shape, dev = tuple(q.shape), q.device
+    if dtype not in ROW_DTYPES:
+        raise RuntimeError(f"dequantize_rows: expected fp32, bf16 or fp16, got {dtype}")
+    if shape[1] == 0:
+        raise RuntimeError("dequantize_rows: rows of no elements")
+    ps = _vector(scale, "dequantize_rows: scale", shape[0], dev)
+    out = _output(out, "out", shape, dtype, dev)
+    po, ldo = _row_matrix(out, "dequantize_rows: out", dtype, shape, dev, output=True)
+    _call("sage_dequantize_rows", dev, pq, ldq, ps, shape[0], shape[1], ROW_DTYPES[dtype], po, ldo)
+    return out
+
+
+def rms_norm_bwd(dy, s, weight, eps=1e-6, dsum=None, need_dx=True, need_dw=True):
+    """Backward of rms_norm_fwd from the stored sum s: (dx, dweight).  dx is the gradient of x and of
+    the residual alike; dsum is the gradient that reaches s over the residual stream."""
+    ps, lds, pd, ldd, pw, wd, shape, dev = _norm_inputs(s, weight, dsum, "rms_norm_bwd")
+    if weight is None or not (need_dx or need_dw):
+        raise RuntimeError("rms_norm_bwd: a weight, and a gradient to compute")
+    py, ldy = _row_matrix(dy, "rms_norm_bwd: dy", s.dtype, shape, dev)
+    dx = torch.empty(shape, dtype=s.dtype, device=dev) if need_dx else None
+    if shape[0] == 0:
+        return dx, torch.zeros_like(weight) if need_dw else None
+    dw = ws = None
+    ws_bytes = 0
+    if need_dw:
+        dw = torch.empty_like(weight)
+        ws_bytes = _lib.load().sage_rms_norm_bwd_workspace_bytes(shape[0], shape[1], ROW_DTYPES[s.dtype])
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call("sage_rms_norm_bwd", dev, py, ldy, ps, lds, pw, wd, pd, ldd, shape[0], shape[1], ROW_DTYPES[s.dtype], eps,
+          dx.data_ptr() if need_dx else None, shape[1], dw.data_ptr() if need_dw else None,
+          ws.data_ptr() if need_dw else None, ws_bytes)
+    return dx, dw
+
+
+def _pieces(t, p, ld):
+    """The matrix itself if its rows are whole pieces of 16 bytes that start on 16 bytes, else a
+    zero-filled copy that is: (pointer, row stride in elements, columns, what must stay alive)."""
+    size, (rows, cols) = t.element_size(), t.shape
+    if p % 16 == 0 and ld * size % 16 == 0 and cols * size % 16 == 0:
+        return p, ld, cols, t
+    each = 16 // size
+    wide = (cols + each - 1) // each * each
+    out = torch.empty((rows, wide), dtype=t.dtype, device=t.device)
+    _call("sage_pad_rows", t.device, p, ld * size, rows, cols * size, out.data_ptr(), wide * size)
+    return out.data_ptr(), wide, wide, out
+
+
+def _int8_operand(q, scale, name, k=None, device=None):
+    p, ld = _row_matrix(q, name, torch.int8, None, device)
+    if q.size(1) == 0 or (k is not None and q.size(1) != k):
+        raise RuntimeError(f"{name}: expected rows of {k if k else 'some'} elements, got {q.size(1)}")
+    ps = _vector(scale, f"{name} scale", q.size(0), q.device)
+    return p, ld, ps
+
+
+def _int8_product(name, x, x_scale, weights, extra, out_dtype, out):
+    if out_dtype not in ROW_DTYPES:
+        raise RuntimeError(f"{name}: output in fp32, bf16 or fp16, not {out_dtype}")
+    px, ldx, psx = _int8_operand(x, x_scale, f"{name}: x")
+    (m, k), dev = x.shape, x.device
+    n = weights[0][0].size(0)
+    given = []
+    for w, scale in weights:
+        pw, ldw, psw = _int8_operand(w, scale, f"{name}: weight", k, dev)
+        if w.size(0) != n or n == 0:
+            raise RuntimeError(f"{name}: weights of {w.size(0)} rows")
+        given.append((w, pw, ldw, psw))
+    out = _output(out, "out", (m, n), out_dtype, dev)
+    po, ldo = _row_matrix(out, f"{name}: out", out_dtype, (m, n), dev, output=True)
+    if m == 0:
+        return out
+    px, ldx, wide, keep = _pieces(x, px, ldx)
+    args, kept = [], [keep]
+    for w, pw, ldw, psw in given:
+        pw, ldw, _, keep = _pieces(w, pw, ldw)
+        args += [pw, ldw, psw]
+        kept.append(keep)
+    _call(f"sage_{name}", dev, px, ldx, psx, *args, extra(n, dev), m, n, wide, ROW_DTYPES[out_dtype], po, ldo)
+    return out
+
+
+def int8_linear(x, x_scale, weight, w_scale, bias=None, out_dtype=torch.float32, out=None):
+    """out[m, n] = x_scale[m] * w_scale[n] * (x @ weight^T)[m, n] + bias[n] for int8 x [m, k] and weight
+    [n, k] (k <= 131056: the integer sum is exact), fp32 scales and bias."""
+    return _int8_product("int8_linear", x, x_scale, [(weight, w_scale)],
+                         lambda n, dev: None if bias is None else _vector(bias, "int8_linear: bias", n, dev), out_dtype, out)
+
+
+def int8_gated_linear(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation="silu", out_dtype=torch.float32, out=None):
+    """activation(x @ w_gate^T) * (x @ w_up^T), both 8-bit products with token and channel scales."""
+    act = _activation(activation)
+    return _int8_product("int8_gated_linear", x, x_scale, [(w_gate, gate_scale), (w_up, up_scale)], lambda n, dev: act,
+                         out_dtype, out)
+
+
+def _gated_inputs(x, w_gate, w_up, what):
+    px, ldx = _row_matrix(x, f"{what}: x")
+    (m, k), dev = x.shape, x.device
+    pg, ldg = _row_matrix(w_gate, f"{what}: w_gate", x.dtype, (w_gate.size(0), k) if isinstance(w_gate, torch.Tensor) else None, dev)
+    h = w_gate.size(0)
+    pu, ldu = _row_matrix(w_up, f"{what}: w_up", x.dtype, (h, k), dev)
+    if h == 0 or k == 0:
+        raise RuntimeError(f"{what}: weights of shape {[h, k]}")
+    return px, ldx, pg, ldg, pu, ldu, m, h, k, dev
+
+
+def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
+    """activation(x @ w_gate^T) * (x @ w_up^T) for x [m, k], weights [h, k] of one dtype (fp32 / bf16 /
+    fp16; fp32 sums).  Returns (out [m, h], saved): with save, saved [2, m, h] holds both products in
+    fp32 for gated_linear_bwd, else None."""
+    px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up, "gated_linear_fwd")
+    act = _activation(activation)
+    out = _output(out, "out", (m, h), x.dtype, dev)
+    po, ldo = _row_matrix(out, "gated_linear_fwd: out", x.dtype, (m, h), dev, output=True)
+    saved = torch.empty((2, m, h), dtype=torch.float32, device=dev) if save else None
+    if m == 0:
+        return out, saved
+    px, ldx, wide, keep_x = _pieces(x, px, ldx)
+    pg, ldg, _, keep_g = _pieces(w_gate, pg, ldg)
+    pu, ldu, _, keep_u = _pieces(w_up, pu, ldu)
+    _call("sage_gated_linear_fwd", dev, px, ldx, pg, ldg, pu, ldu, act, m, h, wide, ROW_DTYPES[x.dtype], po, ldo,
+          saved.data_ptr() if save else None)
+    return out, saved
+
+
+def gated_linear_bwd(dh, x, w_gate, w_up, saved, activation="silu", need_dx=True, need_dw=True):
+    """Gradients of gated_linear_fwd: (dx, dw_gate, dw_up); the two weight gradients are the halves of
+    one [2 h, k] buffer."""
+    px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up, "gated_linear_bwd")
+    act = _activation(activation)
+    pd, ldd = _row_matrix(dh, "gated_linear_bwd: dh", x.dtype, (m, h), dev)
+    if not isinstance(saved, torch.Tensor) or saved.shape != (2, m, h) or saved.dtype != torch.float32 or \
+            not saved.is_contiguous() or saved.device != dev:
+        raise RuntimeError(f"gated_linear_bwd: saved: expected what gated_linear_fwd(save=True) returned, fp32 {[2, m, h]}")
+    if not (need_dx or need_dw):
+        raise RuntimeError("gated_linear_bwd: no gradient to compute")
+    dx = torch.empty((m, k), dtype=x.dtype, device=dev) if need_dx else None
+    if m == 0:
+        dw = torch.zeros((2 * h, k), dtype=x.dtype, device=dev) if need_dw else None
+    else:
+        dw = torch.empty((2 * h, k), dtype=x.dtype, device=dev) if need_dw else None
+        ws_bytes = _lib.load().sage_gated_linear_bwd_workspace_bytes(m, h, k, ROW_DTYPES[x.dtype])
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _call("sage_gated_linear_bwd", dev, pd, ldd, px, ldx, pg, ldg, pu, ldu, saved.data_ptr(), act, m, h, k,
+              ROW_DTYPES[x.dtype], dx.data_ptr() if need_dx else None, k, dw.data_ptr() if need_dw else None,
+              ws.data_ptr(), ws_bytes)
+    return dx, (dw[:h] if need_dw else None), (dw[h:] if need_dw else None)

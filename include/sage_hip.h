@@ -746,6 +746,76 @@ int sage_adam_step_parts(float* param, float* grad, float* exp_avg, float* exp_a
                          int parts, sage_i64 region_off, sage_i64 region_len, void* done_event,
                          void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * The residual feed-forward block behind a layer: root-mean-square norm with the residual's
+ * addition, 8-bit products for serving, gated projections.  No counterpart in the reference
+ * (its layers end at layers/sage.py:131-134); graphsage_amd/layers/feed_forward.py is the
+ * caller.  These entry points take fp32, bf16 and fp16 rows; strides are in elements.
+ * ---------------------------------------------------------------------------------- */
+#define SAGE_F32 0
+#define SAGE_BF16 1
+#define SAGE_F16 2
+#define SAGE_ACT_SILU 0 /* g * sigmoid(g)                       */
+#define SAGE_ACT_GELU 1 /* g * (1 + erf(g / sqrt 2)) / 2        */
+#define SAGE_ACT_RELU 2
+#define SAGE_INT8_MAX_K 131056 /* whole pieces of 16, k * 128 * 128 < 2^31 */
+
+/* s = x + residual (fp32 sum; residual may be NULL), rstd = 1 / sqrt(mean(s^2) + eps),
+ * y = s * rstd * weight, each output rounded once to the rows' type.  sum (may be NULL) is s.
+ * The weight is in the rows' type or in fp32.  Rows may start at any element; stride 0 repeats
+ * a row.  sum may be the residual's own buffer. */
+int sage_rms_norm_fwd(const void* x, sage_i64 ld_x, const void* residual, sage_i64 ld_r, const void* weight,
+                      int weight_dtype, sage_i64 rows, sage_i64 dim, int dtype, float eps, void* y, sage_i64 ld_y,
+                      void* sum, sage_i64 ld_sum, void* stream);
+/* The same with an 8-bit output: t = s * weight, a = max |t| over the row,
+ * q = rint(t * 127 / a) (half to even), scale = a * rstd / 127, so that q * scale is y.
+ * A row of zeros has scale 0; a row with an infinity or NaN has q = 0 and scale NaN.
+ * q_cols >= dim columns of q are written, zeros behind dim (a product's rows end on 16 bytes).
+ * normalise = 0: rstd is 1 (quantisation alone; weight may be NULL = ones in either case). */
+int sage_rms_norm_int8(const void* x, sage_i64 ld_x, const void* residual, sage_i64 ld_r, const void* weight,
+                       int weight_dtype, sage_i64 rows, sage_i64 dim, int dtype, float eps, int normalise, int8_t* q,
+                       sage_i64 ld_q, sage_i64 q_cols, float* scale, void* sum, sage_i64 ld_sum, void* stream);
+/* out[r, c] = q[r, c] * scale[r], rounded once */
+int sage_dequantize_rows(const int8_t* q, sage_i64 ld_q, const float* scale, sage_i64 rows, sage_i64 dim, int dtype,
+                         void* out, sage_i64 ld_out, void* stream);
+/* Backward of sage_rms_norm_fwd from the stored sum: xh = sum * rstd, c = mean(dy * weight * xh),
+ * dx = rstd * (dy * weight - xh * c) + dsum (the gradient of x and of the residual alike),
+ * dweight = sum over rows of dy * xh (fixed order, fp32 sums; in the weight's type).
+ * dsum, and one of dx and dweight, may be NULL. */
+size_t sage_rms_norm_bwd_workspace_bytes(sage_i64 rows, sage_i64 dim, int dtype);
+int sage_rms_norm_bwd(const void* dy, sage_i64 ld_dy, const void* sum, sage_i64 ld_sum, const void* weight,
+                      int weight_dtype, const void* dsum, sage_i64 ld_dsum, sage_i64 rows, sage_i64 dim, int dtype,
+                      float eps, void* dx, sage_i64 ld_dx, void* dweight, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* Rows of row_bytes bytes into rows that start on 16 bytes and end, zero-filled, on 16 bytes:
+ * what the products below take (both operands' rows, and k, in whole pieces of 16 bytes). */
+int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows, sage_i64 row_bytes, void* out,
+                  sage_i64 ld_out_bytes, void* stream);
+/* out[m, n] = x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]; the sum is exact (32-bit
+ * integers, k <= SAGE_INT8_MAX_K), the rest fp32, rounded once to out_dtype.  bias may be NULL. */
+int sage_int8_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w, sage_i64 ld_w,
+                     const float* w_scale, const float* bias, sage_i64 m, sage_i64 n, sage_i64 k, int out_dtype,
+                     void* out, sage_i64 ld_out, void* stream);
+/* out = activation(gate product) * (up product), both as above without a bias */
+int sage_int8_gated_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w_gate, sage_i64 ld_g,
+                           const float* gate_scale, const int8_t* w_up, sage_i64 ld_u, const float* up_scale,
+                           int activation, sage_i64 m, sage_i64 n, sage_i64 k, int out_dtype, void* out,
+                           sage_i64 ld_out, void* stream);
+/* out[m, h] = activation(g) * u,  g = x w_gate^T, u = x w_up^T (fp32 sums, rounded once at the end).
+ * saved (may be NULL): [2, m, h] fp32, g and u for the backward pass. */
+int sage_gated_linear_fwd(const void* x, sage_i64 ld_x, const void* w_gate, sage_i64 ld_g, const void* w_up,
+                          sage_i64 ld_u, int activation, sage_i64 m, sage_i64 h, sage_i64 k, int dtype, void* out,
+                          sage_i64 ld_out, float* saved, void* stream);
+/* Gradients: dg = dh * u * activation'(g), du = dh * activation(g) (rounded to dtype: the products'
+ * operands), dx = dg w_gate + du w_up, dw = [dg^T x ; du^T x] as one [2 h, k] matrix.  dx or dw may
+ * be NULL.  The workspace starts on 256 bytes. */
+size_t sage_gated_linear_bwd_workspace_bytes(sage_i64 m, sage_i64 h, sage_i64 k, int dtype);
+int sage_gated_linear_bwd(const void* dh, sage_i64 ld_dh, const void* x, sage_i64 ld_x, const void* w_gate,
+                          sage_i64 ld_g, const void* w_up, sage_i64 ld_u, const float* saved, int activation,
+                          sage_i64 m, sage_i64 h, sage_i64 k, int dtype, void* dx, sage_i64 ld_dx, void* dw,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,339 @@
+"""Operators of the feed-forward block (norm with the residual's addition, 8-bit output, 8-bit
+products, gated projections) against their definitions in 64 bits.
+
+Tolerances are bounds by arithmetic, element by element, from the 64-bit values: u is half a step of
+the output's type (relative to the value), E = 2^-24 that of an fp32 operation, and a sum of n terms
+in fp32, in any order, is off by at most n E times the sum of the magnitudes.
+"""
+import math
+
+import pytest
+import torch
+
+from graphsage_amd import functional as SF
+from graphsage_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -140, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}   # half a subnormal step
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g, device=g.device) * scale).to(dtype)
+
+
+def within(got, want, bound, what):
+    got = got.double()
+    assert got.shape == want.shape, what
+    over = (got - want).abs() - bound
+    assert bool((over <= 0).all()), f"{what}: {int((over > 0).sum())} beyond their bound, worst by {float(over.max()):.3g}"
+
+
+def norm_ref(x, w, r, eps):
+    s = x.double() + (0 if r is None else r.double())
+    rstd = (s.square().mean(1, keepdim=True) + eps).rsqrt()
+    return s, rstd, s * rstd * w.double()
+
+
+# a row's fp32 statistics: a term's path through the tree is at most 64 additions (vectors of a thread, lanes, waves),
+# so the mean is off by 66 E and its root by half of that; x + r, the two products and the root add a few E
+STAT = 40 * E
+
+ROWS = [(1, 1), (1, 7), (3, 64), (5, 255), (2, 256), (130, 602), (9, 1023), (4, 2047), (3, 4104), (2, 8192), (2, 16390), (1, 40001)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", ROWS)
+def test_rms_norm_forward(dev, dtype, rows, dim):
+    g = gen(dev, rows * 7919 + dim)
+    x, r = normal(g, rows, dim, dtype=dtype, scale=3.0), normal(g, rows, dim, dtype=dtype)
+    for w in (normal(g, dim, dtype=dtype), normal(g, dim)):
+        for res in (None, r):
+            y, total = ops.rms_norm_fwd(x, w, residual=res, eps=1e-6)
+            s, rstd, want = norm_ref(x, w, res, 1e-6)
+            if res is None:
+                assert total is x
+            else:
+                within(total, s, s.abs() * (U[dtype] + E) + TINY[dtype], "sum")
+            within(y, want, want.abs() * (U[dtype] + STAT) * (1 + 2 ** -7) + TINY[dtype], "y")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rms_norm_strides_and_outputs(dev, dtype):
+    """Rows that start anywhere, one row repeated (stride 0), outputs inside larger buffers, the
+    residual stream updated in place; what lies around the outputs stays as it was."""
+    g = gen(dev, 5)
+    rows, dim = 37, 203
+    big = normal(g, rows, 3 * dim + 5, dtype=dtype)
+    x, r = big[:, 1:1 + dim], normal(g, 1, dim, dtype=dtype).expand(rows, dim)
+    w = normal(g, dim, dtype=dtype)
+    hold = torch.full((rows + 2, dim + 9), 7.0, dtype=dtype, device=dev)
+    y, total = ops.rms_norm_fwd(x, w, residual=r, out=hold[1:-1, 3:3 + dim])
+    want_y, want_s = ops.rms_norm_fwd(x.contiguous(), w, residual=r.contiguous())
+    assert torch.equal(y, want_y) and torch.equal(total, want_s)
+    hold[1:-1, 3:3 + dim] = 7.0
+    assert bool((hold == 7.0).all())
+    stream = r.contiguous()
+    y2, s2 = ops.rms_norm_fwd(x, w, residual=stream, sum_out=stream)
+    assert s2 is stream and torch.equal(stream, want_s) and torch.equal(y2, want_y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", ROWS)
+def test_rms_norm_int8(dev, dtype, rows, dim):
+    g = gen(dev, rows * 31 + dim)
+    x, r, w = normal(g, rows, dim, dtype=dtype, scale=2.0), normal(g, rows, dim, dtype=dtype), normal(g, dim, dtype=dtype)
+    q, scale, total = ops.rms_norm_int8(x, w, residual=r)
+    s, rstd, y = norm_ref(x, w, r, 1e-6)
+    within(total, s, s.abs() * (U[dtype] + E) + TINY[dtype], "sum")
+    want = y.abs().amax(1) / 127
+    within(scale, want, want * (STAT + 4 * E), "scale")
+    # q is 127 t / max|t| with t off by 2 E and the quotient by 3 E: rounding adds half a step
+    v = (s * w.double()) / (s * w.double()).abs().amax(1, keepdim=True) * 127
+    within(q, v, 0.5 + 127 * 8 * E, "q")
+    assert int(q.abs().max()) == 127
+    wide, scale2, _ = ops.rms_norm_int8(x, w, residual=r, padded=True)
+    assert wide.size(1) == (dim + 15) // 16 * 16 and torch.equal(wide[:, :dim], q) and torch.equal(scale, scale2)
+    assert not wide[:, dim:].any()
+    q3, scale3 = ops.quantize_rows(x)
+    top = x.double().abs().amax(1)
+    within(scale3, top / 127, top / 127 * 2 * E, "quantize_rows scale")
+    within(q3, x.double() / top[:, None] * 127, 0.5 + 127 * 8 * E, "quantize_rows q")
+    for out in DTYPES:
+        back = ops.dequantize_rows(q, scale, out)
+        want = q.double() * scale.double()[:, None]
+        within(back, want, want.abs() * (U[out] + 2 * E) + TINY[out], "dequantize_rows")
+
+
+def test_quantised_rows_of_special_values(dev):
+    """Zeros, subnormals, the type's largest values, infinities and NaN in a row; its neighbours are
+    not touched by them."""
+    x = torch.ones(9, 130, device=dev)
+    x[1] = 0.0
+    x[2] = 0.0
+    x[2, 77] = 2.0 ** -149
+    x[3] *= 1e-38
+    x[4, 3] = 3.4e38
+    x[5, 129] = float("inf")
+    x[6, 64] = float("nan")
+    x[7, 0] = -float("inf")
+    q, scale = ops.quantize_rows(x)
+    for row in (5, 6, 7):
+        assert math.isnan(float(scale[row])) and not q[row].any()
+        assert bool(torch.isnan(ops.dequantize_rows(q, scale)[row]).all())
+    assert float(scale[1]) == 0 and not q[1].any()
+    assert int(q[2, 77]) == 127 and int(q[2].abs().sum()) == 127
+    assert bool((q[3] == 127).all()) and int(q[4, 3]) == 127 and int(q[4].abs().sum()) == 127
+    for row in (0, 8):
+        assert bool((q[row] == 127).all()) and abs(float(scale[row]) * 127 - 1) <= 4 * E
+    y, _ = ops.rms_norm_fwd(x, torch.ones(130, device=dev))
+    assert bool(torch.isnan(y[6]).all()) and float(y[5, 0]) == 0 and math.isnan(float(y[5, 129]))
+    assert not y[1].any() and bool(torch.isfinite(y[[0, 1, 2, 3, 8]]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", ROWS + [(4999, 96), (3000, 1200), (1500, 4100)])
+def test_rms_norm_backward(dev, dtype, rows, dim):
+    g = gen(dev, rows * 17 + dim)
+    s, dy, ds = (normal(g, rows, dim, dtype=dtype) for _ in range(3))
+    for w in (1 + normal(g, dim, dtype=dtype), 1 + normal(g, dim)):
+        for dsum in (None, ds):
+            dx, dw = ops.rms_norm_bwd(dy, s, w, dsum=dsum)
+            s64, rstd, _ = norm_ref(s, w, None, 1e-6)
+            xh, gw = s64 * rstd, dy.double() * w.double()
+            c, c_mag = (gw * xh).mean(1, keepdim=True), (gw * xh).abs().mean(1, keepdim=True)
+            want = rstd * (gw - xh * c) + (0 if dsum is None else ds.double())
+            # c: 66 terms' additions on the magnitudes and the statistics; the rest a few operations each
+            mag = rstd * (gw.abs() + xh.abs() * c_mag) + (0 if dsum is None else ds.double().abs())
+            within(dx, want, mag * (72 * E + 2 * STAT) + want.abs() * U[dtype] * (1 + 2 ** -7) + TINY[dtype], "dx")
+            want_w, mag_w = (dy.double() * xh).sum(0), (dy.double() * xh).abs().sum(0)
+            # a column's sum: at most rows / groups terms in a thread, then the groups; no more than rows + 16 in all
+            within(dw, want_w, mag_w * ((min(rows, rows / 1024 + 1100) + 16) * E + STAT) + want_w.abs() * U[w.dtype] * (1 + 2 ** -7)
+                   + TINY[w.dtype], "dw")
+            again = ops.rms_norm_bwd(dy, s, w, dsum=dsum)
+            assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+            only = ops.rms_norm_bwd(dy, s, w, dsum=dsum, need_dw=False)
+            assert only[1] is None and torch.equal(only[0], dx)
+            only = ops.rms_norm_bwd(dy, s, w, dsum=dsum, need_dx=False)
+            assert only[0] is None and torch.equal(only[1], dw)
+
+
+# ------------------------------------------------------------------------------- 8-bit product
+def eight(g, rows, k):
+    q = torch.randint(-128, 128, (rows, k), generator=g, device=g.device, dtype=torch.int32).to(torch.int8)
+    return q, 0.01 * (0.5 + torch.rand(rows, generator=g, device=g.device))
+
+
+PRODUCTS = [(1, 1, 1), (1, 48, 16), (3, 17, 250), (16, 33, 64), (17, 130, 4096), (31, 64, 1008), (33, 257, 129), (64, 100, 528),
+            (65, 16, 48), (65, 300, 16), (129, 127, 272), (200, 515, 602), (513, 258, 128), (1000, 2100, 144), (4099, 5003, 80)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_int8_linear(dev, m, n, k):
+    g = gen(dev, m + n + k)
+    (x, xs), (w, ws), bias = eight(g, m, k), eight(g, n, k), normal(g, n)
+    acc = torch.mm(x.double(), w.double().t())            # whole numbers below 2^53: exact
+    for out_dtype in DTYPES:
+        for b in (None, bias):
+            got = ops.int8_linear(x, xs, w, ws, bias=b, out_dtype=out_dtype)
+            prod = acc * xs.double()[:, None] * ws.double()
+            want = prod + (0 if b is None else b.double())
+            within(got, want, prod.abs() * 4 * E + want.abs() * (U[out_dtype] + 2 * E) + TINY[out_dtype], f"{out_dtype} {b is None}")
+
+
+def test_int8_linear_largest_sums(dev):
+    """The widest row whose sum cannot leave 32 bits, all products at their largest; one more is refused."""
+    k = 131056
+    x = torch.full((2, k), -128, dtype=torch.int8, device=dev)
+    one = torch.ones(2, device=dev)
+    assert ops.int8_linear(x, one, x, one).tolist() == [[float(k * 16384)] * 2] * 2      # 17 bits times 2^14: exact in fp32
+    with pytest.raises(RuntimeError, match="32 bits"):
+        y = torch.zeros((2, k + 1), dtype=torch.int8, device=dev)
+        ops.int8_linear(y, one, y, one)
+
+
+def act64(v, name):
+    if name == "silu":
+        return v * torch.sigmoid(v)
+    if name == "gelu":
+        return 0.5 * v * (1 + torch.erf(v / math.sqrt(2)))
+    return v.clamp_min(0)
+
+
+def slope64(v, name):
+    if name == "silu":
+        p = torch.sigmoid(v)
+        return p * (1 + v * (1 - p))
+    if name == "gelu":
+        return 0.5 * (1 + torch.erf(v / math.sqrt(2))) + v * torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+    return (v > 0).double()
+
+
+# fp32 evaluation of an activation or its slope: the exponential's argument rounds by E |g| (times log2 e), its
+# value by 2 E more; division, erf and products add a few E.  |value| <= |g| + 0.2, |slope| <= 1.2.
+def act_error(g, name):
+    return (12 * E + 4 * E * g.abs()) * (g.abs() + 0.2)
+
+
+def slope_error(g, name):
+    return (16 * E + 6 * E * g.abs() * (1 + g.abs())) * 1.2
+
+
+def gated_bound(g, u, dg, du, name):
+    """Bound of |act(g) u| when g, u are off by dg, du (slopes of the activations stay below 1.2)."""
+    a = act64(g, name)
+    return (1.2 * dg + act_error(g, name)) * (u.abs() + du) + a.abs() * du + (a * u).abs() * 2 * E
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 40, 64), (5, 17, 250), (24, 130, 2048), (64, 48, 112), (65, 65, 96), (300, 515, 602), (1000, 4200, 144)])
+def test_int8_gated_linear(dev, act, m, n, k):
+    g = gen(dev, m * 3 + n + k)
+    (x, xs), (w, ws), (v, vs) = eight(g, m, k), eight(g, n, k), eight(g, n, k)
+    xs = xs * 0.02
+    gate = torch.mm(x.double(), w.double().t()) * xs.double()[:, None] * ws.double()
+    up = torch.mm(x.double(), v.double().t()) * xs.double()[:, None] * vs.double()
+    want = act64(gate, act) * up
+    bound = gated_bound(gate, up, gate.abs() * 4 * E, up.abs() * 4 * E, act)
+    for out_dtype in DTYPES:
+        got = ops.int8_gated_linear(x, xs, w, ws, v, vs, activation=act, out_dtype=out_dtype)
+        within(got, want, bound * (1 + 2 ** -7) + want.abs() * U[out_dtype] + TINY[out_dtype], f"{out_dtype}")
+
+
+# ------------------------------------------------------------------------------- gated projections
+GATED = [(1, 1, 1), (1, 40, 64), (4, 130, 600), (17, 33, 8), (64, 70, 1000), (65, 16, 24), (66, 65, 33), (130, 257, 128), (700, 530, 602), (2050, 2100, 72)]
+
+
+def gated_ref(x, wg, wu, act):
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    g, u = x @ wg.t(), x @ wu.t()
+    # k products (exact or E each) and their sum in fp32
+    k = x.size(1) + 2
+    return g, u, x.abs() @ wg.abs().t() * k * E, x.abs() @ wu.abs().t() * k * E
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,h,k", GATED)
+def test_gated_linear_forward(dev, dtype, act, m, h, k):
+    rng = gen(dev, m + h * 3 + k)
+    x, wg, wu = normal(rng, m, k, dtype=dtype, scale=2.0), normal(rng, h, k, dtype=dtype, scale=k ** -0.5), normal(rng, h, k, dtype=dtype, scale=k ** -0.5)
+    out, saved = ops.gated_linear_fwd(x, wg, wu, activation=act, save=True)
+    g, u, dg, du = gated_ref(x, wg, wu, act)
+    within(saved[0], g, dg + g.abs() * E, "gate")
+    within(saved[1], u, du + u.abs() * E, "up")
+    want = act64(g, act) * u
+    within(out, want, gated_bound(g, u, dg, du, act) * (1 + 2 ** -7) + want.abs() * U[dtype] + TINY[dtype], "out")
+    plain, none = ops.gated_linear_fwd(x, wg, wu, activation=act)
+    assert none is None and torch.equal(plain, out)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,h,k", GATED)
+def test_gated_linear_backward(dev, dtype, act, m, h, k):
+    rng = gen(dev, m + h * 5 + k)
+    x, wg, wu = normal(rng, m, k, dtype=dtype), normal(rng, h, k, dtype=dtype, scale=k ** -0.5), normal(rng, h, k, dtype=dtype, scale=k ** -0.5)
+    dh = normal(rng, m, h, dtype=dtype)
+    _, saved = ops.gated_linear_fwd(x, wg, wu, activation=act, save=True)
+    dx, dwg, dwu = ops.gated_linear_bwd(dh, x, wg, wu, saved, activation=act)
+    # from the saved products, which the forward test bounds: what is left is the operands' rounding
+    g, u, d = saved[0].double(), saved[1].double(), dh.double()
+    slope, a = slope64(g, act), act64(g, act)
+    dg, du = d * u * slope, d * a
+    dg_off = (d * u).abs() * slope_error(g, act) + dg.abs() * (U[dtype] + 3 * E) * (1 + 2 ** -7) + TINY[dtype]
+    du_off = d.abs() * act_error(g, act) + du.abs() * (U[dtype] + 3 * E) * (1 + 2 ** -7) + TINY[dtype]
+    x64, g64, u64 = x.double(), wg.double(), wu.double()
+
+    def check(got, want, mag, off, terms, what):
+        within(got, want, off + (mag + off) * (terms + 2) * E + want.abs() * U[dtype] * (1 + 2 ** -7) + TINY[dtype], what)
+
+    check(dx, dg @ g64 + du @ u64, dg.abs() @ g64.abs() + du.abs() @ u64.abs(), dg_off @ g64.abs() + du_off @ u64.abs(), 2 * h, "dx")
+    check(dwg, dg.t() @ x64, dg.abs().t() @ x64.abs(), dg_off.t() @ x64.abs(), m, "dw_gate")
+    check(dwu, du.t() @ x64, du.abs().t() @ x64.abs(), du_off.t() @ x64.abs(), m, "dw_up")
+    one = ops.gated_linear_bwd(dh, x, wg, wu, saved, activation=act, need_dw=False)
+    assert one[1] is None and one[2] is None and torch.equal(one[0], dx)
+    one = ops.gated_linear_bwd(dh, x, wg, wu, saved, activation=act, need_dx=False)
+    assert one[0] is None and torch.equal(one[1], dwg) and torch.equal(one[2], dwu)
+
+
+@pytest.mark.parametrize("dtype", DTYPES + [torch.int8])
+def test_products_take_any_rows(dev, dtype):
+    """Views whose rows start anywhere or repeat, and an output inside a larger buffer."""
+    rng = gen(dev, 11)
+    for m in (9, 140):
+        big = normal(rng, m, 400, scale=30.0).to(dtype)
+        w = normal(rng, 77, 400, scale=30.0).to(dtype)
+        x, wg, wu = big[:, 3:3 + 96], w[:, 16:112], w[:, 201:297]
+        row = x[:1].expand(m, 96)
+        hold = torch.full((m + 1, 90), 5.0, dtype=torch.float32 if dtype == torch.int8 else dtype, device=dev)
+        for a in (x, row):
+            if dtype == torch.int8:
+                s, t = torch.ones(m, device=dev) * 1e-3, torch.ones(77, device=dev) * 1e-3
+                got = ops.int8_gated_linear(a, s, wg, t, wu, t, out=hold[:m, 5:82])
+                want = ops.int8_gated_linear(a.contiguous(), s, wg.contiguous(), t, wu.contiguous(), t)
+                plain = ops.int8_linear(a, s, wg, t, out_dtype=torch.float32)
+                assert torch.equal(plain, ops.int8_linear(a.contiguous(), s, wg.contiguous(), t))
+            else:
+                got = ops.gated_linear_fwd(a, wg, wu, out=hold[:m, 5:82])[0]
+                want = ops.gated_linear_fwd(a.contiguous(), wg.contiguous(), wu.contiguous())[0]
+            assert torch.equal(got, want)
+            hold[:m, 5:82] = 5.0
+            assert bool((hold == 5.0).all())
+
+
+def test_not_a_number_stays_in_its_row(dev):
+    """A NaN in a row of x reaches that row's outputs and no others, also through rows that fill a tile."""
+    for m in (3, 70, 300):
+        for dtype in DTYPES:
+            x, w = torch.ones(m, 72, dtype=dtype, device=dev), torch.ones(33, 72, dtype=dtype, device=dev)
+            x[m - 1, 71] = float("nan")
+            out, _ = ops.gated_linear_fwd(x, w, w)
+            assert bool(torch.isnan(out[m - 1]).all()) and bool(torch.isfinite(out[:m - 1]).all())
