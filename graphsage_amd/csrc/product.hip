@@ -242,46 +242,54 @@ __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tile
   const int tm = first_m + in_g % rows_g, tn = in_g / rows_g;
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * S::kColsOut;
 
-  // a lane's pieces: row (of 8 a wave and load) and piece of the row, permuted as LDS holds them
-  const int piece_row = lane >> 3;
-  const char* ga[S::kLoadA];
-  const char* gb[S::kLoadB];
-  int ka[S::kLoadA], kb[S::kLoadB];
+  // a lane's pieces: row (of 8 a wave and load) and piece of the row, permuted as LDS holds them; as
+  // offsets of 32 bits from the tile's first row (a row's stride is below 2^23 bytes)
   constexpr int kRowsLoad = S::kThreads / 8;        // rows a load of the whole block fills
+  const char* a_base = p.a + m0 * p.lda;
+  const char* b_base0 = p.b0 + n0 * p.ldb0;
+  const char* b_base1 = kGated ? p.b1 + n0 * p.ldb1 : nullptr;
+  const int rows_left = p.m - m0 < BM ? static_cast<int>(p.m - m0) : BM;
+  const int cols_left = p.n - n0 < S::kColsOut ? static_cast<int>(p.n - n0) : S::kColsOut;
+  const uint32_t lda = static_cast<uint32_t>(p.lda), ldb0 = static_cast<uint32_t>(p.ldb0), ldb1 = static_cast<uint32_t>(p.ldb1);
+  uint32_t oa[S::kLoadA], ob[S::kLoadB];
+  // the load's rows are a multiple of 16, so every load of a lane takes the same piece of its row
+  static_assert(kRowsLoad % 16 == 0, "the piece of a lane");
+  const int lane_row = wave * 8 + (lane >> 3);
+  const int piece_at = ((lane & 7) ^ ((lane_row >> 1) & 7)) * 16;
 #pragma unroll
   for (int j = 0; j < S::kLoadA; ++j) {
-    const int r = j * kRowsLoad + wave * 8 + piece_row;
-    ka[j] = ((lane & 7) ^ ((r >> 1) & 7)) * 16;
-    const int64_t row = m0 + r < p.m ? m0 + r : p.m - 1;     // rows behind the last: their outputs are not stored
-    ga[j] = p.a + row * p.lda + ka[j];
+    const int r = j * kRowsLoad + lane_row;
+    oa[j] = static_cast<uint32_t>(r < rows_left ? r : rows_left - 1) * lda + piece_at;     // rows behind the last are not stored
   }
 #pragma unroll
   for (int j = 0; j < S::kLoadB; ++j) {
-    const int r = j * kRowsLoad + wave * 8 + piece_row;
-    kb[j] = ((lane & 7) ^ ((r >> 1) & 7)) * 16;
     int which;
-    const int64_t col = n0 + slot_column<kGated>(r, &which);
-    const int64_t row = col < p.n ? col : p.n - 1;
-    gb[j] = (which ? p.b1 + row * p.ldb1 : p.b0 + row * p.ldb0) + kb[j];
+    const int c = slot_column<kGated>(j * kRowsLoad + lane_row, &which);
+    ob[j] = static_cast<uint32_t>(c < cols_left ? c : cols_left - 1) * (which ? ldb1 : ldb0) + piece_at;
   }
   const char* zero = reinterpret_cast<const char*>(&kZeroPiece);
+  auto b_base = [&](int j) {      // a wave's 8 rows of a load are all of one B
+    if constexpr (!kGated) return b_base0;
+    return (((j * kRowsLoad + wave * 8) >> 5) & 1) ? b_base1 : b_base0;
+  };
   auto fetch = [&](char* a_lds, char* b_lds, int64_t k0) {
     const int64_t left = p.kbytes - k0;
     if (left >= 128) {
 #pragma unroll
       for (int j = 0; j < S::kLoadA; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(ga[j] + k0), (lptr_t)(a_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t)(a_base + k0 + oa[j]), (lptr_t)(a_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
 #pragma unroll
       for (int j = 0; j < S::kLoadB; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(gb[j] + k0), (lptr_t)(b_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t)(b_base(j) + k0 + ob[j]), (lptr_t)(b_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
     } else {
+      const bool in = piece_at < left;
 #pragma unroll
       for (int j = 0; j < S::kLoadA; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(ka[j] < left ? ga[j] + k0 : zero),
+        __builtin_amdgcn_global_load_lds((gptr_t)(in ? a_base + k0 + oa[j] : zero),
                                          (lptr_t)(a_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
 #pragma unroll
       for (int j = 0; j < S::kLoadB; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(kb[j] < left ? gb[j] + k0 : zero),
+        __builtin_amdgcn_global_load_lds((gptr_t)(in ? b_base(j) + k0 + ob[j] : zero),
                                          (lptr_t)(b_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
     }
   };
@@ -307,21 +315,22 @@ __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tile
       for (int i = 0; i < S::kMI; ++i)
 #pragma unroll
         for (int j = 0; j < S::kNI; ++j) acc[i][j] = Mma<T>::mma(b[j], a[i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);      // one half's operands in registers at a time
     }
   };
 
   const int64_t steps = (p.kbytes + 127) / 128;
   fetch(a_lds0, b_lds0, 0);
   __syncthreads();
-  for (int64_t s = 0; s < steps; s += 2) {
-    if (s + 1 < steps) fetch(a_lds1, b_lds1, (s + 1) * 128);
+  for (int64_t pair = 0; pair < steps / 2; ++pair) {
+    fetch(a_lds1, b_lds1, (2 * pair + 1) * 128);
     multiply(a_lds0, b_lds0);
     __syncthreads();
-    if (s + 1 >= steps) break;
-    if (s + 2 < steps) fetch(a_lds0, b_lds0, (s + 2) * 128);
+    if (2 * pair + 2 < steps) fetch(a_lds0, b_lds0, (2 * pair + 2) * 128);
     multiply(a_lds1, b_lds1);
     __syncthreads();
   }
+  if (steps & 1) multiply(a_lds0, b_lds0);
 
   // C^T layout of the MFMA (B's rows are its first operand): lane l holds row l & 15, and of slot
   // group j columns 4 (l >> 4) + 0..3, which the slot order makes consecutive over j
