@@ -99,6 +99,8 @@ struct Product {
   const float* sb1;
   const float* bias;
   float* saved;         // gated, training: pre-activations [2, m, n] in fp32
+  i32x4* partial;       // k split over blockIdx.y: the slices' sums, as the waves hold them
+  int64_t slice_bytes;  // of a row, a multiple of 128
 };
 
 template <int n, typename T>
@@ -216,6 +218,39 @@ __device__ inline int slot_column(int s, int* which) {
   return wn * 64 + (i >> 2) * 16 + j * 4 + (i & 3);
 }
 
+// Tile t's place: runs of tiles go down groups of 8 tile rows, so that the blocks of a run share operands.
+__device__ inline void tile_place(int tile, int tiles_m, int tiles_n, int* tm, int* tn) {
+  constexpr int kGroup = 8;
+  const int group = tile / (kGroup * tiles_n);
+  const int first_m = group * kGroup;
+  const int rows = tiles_m - first_m < kGroup ? tiles_m - first_m : kGroup;
+  const int in = tile - group * kGroup * tiles_n;
+  *tm = first_m + in % rows;
+  *tn = in / rows;
+}
+
+// C^T layout of the MFMA (B's rows are its first operand): lane l holds row l & 15, and of slot group j
+// columns 4 (l >> 4) + 0..3, which the slot order makes consecutive over j.
+template <typename T, typename S, bool kGated, typename Acc>
+__device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[S::kNI]) {
+  using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
+  const int l15 = lane & 15, q = lane >> 4;
+  if constexpr (kGated) {
+    E g[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      g[e] = acc[e >> 2][e & 3];
+      u[e] = acc[2 + (e >> 2)][e & 3];
+    }
+    finish_gated<T, 8>(p, m0 + row + l15, n0 + wn * 32 + q * 8, g, u);
+  } else {
+    E c[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) c[e] = acc[e >> 2][e & 3];
+    finish<T, 16>(p, m0 + row + l15, n0 + wn * 64 + q * 16, c);
+  }
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool kGated>
 __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tiles_m, int tiles_n) {
   using S = TileShape<BM, BN, WM, WN, kGated>;
@@ -226,28 +261,25 @@ __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tile
   __shared__ __attribute__((aligned(1024))) char b_lds1[BN * 128];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // tiles: each XCD (blockIdx modulo 8) takes a contiguous run of them, and a run goes down groups of
-  // 8 tile rows, so that an XCD's L2 holds the operands that its blocks share
+  // tiles: each XCD (blockIdx modulo 8) takes a contiguous run of them: its L2 holds what they share
   const int total = tiles_m * tiles_n;
   int tile = blockIdx.x;
   {
     const int per = total / 8, rest = total % 8, xcd = tile % 8, at = tile / 8;
     tile = xcd * per + (xcd < rest ? xcd : rest) + at;
   }
-  constexpr int kGroup = 8;
-  const int group = tile / (kGroup * tiles_n);
-  const int first_m = group * kGroup;
-  const int rows_g = tiles_m - first_m < kGroup ? tiles_m - first_m : kGroup;
-  const int in_g = tile - group * kGroup * tiles_n;
-  const int tm = first_m + in_g % rows_g, tn = in_g / rows_g;
+  int tm, tn;
+  tile_place(tile, tiles_m, tiles_n, &tm, &tn);
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * S::kColsOut;
 
   // a lane's pieces: row (of 8 a wave and load) and piece of the row, permuted as LDS holds them; as
   // offsets of 32 bits from the tile's first row (a row's stride is below 2^23 bytes)
   constexpr int kRowsLoad = S::kThreads / 8;        // rows a load of the whole block fills
-  const char* a_base = p.a + m0 * p.lda;
-  const char* b_base0 = p.b0 + n0 * p.ldb0;
-  const char* b_base1 = kGated ? p.b1 + n0 * p.ldb1 : nullptr;
+  const int64_t k_first = static_cast<int64_t>(blockIdx.y) * p.slice_bytes;
+  const int64_t kbytes = p.kbytes - k_first < p.slice_bytes ? p.kbytes - k_first : p.slice_bytes;
+  const char* a_base = p.a + m0 * p.lda + k_first;
+  const char* b_base0 = p.b0 + n0 * p.ldb0 + k_first;
+  const char* b_base1 = kGated ? p.b1 + n0 * p.ldb1 + k_first : nullptr;
   const int rows_left = p.m - m0 < BM ? static_cast<int>(p.m - m0) : BM;
   const int cols_left = p.n - n0 < S::kColsOut ? static_cast<int>(p.n - n0) : S::kColsOut;
   const uint32_t lda = static_cast<uint32_t>(p.lda), ldb0 = static_cast<uint32_t>(p.ldb0), ldb1 = static_cast<uint32_t>(p.ldb1);
@@ -273,7 +305,7 @@ __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tile
     return (((j * kRowsLoad + wave * 8) >> 5) & 1) ? b_base1 : b_base0;
   };
   auto fetch = [&](char* a_lds, char* b_lds, int64_t k0) {
-    const int64_t left = p.kbytes - k0;
+    const int64_t left = kbytes - k0;
     if (left >= 128) {
 #pragma unroll
       for (int j = 0; j < S::kLoadA; ++j)
@@ -302,57 +334,126 @@ __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tile
   const int wm = wave / WN, wn = wave % WN;
   const int l15 = lane & 15, q = lane >> 4, swz = (l15 >> 1) & 7;
   const int a_row = (wm * S::kRowsM + l15) * 128, b_row = (wn * 64 + l15) * 128;
-  auto multiply = [&](const char* a_lds, const char* b_lds) {
+  i32x4 a[S::kMI], b[S::kNI];
+  auto read = [&](const char* a_lds, const char* b_lds, int h) {
+    const int piece = ((h * 4 + q) ^ swz) * 16;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int piece = ((h * 4 + q) ^ swz) * 16;
-      i32x4 a[S::kMI], b[S::kNI];
+    for (int j = 0; j < S::kNI; ++j) b[j] = *reinterpret_cast<const i32x4*>(b_lds + b_row + j * 2048 + piece);
 #pragma unroll
-      for (int j = 0; j < S::kNI; ++j) b[j] = *reinterpret_cast<const i32x4*>(b_lds + b_row + j * 2048 + piece);
+    for (int i = 0; i < S::kMI; ++i) a[i] = *reinterpret_cast<const i32x4*>(a_lds + a_row + i * 2048 + piece);
+  };
+  auto multiply = [&]() {
 #pragma unroll
-      for (int i = 0; i < S::kMI; ++i) a[i] = *reinterpret_cast<const i32x4*>(a_lds + a_row + i * 2048 + piece);
+    for (int i = 0; i < S::kMI; ++i)
 #pragma unroll
-      for (int i = 0; i < S::kMI; ++i)
-#pragma unroll
-        for (int j = 0; j < S::kNI; ++j) acc[i][j] = Mma<T>::mma(b[j], a[i], acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);      // one half's operands in registers at a time
-    }
+      for (int j = 0; j < S::kNI; ++j) acc[i][j] = Mma<T>::mma(b[j], a[i], acc[i][j]);
   };
 
-  const int64_t steps = (p.kbytes + 127) / 128;
+  const int64_t steps = (kbytes + 127) / 128;
   fetch(a_lds0, b_lds0, 0);
   __syncthreads();
-  for (int64_t pair = 0; pair < steps / 2; ++pair) {
-    fetch(a_lds1, b_lds1, (2 * pair + 1) * 128);
-    multiply(a_lds0, b_lds0);
-    __syncthreads();
-    if (2 * pair + 2 < steps) fetch(a_lds0, b_lds0, (2 * pair + 2) * 128);
-    multiply(a_lds1, b_lds1);
-    __syncthreads();
-  }
-  if (steps & 1) multiply(a_lds0, b_lds0);
-
-  // C^T layout of the MFMA (B's rows are its first operand): lane l holds row l & 15, and of slot
-  // group j columns 4 (l >> 4) + 0..3, which the slot order makes consecutive over j
-  using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
-#pragma unroll
-  for (int i = 0; i < S::kMI; ++i) {
-    const int64_t row = m0 + wm * S::kRowsM + i * 16 + l15;
-    if constexpr (kGated) {
-      E g[8], u[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        g[e] = acc[i][e >> 2][e & 3];
-        u[e] = acc[i][2 + (e >> 2)][e & 3];
-      }
-      finish_gated<T, 8>(p, row, n0 + wn * 32 + q * 8, g, u);
-    } else {
-      E c[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) c[e] = acc[i][e >> 2][e & 3];
-      finish<T, 16>(p, row, n0 + wn * 64 + q * 16, c);
+  if constexpr (S::kThreads == 512) {
+    // Two waves a SIMD, one of each half of the block (wave / 4), kept half a phase apart: while one
+    // half's waves read their operands from LDS, the other's multiply, so neither unit waits for the
+    // other.  A step is four phases, each ended by a barrier of the whole block: read and multiply its
+    // first 64 bytes, read and multiply its second; the second half runs one phase behind (the extra
+    // barrier before the loop, and the first half's after it).
+    // With the first half's phases of step t numbered 4 t .. 4 t + 3: the buffer of step t - 1 is last read
+    // by the second half in phase 4 t - 1, whose reads have landed (lgkmcnt(0)) before the barrier that
+    // ends it, so step t + 1 may be fetched into it from phase 4 t on; and it is first read in phase 4 t + 4,
+    // before which the first half has waited for its loads in 4 t + 3 and the second half in its phase 4 t + 2.
+    const int half = wave >> 2;
+    auto meet = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](char* a_now, char* b_now, char* a_next, char* b_next, int64_t t) {
+      if (t + 1 < steps) fetch(a_next, b_next, (t + 1) * 128);
+      read(a_now, b_now, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      meet();
+      __builtin_amdgcn_s_setprio(1);
+      multiply();
+      __builtin_amdgcn_s_setprio(0);
+      meet();
+      read(a_now, b_now, 1);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (half) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      meet();
+      __builtin_amdgcn_s_setprio(1);
+      multiply();
+      __builtin_amdgcn_s_setprio(0);
+      if (!half) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      meet();
+    };
+    if (half) meet();
+    for (int64_t pair = 0; pair < steps / 2; ++pair) {
+      step(a_lds0, b_lds0, a_lds1, b_lds1, 2 * pair);
+      step(a_lds1, b_lds1, a_lds0, b_lds0, 2 * pair + 1);
     }
+    if (steps & 1) step(a_lds0, b_lds0, a_lds1, b_lds1, steps - 1);
+    if (!half) meet();
+  } else {
+    auto both = [&](const char* a_lds, const char* b_lds) {
+      read(a_lds, b_lds, 0);
+      multiply();
+      __builtin_amdgcn_sched_barrier(0);      // one half's operands in registers at a time
+      read(a_lds, b_lds, 1);
+      multiply();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int64_t pair = 0; pair < steps / 2; ++pair) {
+      fetch(a_lds1, b_lds1, (2 * pair + 1) * 128);
+      both(a_lds0, b_lds0);
+      __syncthreads();
+      if (2 * pair + 2 < steps) fetch(a_lds0, b_lds0, (2 * pair + 2) * 128);
+      both(a_lds1, b_lds1);
+      __syncthreads();
+    }
+    if (steps & 1) both(a_lds0, b_lds0);
   }
+
+  if (p.partial != nullptr) {
+    i32x4* to = p.partial + (((static_cast<int64_t>(blockIdx.y) * total + tile) * (WM * WN) + wave) * (S::kMI * S::kNI)) * kWave + lane;
+#pragma unroll
+    for (int i = 0; i < S::kMI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::kNI; ++j) to[(i * S::kNI + j) * kWave] = __builtin_bit_cast(i32x4, acc[i][j]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < S::kMI; ++i) finish_rows<T, S, kGated>(p, m0, n0, wm * S::kRowsM + i * 16, wn, lane, acc[i]);
+}
+
+// The slices' sums of a split product, added in order by waves that each take the 16 rows that one wave
+// of the tile kernel holds in acc[i], and finished as there.
+template <typename T, int BM, int BN, int WM, int WN, bool kGated>
+__global__ void __launch_bounds__(256) join_kernel(Product p, int tiles_m, int tiles_n, int slices) {
+  using S = TileShape<BM, BN, WM, WN, kGated>;
+  using Acc = typename Mma<T>::Acc;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;   // (tile, wave, i)
+  const int64_t total = static_cast<int64_t>(tiles_m) * tiles_n, per_tile = WM * WN * S::kMI;
+  if (unit >= total * per_tile) return;
+  const int tile = static_cast<int>(unit / per_tile), in_tile = static_cast<int>(unit - tile * per_tile);
+  const int wave = in_tile / S::kMI, i = in_tile - wave * S::kMI;
+  int tm, tn;
+  tile_place(tile, tiles_m, tiles_n, &tm, &tn);
+  const i32x4* from = p.partial + ((static_cast<int64_t>(tile) * (WM * WN) + wave) * S::kMI + i) * S::kNI * kWave + lane;
+  const int64_t stride = total * (WM * WN) * S::kMI * S::kNI * kWave;
+  Acc acc[S::kNI];
+#pragma unroll
+  for (int j = 0; j < S::kNI; ++j) acc[j] = __builtin_bit_cast(Acc, from[j * kWave]);
+  for (int s = 1; s < slices; ++s) {
+    from += stride;
+#pragma unroll
+    for (int j = 0; j < S::kNI; ++j) acc[j] += __builtin_bit_cast(Acc, from[j * kWave]);
+  }
+  finish_rows<T, S, kGated>(p, static_cast<int64_t>(tm) * BM, static_cast<int64_t>(tn) * S::kColsOut,
+                            wave / WN * S::kRowsM + i * 16, wave % WN, lane, acc);
 }
 
 // ------------------------------------------------------------------------------- few rows
@@ -430,27 +531,73 @@ __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_kernel(Product p) {
 }
 
 // ------------------------------------------------------------------------------- launch
+inline bool rows16(const void* p, int64_t ld_bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld_bytes & 15) == 0 && ld_bytes >= 0;
+}
+constexpr int64_t kMaxRowBytes = int64_t{1} << 23;     // the tile loads' offsets: 256 rows in 31 bits
+
+// How a product is cut: few rows; or tiles of `tile` x `tile` (gated: `tile` / 2 columns), k in `slices`.
+struct Plan {
+  int tile, slices;      // tile 0: few_rows_kernel
+  int64_t slice_bytes;
+  size_t workspace;
+};
+
+inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated) {
+  Plan best{0, 1, kbytes, 0};
+  if (m <= 64) return best;
+  const int64_t steps = cdiv(kbytes, 128);
+  double least = 1e300;
+  for (int tile : {256, 128}) {
+    const int64_t tiles = cdiv(m, tile) * cdiv(n, gated ? tile / 2 : tile);
+    // microseconds: a step of 128 bytes of k, a block's start and end, and how many blocks run at once
+    const double step = tile == 256 ? 1.5 : 0.9, ends = tile == 256 ? 6.0 : 4.0;
+    const int64_t at_once = tile == 256 ? 256 : 512;
+    for (int64_t slices = 1; slices <= 32 && slices <= steps; slices *= 2) {
+      const int64_t each = cdiv(steps, slices), used = cdiv(steps, each);
+      if (used != slices) continue;
+      const double bytes = static_cast<double>(slices) * tiles * tile * tile * 4;
+      double time = cdiv(tiles * slices, at_once) * (each * step + ends);
+      if (slices > 1) time += 4.0 + 2.0 * bytes / 4e6;      // written and read at 4 TB/s, one more launch
+      if (time < least) {
+        least = time;
+        best = Plan{tile, static_cast<int>(slices), each * 128, slices > 1 ? static_cast<size_t>(bytes) : 0};
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, bool kGated, int kTile, int WM, int WN>
+void launch_tiles(Product& p, const Plan& plan, int64_t tm, int64_t tn, hipStream_t stream) {
+  hipLaunchKernelGGL((tile_kernel<T, kTile, kTile, WM, WN, kGated>), dim3(static_cast<unsigned>(tm * tn), plan.slices),
+                     dim3(WM * WN * kWave), 0, stream, p, static_cast<int>(tm), static_cast<int>(tn));
+  if (plan.slices > 1) {
+    const int64_t units = tm * tn * (kTile * kTile / (16 * 64));
+    hipLaunchKernelGGL((join_kernel<T, kTile, kTile, WM, WN, kGated>), dim3(static_cast<unsigned>(cdiv(units, 4))), dim3(256), 0,
+                       stream, p, static_cast<int>(tm), static_cast<int>(tn), plan.slices);
+  }
+}
+
 template <typename T, bool kGated>
-int launch_product(const Product& p, hipStream_t stream, const char* what) {
-  const int64_t cus = 256;
-  if (p.m <= 64) {
+int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, const char* what) {
+  const Plan plan = plan_product(p.m, p.n, p.kbytes, kGated);
+  SAGE_REQUIRE(p.lda < kMaxRowBytes && p.ldb0 < kMaxRowBytes && p.ldb1 < kMaxRowBytes, SAGE_ELIMIT, "%s: rows more than %ld bytes apart",
+               what, (long)kMaxRowBytes);
+  if (plan.tile == 0) {
     const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), 1);
     if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
     else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
     else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
   } else {
-    const int64_t big = cdiv(p.m, 256) * cdiv(p.n, kGated ? 128 : 256);
-    if (big >= cus) {
-      const int64_t tm = cdiv(p.m, 256), tn = cdiv(p.n, kGated ? 128 : 256);
-      SAGE_REQUIRE(tm * tn < (int64_t{1} << 31), SAGE_ELIMIT, "%s: too many output tiles", what);
-      hipLaunchKernelGGL((tile_kernel<T, 256, 256, 2, 4, kGated>), dim3(static_cast<unsigned>(tm * tn)), dim3(512), 0, stream, p,
-                         static_cast<int>(tm), static_cast<int>(tn));
-    } else {
-      const int64_t tm = cdiv(p.m, 128), tn = cdiv(p.n, kGated ? 64 : 128);
-      SAGE_REQUIRE(tm * tn < (int64_t{1} << 31), SAGE_ELIMIT, "%s: too many output tiles", what);
-      hipLaunchKernelGGL((tile_kernel<T, 128, 128, 2, 2, kGated>), dim3(static_cast<unsigned>(tm * tn)), dim3(256), 0, stream, p,
-                         static_cast<int>(tm), static_cast<int>(tn));
-    }
+    SAGE_REQUIRE(plan.workspace <= ws_bytes && (plan.workspace == 0 || rows16(ws, 0)), SAGE_EWORKSPACE,
+                 "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, plan.workspace);
+    const int64_t tm = cdiv(p.m, plan.tile), tn = cdiv(p.n, kGated ? plan.tile / 2 : plan.tile);
+    SAGE_REQUIRE(tm * tn < (int64_t{1} << 24), SAGE_ELIMIT, "%s: %ld output tiles", what, (long)(tm * tn));
+    p.slice_bytes = plan.slice_bytes;
+    p.partial = plan.slices > 1 ? static_cast<i32x4*>(ws) : nullptr;
+    if (plan.tile == 256) launch_tiles<T, kGated, 256, 2, 4>(p, plan, tm, tn, stream);
+    else launch_tiles<T, kGated, 128, 2, 2>(p, plan, tm, tn, stream);
   }
   SAGE_CHECK_LAUNCH(what);
   return SAGE_OK;
@@ -459,15 +606,12 @@ int launch_product(const Product& p, hipStream_t stream, const char* what) {
 inline int size_of(int dtype) { return dtype == SAGE_F32 ? 4 : 2; }
 inline bool known_dtype(int d) { return d == SAGE_F32 || d == SAGE_BF16 || d == SAGE_F16; }
 inline bool known_act(int a) { return a == SAGE_ACT_SILU || a == SAGE_ACT_GELU || a == SAGE_ACT_RELU; }
-inline bool rows16(const void* p, int64_t ld_bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld_bytes & 15) == 0 && ld_bytes >= 0;
-}
 
 template <bool kGated>
-int product_by_type(const Product& p, int dtype, hipStream_t stream, const char* what) {
-  if (dtype == SAGE_F32) return launch_product<float, kGated>(p, stream, what);
-  if (dtype == SAGE_BF16) return launch_product<__bf16, kGated>(p, stream, what);
-  return launch_product<_Float16, kGated>(p, stream, what);
+int product_by_type(const Product& p, int dtype, void* ws, size_t ws_bytes, hipStream_t stream, const char* what) {
+  if (dtype == SAGE_F32) return launch_product<float, kGated>(p, ws, ws_bytes, stream, what);
+  if (dtype == SAGE_BF16) return launch_product<__bf16, kGated>(p, ws, ws_bytes, stream, what);
+  return launch_product<_Float16, kGated>(p, ws, ws_bytes, stream, what);
 }
 
 // ------------------------------------------------------------------------------- backward pass
@@ -550,7 +694,7 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const uint8_t* in, int64_
 
 struct BwdLayout {
   int64_t ld_rows, ld_cols, ld_w;          // in elements
-  size_t rows, cols, xt, wt, bytes;        // offsets
+  size_t rows, cols, xt, wt, part, part_bytes, bytes;        // offsets
 };
 inline BwdLayout bwd_layout(int64_t m, int64_t h, int64_t k, int dtype) {
   const int64_t piece = 16 / size_of(dtype);
@@ -568,7 +712,12 @@ inline BwdLayout bwd_layout(int64_t m, int64_t h, int64_t k, int dtype) {
   l.cols = take(2 * h * l.ld_cols);
   l.xt = take(k * l.ld_cols);
   l.wt = take(k * l.ld_w);
-  l.bytes = off;
+  // the two products run one after the other and share the room for their slices
+  l.part = off;
+  const size_t for_dx = plan_product(m, k, l.ld_rows * size_of(dtype), false).workspace;
+  const size_t for_dw = plan_product(2 * h, k, l.ld_cols * size_of(dtype), false).workspace;
+  l.part_bytes = for_dx > for_dw ? for_dx : for_dw;
+  l.bytes = off + l.part_bytes;
   return l;
 }
 
@@ -598,7 +747,7 @@ int gated_bwd(const void* dh, int64_t ld_dh, const void* x, int64_t ld_x, const 
     p.b0 = reinterpret_cast<const char*>(wt); p.ldb0 = l.ld_w * sizeof(T);
     p.m = m; p.n = k; p.kbytes = l.ld_rows * sizeof(T);
     p.out = dx; p.ldo = ld_dx; p.out_dtype = dtype;
-    const int rc = launch_product<T, false>(p, st, what);
+    const int rc = launch_product<T, false>(p, ws + l.part, l.part_bytes, st, what);
     if (rc != SAGE_OK) return rc;
   }
   if (dw != nullptr) {
@@ -610,7 +759,7 @@ int gated_bwd(const void* dh, int64_t ld_dh, const void* x, int64_t ld_x, const 
     p.b0 = reinterpret_cast<const char*>(xt); p.ldb0 = l.ld_cols * sizeof(T);
     p.m = 2 * h; p.n = k; p.kbytes = l.ld_cols * sizeof(T);
     p.out = dw; p.ldo = k; p.out_dtype = dtype;
-    return launch_product<T, false>(p, st, what);
+    return launch_product<T, false>(p, ws + l.part, l.part_bytes, st, what);
   }
   return SAGE_OK;
 }
@@ -635,6 +784,11 @@ extern "C" int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows
   return SAGE_OK;
 }
 
+extern "C" size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated) {
+  if (m <= 0 || n <= 0 || row_bytes <= 0) return 0;
+  return plan_product(m, n, row_bytes, gated != 0).workspace;
+}
+
 #define SAGE_INT8_CHECKS(what)                                                                                          \
   SAGE_REQUIRE(known_dtype(out_dtype), SAGE_EINVAL, what ": unknown output dtype %d", out_dtype);                       \
   SAGE_REQUIRE(m >= 0 && n > 0 && k > 0, SAGE_EINVAL, what ": bad shape m %ld n %ld k %ld", (long)m, (long)n, (long)k); \
@@ -642,7 +796,7 @@ extern "C" int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows
 
 extern "C" int sage_int8_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w, sage_i64 ld_w,
                                 const float* w_scale, const float* bias, sage_i64 m, sage_i64 n, sage_i64 k, int out_dtype,
-                                void* out, sage_i64 ld_out, void* stream) {
+                                void* out, sage_i64 ld_out, void* workspace, size_t workspace_bytes, void* stream) {
   SAGE_INT8_CHECKS("sage_int8_linear");
   if (m == 0) return SAGE_OK;
   SAGE_REQUIRE(x && x_scale && w && w_scale && out, SAGE_EINVAL, "sage_int8_linear: NULL pointer");
@@ -654,13 +808,13 @@ extern "C" int sage_int8_linear(const int8_t* x, sage_i64 ld_x, const float* x_s
   p.m = m; p.n = n; p.kbytes = k;
   p.out = out; p.ldo = ld_out; p.out_dtype = out_dtype;
   p.sa = x_scale; p.sb0 = w_scale; p.bias = bias;
-  return launch_product<int8_t, false>(p, static_cast<hipStream_t>(stream), "sage_int8_linear");
+  return launch_product<int8_t, false>(p, workspace, workspace_bytes, static_cast<hipStream_t>(stream), "sage_int8_linear");
 }
 
 extern "C" int sage_int8_gated_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w_gate, sage_i64 ld_g,
                                       const float* gate_scale, const int8_t* w_up, sage_i64 ld_u, const float* up_scale,
                                       int activation, sage_i64 m, sage_i64 n, sage_i64 k, int out_dtype, void* out,
-                                      sage_i64 ld_out, void* stream) {
+                                      sage_i64 ld_out, void* workspace, size_t workspace_bytes, void* stream) {
   SAGE_INT8_CHECKS("sage_int8_gated_linear");
   SAGE_REQUIRE(known_act(activation), SAGE_EINVAL, "sage_int8_gated_linear: unknown activation %d", activation);
   if (m == 0) return SAGE_OK;
@@ -674,12 +828,12 @@ extern "C" int sage_int8_gated_linear(const int8_t* x, sage_i64 ld_x, const floa
   p.m = m; p.n = n; p.kbytes = k;
   p.out = out; p.ldo = ld_out; p.out_dtype = out_dtype; p.act = activation;
   p.sa = x_scale; p.sb0 = gate_scale; p.sb1 = up_scale;
-  return launch_product<int8_t, true>(p, static_cast<hipStream_t>(stream), "sage_int8_gated_linear");
+  return launch_product<int8_t, true>(p, workspace, workspace_bytes, static_cast<hipStream_t>(stream), "sage_int8_gated_linear");
 }
 
 extern "C" int sage_gated_linear_fwd(const void* x, sage_i64 ld_x, const void* w_gate, sage_i64 ld_g, const void* w_up,
                                      sage_i64 ld_u, int activation, sage_i64 m, sage_i64 h, sage_i64 k, int dtype, void* out,
-                                     sage_i64 ld_out, float* saved, void* stream) {
+                                     sage_i64 ld_out, float* saved, void* workspace, size_t workspace_bytes, void* stream) {
   SAGE_REQUIRE(known_dtype(dtype), SAGE_EINVAL, "sage_gated_linear_fwd: unknown dtype %d", dtype);
   SAGE_REQUIRE(known_act(activation), SAGE_EINVAL, "sage_gated_linear_fwd: unknown activation %d", activation);
   SAGE_REQUIRE(m >= 0 && h > 0 && k > 0, SAGE_EINVAL, "sage_gated_linear_fwd: bad shape m %ld h %ld k %ld", (long)m, (long)h, (long)k);
@@ -694,7 +848,7 @@ extern "C" int sage_gated_linear_fwd(const void* x, sage_i64 ld_x, const void* w
   p.b1 = static_cast<const char*>(w_up); p.ldb1 = ld_u * size;
   p.m = m; p.n = h; p.kbytes = k * size;
   p.out = out; p.ldo = ld_out; p.out_dtype = dtype; p.act = activation; p.saved = saved;
-  return product_by_type<true>(p, dtype, static_cast<hipStream_t>(stream), "sage_gated_linear_fwd");
+  return product_by_type<true>(p, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream), "sage_gated_linear_fwd");
 }
 
 extern "C" size_t sage_gated_linear_bwd_workspace_bytes(sage_i64 m, sage_i64 h, sage_i64 k, int dtype) {

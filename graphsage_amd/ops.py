@@ -1500,13 +1500,22 @@ def _pieces(t, p, ld):
     """The matrix itself if its rows are whole pieces of 16 bytes that start on 16 bytes, else a
     zero-filled copy that is: (pointer, row stride in elements, columns, what must stay alive)."""
     size, (rows, cols) = t.element_size(), t.shape
-    if p % 16 == 0 and ld * size % 16 == 0 and cols * size % 16 == 0:
+    if p % 16 == 0 and ld * size % 16 == 0 and cols * size % 16 == 0 and ld * size < 1 << 23:
         return p, ld, cols, t
     each = 16 // size
     wide = (cols + each - 1) // each * each
     out = torch.empty((rows, wide), dtype=t.dtype, device=t.device)
     _call("sage_pad_rows", t.device, p, ld * size, rows, cols * size, out.data_ptr(), wide * size)
     return out.data_ptr(), wide, wide, out
+
+
+def _product_workspace(m, n, row_bytes, gated, device):
+    """(pointer, bytes, owner) of what a product of few tiles splits k into; few rows take none."""
+    size = _lib.load().sage_product_workspace_bytes(m, n, row_bytes, gated) if m > 64 else 0
+    if size == 0:
+        return None, 0, None
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    return ws.data_ptr(), size, ws
 
 
 def _int8_operand(q, scale, name, k=None, device=None):
@@ -1539,7 +1548,8 @@ def _int8_product(name, x, x_scale, weights, extra, out_dtype, out):
         pw, ldw, _, keep = _pieces(w, pw, ldw)
         args += [pw, ldw, psw]
         kept.append(keep)
-    _call(f"sage_{name}", dev, px, ldx, psx, *args, extra(n, dev), m, n, wide, ROW_DTYPES[out_dtype], po, ldo)
+    ws, ws_bytes, keep = _product_workspace(m, n, wide, len(weights) - 1, dev)
+    _call(f"sage_{name}", dev, px, ldx, psx, *args, extra(n, dev), m, n, wide, ROW_DTYPES[out_dtype], po, ldo, ws, ws_bytes)
     return out
 
 
@@ -1582,8 +1592,9 @@ def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
     px, ldx, wide, keep_x = _pieces(x, px, ldx)
     pg, ldg, _, keep_g = _pieces(w_gate, pg, ldg)
     pu, ldu, _, keep_u = _pieces(w_up, pu, ldu)
+    ws, ws_bytes, keep = _product_workspace(m, h, wide * x.element_size(), 1, dev)
     _call("sage_gated_linear_fwd", dev, px, ldx, pg, ldg, pu, ldu, act, m, h, wide, ROW_DTYPES[x.dtype], po, ldo,
-          saved.data_ptr() if save else None)
+          saved.data_ptr() if save else None, ws, ws_bytes)
     return out, saved
 
 

@@ -792,21 +792,25 @@ int sage_rms_norm_bwd(const void* dy, sage_i64 ld_dy, const void* sum, sage_i64 
  * what the products below take (both operands' rows, and k, in whole pieces of 16 bytes). */
 int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows, sage_i64 row_bytes, void* out,
                   sage_i64 ld_out_bytes, void* stream);
+/* Workspace of a product below (starts on 16 bytes; 0 bytes: none, NULL): where an output has too few
+ * tiles to fill the chip, k is split and the slices' sums meet there.  row_bytes is k times the
+ * element's size; gated: two weights.  The operands' rows are less than 2^23 bytes apart. */
+size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated);
 /* out[m, n] = x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]; the sum is exact (32-bit
  * integers, k <= SAGE_INT8_MAX_K), the rest fp32, rounded once to out_dtype.  bias may be NULL. */
 int sage_int8_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w, sage_i64 ld_w,
                      const float* w_scale, const float* bias, sage_i64 m, sage_i64 n, sage_i64 k, int out_dtype,
-                     void* out, sage_i64 ld_out, void* stream);
+                     void* out, sage_i64 ld_out, void* workspace, size_t workspace_bytes, void* stream);
 /* out = activation(gate product) * (up product), both as above without a bias */
 int sage_int8_gated_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w_gate, sage_i64 ld_g,
                            const float* gate_scale, const int8_t* w_up, sage_i64 ld_u, const float* up_scale,
                            int activation, sage_i64 m, sage_i64 n, sage_i64 k, int out_dtype, void* out,
-                           sage_i64 ld_out, void* stream);
+                           sage_i64 ld_out, void* workspace, size_t workspace_bytes, void* stream);
 /* out[m, h] = activation(g) * u,  g = x w_gate^T, u = x w_up^T (fp32 sums, rounded once at the end).
  * saved (may be NULL): [2, m, h] fp32, g and u for the backward pass. */
 int sage_gated_linear_fwd(const void* x, sage_i64 ld_x, const void* w_gate, sage_i64 ld_g, const void* w_up,
                           sage_i64 ld_u, int activation, sage_i64 m, sage_i64 h, sage_i64 k, int dtype, void* out,
-                          sage_i64 ld_out, float* saved, void* stream);
+                          sage_i64 ld_out, float* saved, void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients: dg = dh * u * activation'(g), du = dh * activation(g) (rounded to dtype: the products'
  * operands), dx = dg w_gate + du w_up, dw = [dg^T x ; du^T x] as one [2 h, k] matrix.  dx or dw may
  * be NULL.  The workspace starts on 256 bytes. */
