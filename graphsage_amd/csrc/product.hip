@@ -218,6 +218,13 @@ __device__ inline int slot_column(int s, int* which) {
   return wn * 64 + (i >> 2) * 16 + j * 4 + (i & 3);
 }
 
+// The tile of a block: each XCD (blockIdx modulo 8) takes a contiguous run of them, so that its L2 holds what
+// they share.
+__device__ inline int xcd_tile(int block, int total) {
+  const int per = total / 8, rest = total % 8, xcd = block % 8;
+  return xcd * per + (xcd < rest ? xcd : rest) + block / 8;
+}
+
 // Tile t's place: runs of tiles go down groups of 8 tile rows, so that the blocks of a run share operands.
 __device__ inline void tile_place(int tile, int tiles_m, int tiles_n, int* tm, int* tn) {
   constexpr int kGroup = 8;
@@ -261,13 +268,8 @@ __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tile
   __shared__ __attribute__((aligned(1024))) char b_lds1[BN * 128];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // tiles: each XCD (blockIdx modulo 8) takes a contiguous run of them: its L2 holds what they share
   const int total = tiles_m * tiles_n;
-  int tile = blockIdx.x;
-  {
-    const int per = total / 8, rest = total % 8, xcd = tile % 8, at = tile / 8;
-    tile = xcd * per + (xcd < rest ? xcd : rest) + at;
-  }
+  const int tile = xcd_tile(blockIdx.x, total);
   int tm, tn;
   tile_place(tile, tiles_m, tiles_n, &tm, &tn);
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * S::kColsOut;
@@ -352,69 +354,23 @@ __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tile
   const int64_t steps = (kbytes + 127) / 128;
   fetch(a_lds0, b_lds0, 0);
   __syncthreads();
-  if constexpr (S::kThreads == 512) {
-    // Two waves a SIMD, one of each half of the block (wave / 4), kept half a phase apart: while one
-    // half's waves read their operands from LDS, the other's multiply, so neither unit waits for the
-    // other.  A step is four phases, each ended by a barrier of the whole block: read and multiply its
-    // first 64 bytes, read and multiply its second; the second half runs one phase behind (the extra
-    // barrier before the loop, and the first half's after it).
-    // With the first half's phases of step t numbered 4 t .. 4 t + 3: the buffer of step t - 1 is last read
-    // by the second half in phase 4 t - 1, whose reads have landed (lgkmcnt(0)) before the barrier that
-    // ends it, so step t + 1 may be fetched into it from phase 4 t on; and it is first read in phase 4 t + 4,
-    // before which the first half has waited for its loads in 4 t + 3 and the second half in its phase 4 t + 2.
-    const int half = wave >> 2;
-    auto meet = [&]() {
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    auto step = [&](char* a_now, char* b_now, char* a_next, char* b_next, int64_t t) {
-      if (t + 1 < steps) fetch(a_next, b_next, (t + 1) * 128);
-      read(a_now, b_now, 0);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      meet();
-      __builtin_amdgcn_s_setprio(1);
-      multiply();
-      __builtin_amdgcn_s_setprio(0);
-      meet();
-      read(a_now, b_now, 1);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (half) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      meet();
-      __builtin_amdgcn_s_setprio(1);
-      multiply();
-      __builtin_amdgcn_s_setprio(0);
-      if (!half) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      meet();
-    };
-    if (half) meet();
-    for (int64_t pair = 0; pair < steps / 2; ++pair) {
-      step(a_lds0, b_lds0, a_lds1, b_lds1, 2 * pair);
-      step(a_lds1, b_lds1, a_lds0, b_lds0, 2 * pair + 1);
-    }
-    if (steps & 1) step(a_lds0, b_lds0, a_lds1, b_lds1, steps - 1);
-    if (!half) meet();
-  } else {
-    auto both = [&](const char* a_lds, const char* b_lds) {
-      read(a_lds, b_lds, 0);
-      multiply();
-      __builtin_amdgcn_sched_barrier(0);      // one half's operands in registers at a time
-      read(a_lds, b_lds, 1);
-      multiply();
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    for (int64_t pair = 0; pair < steps / 2; ++pair) {
-      fetch(a_lds1, b_lds1, (2 * pair + 1) * 128);
-      both(a_lds0, b_lds0);
-      __syncthreads();
-      if (2 * pair + 2 < steps) fetch(a_lds0, b_lds0, (2 * pair + 2) * 128);
-      both(a_lds1, b_lds1);
-      __syncthreads();
-    }
-    if (steps & 1) both(a_lds0, b_lds0);
+  auto both = [&](const char* a_lds, const char* b_lds) {
+    read(a_lds, b_lds, 0);
+    multiply();
+    __builtin_amdgcn_sched_barrier(0);      // one half's operands in registers at a time
+    read(a_lds, b_lds, 1);
+    multiply();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int64_t pair = 0; pair < steps / 2; ++pair) {
+    fetch(a_lds1, b_lds1, (2 * pair + 1) * 128);
+    both(a_lds0, b_lds0);
+    __syncthreads();
+    if (2 * pair + 2 < steps) fetch(a_lds0, b_lds0, (2 * pair + 2) * 128);
+    both(a_lds1, b_lds1);
+    __syncthreads();
   }
+  if (steps & 1) both(a_lds0, b_lds0);
 
   if (p.partial != nullptr) {
     i32x4* to = p.partial + (((static_cast<int64_t>(blockIdx.y) * total + tile) * (WM * WN) + wave) * (S::kMI * S::kNI)) * kWave + lane;
@@ -426,6 +382,156 @@ __global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tile
   }
 #pragma unroll
   for (int i = 0; i < S::kMI; ++i) finish_rows<T, S, kGated>(p, m0, n0, wm * S::kRowsM + i * 16, wn, lane, acc[i]);
+}
+
+// The 256 x 256 tile of 8 waves (2 x 4), where the products are large enough for the matrix cores to be
+// the bound.  Two waves share a SIMD, one of each half of the block (wave / 4), and the halves run half a
+// phase apart: while one half's waves read their operands from LDS, the other's multiply.
+//
+// k goes in runs of 64 bytes, of which LDS holds four in a ring (32 KB each: 256 rows of A, 256 slots of B).
+// Run u is read in phase 2 u by the first half and in phase 2 u + 1 by the second, and multiplied in the phase
+// after; every phase ends at a barrier of the whole block (the second half passes one more before its first
+// phase, the first half one more behind its last).  Before it reads run u a half fetches run u + 3: into the
+// ring's place of run u - 1, which was last read in phase 2 u - 1, whose reads had landed (lgkmcnt(0)) before
+// the barrier that ended it.  Run u + 1 is first read in phase 2 u + 2: at the end of their reading phases 2 u
+// and 2 u + 1 both halves have waited until no more than the 8 loads of runs u + 2 and u + 3 are under way.  So
+// a load has four phases, over 2000 cycles, to arrive.
+//
+// LDS rows are 64 bytes; piece c of row r lies at c ^ ((r >> 2) & 3): the 16 rows of an operand fall on all banks.
+template <typename T, bool kGated>
+__global__ void __launch_bounds__(512) tile256_kernel(Product p, int tiles_m, int tiles_n) {
+  using S = TileShape<256, 256, 2, 4, kGated>;
+  using Acc = typename Mma<T>::Acc;
+  constexpr int kStage = 2 * 256 * 64;
+  __shared__ __attribute__((aligned(1024))) char stage0[kStage];
+  __shared__ __attribute__((aligned(1024))) char stage1[kStage];
+  __shared__ __attribute__((aligned(1024))) char stage2[kStage];
+  __shared__ __attribute__((aligned(1024))) char stage3[kStage];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int total = tiles_m * tiles_n;
+  const int tile = xcd_tile(blockIdx.x, total);
+  int tm, tn;
+  tile_place(tile, tiles_m, tiles_n, &tm, &tn);
+  const int64_t m0 = static_cast<int64_t>(tm) * 256, n0 = static_cast<int64_t>(tn) * S::kColsOut;
+
+  // a lane fetches one piece of each of two rows of A and two slots of B a run
+  const int64_t k_first = static_cast<int64_t>(blockIdx.y) * p.slice_bytes;
+  const int64_t kbytes = p.kbytes - k_first < p.slice_bytes ? p.kbytes - k_first : p.slice_bytes;
+  const bool up = kGated && ((wave >> 1) & 1);          // slots 32 to 63 of each 64 are the second B's
+  const uint32_t lda = static_cast<uint32_t>(p.lda), ldb = static_cast<uint32_t>(up ? p.ldb1 : p.ldb0);
+  const char* a_base = p.a + m0 * p.lda + k_first;
+  const char* b_base = (up ? p.b1 + n0 * p.ldb1 : p.b0 + n0 * p.ldb0) + k_first;
+  const int rows_left = p.m - m0 < 256 ? static_cast<int>(p.m - m0) : 256;
+  const int cols_left = p.n - n0 < S::kColsOut ? static_cast<int>(p.n - n0) : S::kColsOut;
+  const int piece_at = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+  uint32_t oa[2], ob[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = j * 128 + wave * 16 + (lane >> 2);
+    oa[j] = static_cast<uint32_t>(r < rows_left ? r : rows_left - 1) * lda + piece_at;       // rows behind the last are not stored
+    int which;
+    const int c = slot_column<kGated>(r, &which);
+    ob[j] = static_cast<uint32_t>(c < cols_left ? c : cols_left - 1) * ldb + piece_at;
+  }
+  const char* zero = reinterpret_cast<const char*>(&kZeroPiece);
+  auto fetch = [&](char* stage, int64_t run) {          // a run that the row fills
+    const int64_t k0 = run * 64;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      __builtin_amdgcn_global_load_lds((gptr_t)(a_base + k0 + oa[j]), (lptr_t)(stage + (j * 128 + wave * 16) * 64), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gptr_t)(b_base + k0 + ob[j]), (lptr_t)(stage + 16384 + (j * 128 + wave * 16) * 64), 16, 0, 0);
+    }
+  };
+  auto fetch_last = [&](char* stage, int64_t run) {     // one that it may not fill
+    const int64_t k0 = run * 64;
+    const bool in = piece_at < kbytes - k0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      __builtin_amdgcn_global_load_lds((gptr_t)(in ? a_base + k0 + oa[j] : zero), (lptr_t)(stage + (j * 128 + wave * 16) * 64), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gptr_t)(in ? b_base + k0 + ob[j] : zero),
+                                       (lptr_t)(stage + 16384 + (j * 128 + wave * 16) * 64), 16, 0, 0);
+    }
+  };
+
+  Acc acc[S::kMI][S::kNI];
+#pragma unroll
+  for (int i = 0; i < S::kMI; ++i)
+#pragma unroll
+    for (int j = 0; j < S::kNI; ++j) acc[i][j] = Acc{};
+  const int half = wave >> 2, wn = wave & 3;
+  const int l15 = lane & 15, q = lane >> 4;
+  const int a_at = (half * 128 + l15) * 64 + (q ^ ((l15 >> 2) & 3)) * 16;
+  const int b_at = 16384 + (wn * 64 + l15) * 64 + (q ^ ((l15 >> 2) & 3)) * 16;
+  auto meet = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // Until a wave's LDS reads have landed and no more than the loads of two runs are under way.  (The builtin,
+  // whose counts the compiler takes into account: it adds no waits of its own.)
+  auto wait_loads = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0078);        // vmcnt(8) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+  };
+  const int64_t runs = (kbytes + 63) / 64;
+  // run u in `now`, run u + 3 into `then`; kAll: the row fills it (else zeros behind its end, so that the
+  // number of loads under way is always the same)
+  auto run_step = [&](const char* now, char* then, int64_t u, auto all) {
+    constexpr bool kAll = decltype(all)::value;
+    i32x4 a[S::kMI], b[S::kNI];
+    if constexpr (kAll) fetch(then, u + 3);
+    else fetch_last(then, u + 3);
+#pragma unroll
+    for (int j = 0; j < S::kNI; ++j) b[j] = *reinterpret_cast<const i32x4*>(now + b_at + j * 1024);
+#pragma unroll
+    for (int i = 0; i < S::kMI; ++i) a[i] = *reinterpret_cast<const i32x4*>(now + a_at + i * 1024);
+    wait_loads();
+    meet();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < S::kMI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::kNI; ++j) acc[i][j] = Mma<T>::mma(b[j], a[i], acc[i][j]);
+    __builtin_amdgcn_s_setprio(0);
+    meet();
+  };
+  fetch_last(stage0, 0);
+  fetch_last(stage1, 1);
+  fetch_last(stage2, 2);
+  wait_loads();
+  meet();
+  if (half) meet();
+  int64_t u = 0;
+  const int64_t whole = kbytes / 64;                     // runs that the row fills
+  for (; u + 7 <= whole; u += 4) {
+    run_step(stage0, stage3, u, std::true_type{});
+    run_step(stage1, stage0, u + 1, std::true_type{});
+    run_step(stage2, stage1, u + 2, std::true_type{});
+    run_step(stage3, stage2, u + 3, std::true_type{});
+  }
+  for (; u < runs; u += 4) {
+    run_step(stage0, stage3, u, std::false_type{});
+    if (u + 1 < runs) run_step(stage1, stage0, u + 1, std::false_type{});
+    if (u + 2 < runs) run_step(stage2, stage1, u + 2, std::false_type{});
+    if (u + 3 < runs) run_step(stage3, stage2, u + 3, std::false_type{});
+  }
+  if (!half) meet();
+  __builtin_amdgcn_s_waitcnt(0x0070);        // no load is under way into LDS when the block gives it back
+
+  if (p.partial != nullptr) {
+    i32x4* to = p.partial + ((static_cast<int64_t>(blockIdx.y) * total + tile) * 8 + wave) * (S::kMI * S::kNI) * kWave + lane;
+#pragma unroll
+    for (int i = 0; i < S::kMI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::kNI; ++j) to[(i * S::kNI + j) * kWave] = __builtin_bit_cast(i32x4, acc[i][j]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < S::kMI; ++i) finish_rows<T, S, kGated>(p, m0, n0, half * 128 + i * 16, wn, lane, acc[i]);
 }
 
 // The slices' sums of a split product, added in order by waves that each take the 16 rows that one wave
@@ -570,8 +676,12 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated) {
 
 template <typename T, bool kGated, int kTile, int WM, int WN>
 void launch_tiles(Product& p, const Plan& plan, int64_t tm, int64_t tn, hipStream_t stream) {
-  hipLaunchKernelGGL((tile_kernel<T, kTile, kTile, WM, WN, kGated>), dim3(static_cast<unsigned>(tm * tn), plan.slices),
-                     dim3(WM * WN * kWave), 0, stream, p, static_cast<int>(tm), static_cast<int>(tn));
+  const dim3 grid(static_cast<unsigned>(tm * tn), plan.slices);
+  if constexpr (kTile == 256)
+    hipLaunchKernelGGL((tile256_kernel<T, kGated>), grid, dim3(512), 0, stream, p, static_cast<int>(tm), static_cast<int>(tn));
+  else
+    hipLaunchKernelGGL((tile_kernel<T, kTile, kTile, WM, WN, kGated>), grid, dim3(WM * WN * kWave), 0, stream, p,
+                       static_cast<int>(tm), static_cast<int>(tn));
   if (plan.slices > 1) {
     const int64_t units = tm * tn * (kTile * kTile / (16 * 64));
     hipLaunchKernelGGL((join_kernel<T, kTile, kTile, WM, WN, kGated>), dim3(static_cast<unsigned>(cdiv(units, 4))), dim3(256), 0,

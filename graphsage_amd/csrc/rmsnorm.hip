@@ -40,17 +40,24 @@ __device__ inline float to_f(T v) { return static_cast<float>(v); }
 template <typename T>
 __device__ inline T from_f(float v) { return static_cast<T>(v); }   // round to nearest even
 
+// a vector of a row, zeros behind its end
 template <typename T>
-__device__ inline void load_vec(const T* p, int64_t at, int64_t dim, float (&v)[VecOf<T>::n]) {
+__device__ inline Pack<T> load_pack(const T* p, int64_t at, int64_t dim) {
   constexpr int n = VecOf<T>::n;
+  Pack<T> k;
   if (at + n <= dim) {
-    const Pack<T> k = *reinterpret_cast<const Pack<T>*>(p + at);
-#pragma unroll
-    for (int i = 0; i < n; ++i) v[i] = to_f(k.v[i]);
+    k = *reinterpret_cast<const Pack<T>*>(p + at);
   } else {
 #pragma unroll
-    for (int i = 0; i < n; ++i) v[i] = at + i < dim ? to_f(p[at + i]) : 0.f;
+    for (int i = 0; i < n; ++i) k.v[i] = at + i < dim ? p[at + i] : static_cast<T>(0.f);
   }
+  return k;
+}
+template <typename T>
+__device__ inline void load_vec(const T* p, int64_t at, int64_t dim, float (&v)[VecOf<T>::n]) {
+  const Pack<T> k = load_pack<T>(p, at, dim);
+#pragma unroll
+  for (int i = 0; i < VecOf<T>::n; ++i) v[i] = to_f(k.v[i]);
 }
 
 template <typename T>
@@ -194,17 +201,21 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
   float w[kNV][n];
   float ss = 0.f;
   uint32_t top = 0;
+  {
+    Pack<T> px[kNV], pr[kNV];     // all of a row's loads before the first use
 #pragma unroll
-  for (int j = 0; j < kNV; ++j) {
-    const int64_t at = static_cast<int64_t>(j * kTPR + t) * n;
-    load_vec<T>(x, at, a.dim, s[j]);
+    for (int j = 0; j < kNV; ++j) px[j] = load_pack<T>(x, static_cast<int64_t>(j * kTPR + t) * n, a.dim);
     if (r != nullptr) {
-      float b[n];
-      load_vec<T>(r, at, a.dim, b);
 #pragma unroll
-      for (int i = 0; i < n; ++i) s[j][i] += b[i];
+      for (int j = 0; j < kNV; ++j) pr[j] = load_pack<T>(r, static_cast<int64_t>(j * kTPR + t) * n, a.dim);
     }
-    load_weight<T>(static_cast<const T*>(a.w), a.w32, at, a.dim, w[j]);
+#pragma unroll
+    for (int j = 0; j < kNV; ++j)
+      load_weight<T>(static_cast<const T*>(a.w), a.w32, static_cast<int64_t>(j * kTPR + t) * n, a.dim, w[j]);
+#pragma unroll
+    for (int j = 0; j < kNV; ++j)
+#pragma unroll
+      for (int i = 0; i < n; ++i) s[j][i] = r != nullptr ? to_f(px[j].v[i]) + to_f(pr[j].v[i]) : to_f(px[j].v[i]);
   }
 #pragma unroll
   for (int j = 0; j < kNV; ++j) {
@@ -316,8 +327,9 @@ struct NormBwdArgs {
   float eps;
 };
 
-// Rows r = first, first + step, ... of a block; dw's column sums stay in registers until the block's
-// last row and are written once as a partial row (summed in a fixed order by dweight_sum_kernel).
+// A block goes over rows r, r + step, ...; dw's column sums stay in registers until its last row and are
+// written once, as the block's partial row (dweight_sum_kernel adds those in a fixed order).  A row's three
+// inputs are all loaded before the first is used, and kept in their own type.
 template <typename T, int kTPR, int kNV>
 __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_bwd_kernel(NormBwdArgs a) {
   constexpr int n = VecOf<T>::n;
@@ -326,7 +338,6 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
   __shared__ float lds_a[2][16];
   __shared__ float lds_b[2][16];
   const int t = threadIdx.x % kTPR;
-  const int64_t lane_row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   float w[kNV][n];
   float acc[kNV][n];
@@ -337,23 +348,29 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
     for (int i = 0; i < n; ++i) acc[j][i] = 0.f;
   }
   int flip = 0;
-  for (int64_t row = lane_row; row < a.rows; row += step) {
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; row < a.rows; row += step) {
     const T* sp = static_cast<const T*>(a.s) + row * a.ld_s;
     const T* yp = static_cast<const T*>(a.dy) + row * a.ld_dy;
-    float s[kNV][n], g[kNV][n];
-    float ss = 0.f, dot = 0.f;
+    const T* dsp = a.ds ? static_cast<const T*>(a.ds) + row * a.ld_ds : nullptr;
+    Pack<T> s[kNV], g[kNV], d[kNV];
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
       const int64_t at = static_cast<int64_t>(j * kTPR + t) * n;
-      load_vec<T>(sp, at, a.dim, s[j]);
-      load_vec<T>(yp, at, a.dim, g[j]);
+      s[j] = load_pack<T>(sp, at, a.dim);
+      g[j] = load_pack<T>(yp, at, a.dim);
     }
+    if (dsp != nullptr) {
+#pragma unroll
+      for (int j = 0; j < kNV; ++j) d[j] = load_pack<T>(dsp, static_cast<int64_t>(j * kTPR + t) * n, a.dim);
+    }
+    float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
 #pragma unroll
       for (int i = 0; i < n; ++i) {
-        ss += s[j][i] * s[j][i];
-        dot += g[j][i] * w[j][i] * s[j][i];
+        const float v = to_f(s[j].v[i]);
+        ss += v * v;
+        dot += to_f(g[j].v[i]) * w[j][i] * v;
       }
     }
     ss = wave_add(ss);
@@ -377,36 +394,48 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
     }
     const float rstd = 1.f / sqrtf(ss / static_cast<float>(a.dim) + a.eps);
     const float c = dot * rstd / static_cast<float>(a.dim);          // mean(dy * w * xh)
-    const T* dsp = a.ds ? static_cast<const T*>(a.ds) + row * a.ld_ds : nullptr;
     T* dxp = static_cast<T*>(a.dx) + row * a.ld_dx;
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
-      const int64_t at = static_cast<int64_t>(j * kTPR + t) * n;
       float o[n];
-      if (dsp != nullptr) {
-        load_vec<T>(dsp, at, a.dim, o);
-      } else {
-#pragma unroll
-        for (int i = 0; i < n; ++i) o[i] = 0.f;
-      }
 #pragma unroll
       for (int i = 0; i < n; ++i) {
-        const float xh = s[j][i] * rstd;
-        acc[j][i] += g[j][i] * xh;
-        o[i] += rstd * (g[j][i] * w[j][i] - xh * c);
+        const float xh = to_f(s[j].v[i]) * rstd, gy = to_f(g[j].v[i]);
+        acc[j][i] += gy * xh;
+        o[i] = rstd * (gy * w[j][i] - xh * c) + (dsp != nullptr ? to_f(d[j].v[i]) : 0.f);
       }
-      if (a.dx != nullptr) store_vec<T>(dxp, at, a.dim, o);
+      if (a.dx != nullptr) store_vec<T>(dxp, static_cast<int64_t>(j * kTPR + t) * n, a.dim, o);
     }
   }
   if (a.part == nullptr) return;
-  // one partial row a row-group: [blocks * kRows, dim]
-  float* part = a.part + lane_row * a.dim;
+  float* part = a.part + static_cast<int64_t>(blockIdx.x) * a.dim;
+  if constexpr (kRows > 1) {
+    // the block's rows' sums, added in wave order
+    __shared__ float lds[kTPR * kNV * n];
+    for (int wave = 0; wave < kRows; ++wave) {
+      if (static_cast<int>(threadIdx.x) / kTPR == wave) {
 #pragma unroll
-  for (int j = 0; j < kNV; ++j) {
-    const int64_t at = static_cast<int64_t>(j * kTPR + t) * n;
+        for (int j = 0; j < kNV; ++j)
 #pragma unroll
-    for (int i = 0; i < n; ++i)
-      if (at + i < a.dim) part[at + i] = acc[j][i];
+          for (int i = 0; i < n; ++i) {
+            float* at = lds + (j * n + i) * kTPR + t;
+            *at = (wave == 0 ? 0.f : *at) + acc[j][i];
+          }
+      }
+      __syncthreads();
+    }
+    for (int e = threadIdx.x; e < kTPR * kNV * n; e += kRowBlock) {
+      const int64_t col = static_cast<int64_t>((e / n / kTPR) * kTPR + e / n % kTPR) * n + e % n;
+      if (col < a.dim) part[col] = lds[((e / n / kTPR) * n + e % n) * kTPR + e / n % kTPR];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kNV; ++j) {
+      const int64_t at = static_cast<int64_t>(j * kTPR + t) * n;
+#pragma unroll
+      for (int i = 0; i < n; ++i)
+        if (at + i < a.dim) part[at + i] = acc[j][i];
+    }
   }
 }
 
@@ -473,21 +502,23 @@ __global__ void __launch_bounds__(1024) rms_norm_bwd_long_kernel(NormBwdArgs a) 
   }
 }
 
-// dw[c] = sum of the partial rows, in their order: 16 rows at a time by 16 threads a column, then those.
+// dw[c] = sum of the partial rows: 64 threads a column take every 64th of them, then one adds the 64 in order.
 template <typename T>
-__global__ void __launch_bounds__(256) dweight_sum_kernel(const float* part, int64_t parts, int64_t dim, T* dw) {
-  __shared__ float lds[16][17];
+__global__ void __launch_bounds__(1024) dweight_sum_kernel(const float* part, int64_t parts, int64_t dim, T* dw) {
+  __shared__ float lds[64][17];
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * 16 + c;
   float v = 0.f;
-  if (col < dim)
-    for (int64_t p = g; p < parts; p += 16) v += part[p * dim + col];
+  if (col < dim) {
+#pragma unroll 8
+    for (int64_t p = g; p < parts; p += 64) v += part[p * dim + col];
+  }
   lds[g][c] = v;
   __syncthreads();
   if (g == 0 && col < dim) {
     v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v += lds[i][c];
+    for (int i = 0; i < 64; ++i) v += lds[i][c];
     dw[col] = from_f<T>(v);
   }
 }
@@ -517,24 +548,36 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, int64_
   }
 }
 
-// How a row of `dim` elements is split: the fewest threads whose registers hold it.
-template <typename T, typename F>
-inline bool with_row_shape(int64_t dim, F&& f) {
-  const int64_t v = cdiv(dim, VecOf<T>::n);
-  if (v <= 64) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-  else if (v <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-  else if (v <= 256) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
-  else if (v <= 512) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-  else if (v <= 1024) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-  else if (v <= 2048) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
-  else if (v <= 4096) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
-  else return false;
-  return true;
+// How a row of v vectors is split: threads and vectors a thread; {0, 0}: longer than the registers hold.
+// With many rows a wave takes a row of up to 256 vectors alone: no barrier, and 4 KB of each input under way
+// a wave.  With few (fewer than the chip's waves) a row's latency counts, and four waves share it.
+struct RowShape {
+  int threads, vectors;
+};
+inline RowShape row_shape(int64_t dim, int n, int64_t rows) {
+  const int64_t v = cdiv(dim, n);
+  const int64_t alone = rows >= 2048 ? 256 : 64;
+  if (v <= alone) return {64, static_cast<int>(cdiv(v, 64))};
+  if (v <= 1024) return {256, static_cast<int>(cdiv(v, 256))};
+  if (v <= 2048) return {1024, 2};
+  if (v <= 4096) return {1024, 4};
+  return {0, 0};
+}
+template <typename F>
+inline bool with_row_shape(RowShape s, F&& f) {
+  using std::integral_constant;
+#define SAGE_SHAPE(TPR, NV) \
+  if (s.threads == TPR && s.vectors == NV) { f(integral_constant<int, TPR>{}, integral_constant<int, NV>{}); return true; }
+  SAGE_SHAPE(64, 1) SAGE_SHAPE(64, 2) SAGE_SHAPE(64, 3) SAGE_SHAPE(64, 4)
+  SAGE_SHAPE(256, 1) SAGE_SHAPE(256, 2) SAGE_SHAPE(256, 3) SAGE_SHAPE(256, 4)
+  SAGE_SHAPE(1024, 2) SAGE_SHAPE(1024, 4)
+#undef SAGE_SHAPE
+  return false;
 }
 
 template <typename T, bool kInt8>
 void launch_norm(const NormArgs& a, hipStream_t stream) {
-  const bool held = with_row_shape<T>(kInt8 ? a.q_cols : a.dim, [&](auto tpr, auto nv) {
+  const bool held = with_row_shape(row_shape(kInt8 ? a.q_cols : a.dim, VecOf<T>::n, a.rows), [&](auto tpr, auto nv) {
     constexpr int kTPR = decltype(tpr)::value, kNV = decltype(nv)::value;
     constexpr int threads = kTPR > kRowBlock ? kTPR : kRowBlock;
     const int64_t blocks = cdiv(a.rows, threads / kTPR);
@@ -553,20 +596,17 @@ int norm_by_type(const NormArgs& a, int dtype, hipStream_t stream, const char* w
   return SAGE_OK;
 }
 
-// Blocks of the backward pass: each of the 256 CUs several, and one partial row of dw for each row group.
-constexpr int64_t kBwdBlocks = 1024;
-inline int64_t bwd_rows_per_block(int64_t dim, int dtype) {
-  return cdiv(dim, dtype == SAGE_F32 ? 4 : 8) <= 128 ? kRowBlock / kWave : 1;
-}
+// Blocks of the backward pass: four for each of the 256 CUs at most, and one partial row of dw for each.
 inline int64_t bwd_blocks(int64_t rows, int64_t dim, int dtype) {
-  const int64_t blocks = cdiv(rows, bwd_rows_per_block(dim, dtype));
-  return blocks < kBwdBlocks ? blocks : kBwdBlocks;
+  const RowShape s = row_shape(dim, dtype == SAGE_F32 ? 4 : 8, rows);
+  const int64_t blocks = cdiv(rows, s.threads == 64 ? kRowBlock / kWave : 1);
+  return blocks < 1024 ? blocks : 1024;
 }
 
 template <typename T>
 void launch_norm_bwd(const NormBwdArgs& a, int dtype, hipStream_t stream) {
   const unsigned blocks = static_cast<unsigned>(bwd_blocks(a.rows, a.dim, dtype));
-  const bool held = with_row_shape<T>(a.dim, [&](auto tpr, auto nv) {
+  const bool held = with_row_shape(row_shape(a.dim, VecOf<T>::n, a.rows), [&](auto tpr, auto nv) {
     constexpr int kTPR = decltype(tpr)::value, kNV = decltype(nv)::value;
     constexpr int threads = kTPR > kRowBlock ? kTPR : kRowBlock;
     hipLaunchKernelGGL((rms_norm_bwd_kernel<T, kTPR, kNV>), dim3(blocks), dim3(threads), 0, stream, a);
@@ -644,7 +684,7 @@ extern "C" int sage_dequantize_rows(const int8_t* q, sage_i64 ld_q, const float*
 
 extern "C" size_t sage_rms_norm_bwd_workspace_bytes(sage_i64 rows, sage_i64 dim, int dtype) {
   if (rows <= 0 || dim <= 0) return 0;
-  return static_cast<size_t>(bwd_blocks(rows, dim, dtype) * bwd_rows_per_block(dim, dtype)) * static_cast<size_t>(dim) * sizeof(float);
+  return static_cast<size_t>(bwd_blocks(rows, dim, dtype)) * static_cast<size_t>(dim) * sizeof(float);
 }
 
 extern "C" int sage_rms_norm_bwd(const void* dy, sage_i64 ld_dy, const void* sum, sage_i64 ld_sum, const void* weight,
@@ -673,14 +713,14 @@ extern "C" int sage_rms_norm_bwd(const void* dy, sage_i64 ld_dy, const void* sum
   else launch_norm_bwd<_Float16>(a, dtype, st);
   SAGE_CHECK_LAUNCH("sage_rms_norm_bwd");
   if (dweight != nullptr) {
-    const int64_t parts = bwd_blocks(rows, dim, dtype) * bwd_rows_per_block(dim, dtype);
+    const int64_t parts = bwd_blocks(rows, dim, dtype);
     const dim3 grid(static_cast<unsigned>(cdiv(dim, 16)));
     if (weight_dtype == SAGE_F32)
-      hipLaunchKernelGGL((dweight_sum_kernel<float>), grid, dim3(256), 0, st, a.part, parts, dim, static_cast<float*>(dweight));
+      hipLaunchKernelGGL((dweight_sum_kernel<float>), grid, dim3(1024), 0, st, a.part, parts, dim, static_cast<float*>(dweight));
     else if (weight_dtype == SAGE_BF16)
-      hipLaunchKernelGGL((dweight_sum_kernel<__bf16>), grid, dim3(256), 0, st, a.part, parts, dim, static_cast<__bf16*>(dweight));
+      hipLaunchKernelGGL((dweight_sum_kernel<__bf16>), grid, dim3(1024), 0, st, a.part, parts, dim, static_cast<__bf16*>(dweight));
     else
-      hipLaunchKernelGGL((dweight_sum_kernel<_Float16>), grid, dim3(256), 0, st, a.part, parts, dim, static_cast<_Float16*>(dweight));
+      hipLaunchKernelGGL((dweight_sum_kernel<_Float16>), grid, dim3(1024), 0, st, a.part, parts, dim, static_cast<_Float16*>(dweight));
     SAGE_CHECK_LAUNCH("sage_rms_norm_bwd");
   }
   return SAGE_OK;

@@ -1335,13 +1335,23 @@ ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(name, device, *args):
-    lib = _lib.load()
-    if device.index == torch.cuda.current_device():
-        rc = getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+    """One entry point on the current stream of `device` (a stream's raw handle: the torch object that
+    wraps it costs as much as the launch).  These operators allocate what they return and work in, so
+    a call tape, which keeps pointers only, does not take them."""
+    if _lib._tape is not None:
+        raise RuntimeError(f"{name}: not recordable on a call tape (capture a graph instead)")
+    fn, index = getattr(_lib.load(), name), device.index
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         _lib.check(rc, name)
 
@@ -1350,23 +1360,22 @@ def _row_matrix(t, name, dtype=None, shape=None, device=None, output=False):
     """2-D device matrix with contiguous rows -> (pointer, row stride in elements)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name}: expected a CUDA (HIP) tensor; graphsage_amd has no CPU path")
-    if t.dim() != 2:
-        raise RuntimeError(f"{name}: expected a 2-D tensor, got shape {tuple(t.shape)}")
-    if dtype is None:
-        if t.dtype not in ROW_DTYPES:
-            raise RuntimeError(f"{name}: expected fp32, bf16 or fp16, got {t.dtype}")
-    elif t.dtype != dtype:
-        raise RuntimeError(f"{name}: expected dtype {dtype}, got {t.dtype}")
-    rows, cols = t.shape
-    if shape is not None and (rows, cols) != shape:
-        raise RuntimeError(f"{name}: expected shape {list(shape)}, got {[rows, cols]}")
+    size = t.shape
+    if len(size) != 2:
+        raise RuntimeError(f"{name}: expected a 2-D tensor, got shape {tuple(size)}")
+    kind = t.dtype
+    if kind is not dtype and (dtype is not None or kind not in ROW_DTYPES):
+        raise RuntimeError(f"{name}: expected {dtype or 'fp32, bf16 or fp16'}, got {kind}")
+    if shape is not None and size != shape:
+        raise RuntimeError(f"{name}: expected shape {list(shape)}, got {list(size)}")
     if device is not None and t.device != device:
         raise RuntimeError(f"{name}: on {t.device}, the other operands on {device}")
     ld, inner = t.stride()
+    rows, cols = size
     if inner != 1 and cols > 1:
         raise RuntimeError(f"{name}: expected contiguous rows, got strides {t.stride()}")
-    if rows <= 1:
-        ld = max(ld, cols)
+    if rows <= 1 and ld < cols:
+        ld = cols
     if output and ld < cols:
         raise RuntimeError(f"{name}: the rows of an output must not overlap")
     return t.data_ptr(), ld
@@ -1390,15 +1399,16 @@ def _activation(name):
     return ACTIVATIONS[name]
 
 
-def _norm_inputs(x, weight, residual, what):
-    px, ldx = _row_matrix(x, f"{what}: x")
-    shape, dev = tuple(x.shape), x.device
+def _norm_inputs(x, weight, residual):
+    px, ldx = _row_matrix(x, "norm: rows")
+    shape, dev, kind = x.shape, x.device, x.dtype
     if shape[1] == 0:
-        raise RuntimeError(f"{what}: rows of no elements")
-    pr, ldr = (None, 0) if residual is None else _row_matrix(residual, f"{what}: residual", x.dtype, shape, dev)
-    pw = None if weight is None else _vector(weight, f"{what}: weight", shape[1], dev, (x.dtype, torch.float32))
-    wd = ROW_DTYPES[x.dtype if weight is None else weight.dtype]
-    return px, ldx, pr, ldr, pw, wd, shape, dev
+        raise RuntimeError("norm: rows of no elements")
+    pr, ldr = (None, 0) if residual is None else _row_matrix(residual, "norm: residual", kind, shape, dev)
+    pw, wd = None, kind
+    if weight is not None:
+        pw, wd = _vector(weight, "norm: weight", shape[1], dev, (kind, torch.float32)), weight.dtype
+    return px, ldx, pr, ldr, pw, ROW_DTYPES[wd], shape, dev
 
 
 def _output(out, name, shape, dtype, device):
@@ -1407,19 +1417,25 @@ def _output(out, name, shape, dtype, device):
     return out
 
 
+def _like(t, out, name):
+    """`out`, checked against t's shape and dtype, or a new tensor: (tensor, pointer, row stride)."""
+    if out is not None:
+        return (out, *_row_matrix(out, name, t.dtype, t.shape, t.device, output=True))
+    out = t.new_empty(t.shape)
+    return out, out.data_ptr(), t.shape[1]
+
+
 def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out=None, sum_out=None):
     """s = x + residual; y = s / sqrt(mean(s^2) + eps) * weight over each row of x [rows, dim]
     (fp32 / bf16 / fp16; weight in x's dtype or fp32).  Returns (y, s); without a residual s is x
     itself.  sum_out may be `residual` (the residual stream updated in place)."""
-    px, ldx, pr, ldr, pw, wd, shape, dev = _norm_inputs(x, weight, residual, "rms_norm_fwd")
+    px, ldx, pr, ldr, pw, wd, shape, dev = _norm_inputs(x, weight, residual)
     if weight is None:
         raise RuntimeError("rms_norm_fwd: weight: tensor required")
-    y = _output(out, "out", shape, x.dtype, dev)
-    py, ldy = _row_matrix(y, "rms_norm_fwd: out", x.dtype, shape, dev, output=True)
-    ps, lds, s = None, 0, x
+    y, py, ldy = _like(x, out, "rms_norm_fwd: out")
+    s, ps, lds = x, None, 0
     if residual is not None:
-        s = _output(sum_out, "sum_out", shape, x.dtype, dev)
-        ps, lds = _row_matrix(s, "rms_norm_fwd: sum_out", x.dtype, shape, dev, output=True)
+        s, ps, lds = _like(x, sum_out, "rms_norm_fwd: sum_out")
     elif sum_out is not None:
         raise RuntimeError("rms_norm_fwd: sum_out without a residual")
     _call("sage_rms_norm_fwd", dev, px, ldx, pr, ldr, pw, wd, shape[0], shape[1], ROW_DTYPES[x.dtype], eps,
@@ -1427,18 +1443,17 @@ def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out=None, sum_out=None):
     return y, s
 
 
-def _int8_rows(x, weight, residual, eps, normalise, padded, sum_out, what):
-    px, ldx, pr, ldr, pw, wd, shape, dev = _norm_inputs(x, weight, residual, what)
+def _int8_rows(x, weight, residual, eps, normalise, padded, sum_out):
+    px, ldx, pr, ldr, pw, wd, shape, dev = _norm_inputs(x, weight, residual)
     rows, dim = shape
     wide = (dim + 15) // 16 * 16
     q = torch.empty((rows, wide), dtype=torch.int8, device=dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    ps, lds, s = None, 0, x
+    s, ps, lds = x, None, 0
     if residual is not None:
-        s = _output(sum_out, "sum_out", shape, x.dtype, dev)
-        ps, lds = _row_matrix(s, f"{what}: sum_out", x.dtype, shape, dev, output=True)
+        s, ps, lds = _like(x, sum_out, "rms_norm_int8: sum_out")
     elif sum_out is not None:
-        raise RuntimeError(f"{what}: sum_out without a residual")
+        raise RuntimeError("rms_norm_int8: sum_out without a residual")
     _call("sage_rms_norm_int8", dev, px, ldx, pr, ldr, pw, wd, rows, dim, ROW_DTYPES[x.dtype], eps, normalise,
           q.data_ptr(), wide, wide, scale.data_ptr(), ps, lds)
     return (q if padded or wide == dim else q[:, :dim]), scale, s
@@ -1451,12 +1466,12 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6, padded=False, sum_out=None
     8-bit product with weights padded alike takes them as they are."""
     if weight is None:
         raise RuntimeError("rms_norm_int8: weight: tensor required")
-    return _int8_rows(x, weight, residual, eps, 1, padded, sum_out, "rms_norm_int8")
+    return _int8_rows(x, weight, residual, eps, 1, padded, sum_out)
 
 
 def quantize_rows(x, padded=False):
     """(q int8, scale fp32 [rows]) with x ~ q * scale: each row by its largest magnitude over 127."""
-    return _int8_rows(x, None, None, 0.0, 0, padded, None, "quantize_rows")[:2]
+    return _int8_rows(x, None, None, 0.0, 0, padded, None)[:2]
 
 
 def dequantize_rows(q, scale, dtype=torch.float32, out=None):
@@ -1477,11 +1492,11 @@ def dequantize_rows(q, scale, dtype=torch.float32, out=None):
 def rms_norm_bwd(dy, s, weight, eps=1e-6, dsum=None, need_dx=True, need_dw=True):
     """Backward of rms_norm_fwd from the stored sum s: (dx, dweight).  dx is the gradient of x and of
     the residual alike; dsum is the gradient that reaches s over the residual stream."""
-    ps, lds, pd, ldd, pw, wd, shape, dev = _norm_inputs(s, weight, dsum, "rms_norm_bwd")
+    ps, lds, pd, ldd, pw, wd, shape, dev = _norm_inputs(s, weight, dsum)
     if weight is None or not (need_dx or need_dw):
         raise RuntimeError("rms_norm_bwd: a weight, and a gradient to compute")
     py, ldy = _row_matrix(dy, "rms_norm_bwd: dy", s.dtype, shape, dev)
-    dx = torch.empty(shape, dtype=s.dtype, device=dev) if need_dx else None
+    dx = s.new_empty(shape) if need_dx else None
     if shape[0] == 0:
         return dx, torch.zeros_like(weight) if need_dw else None
     dw = ws = None
@@ -1518,63 +1533,74 @@ def _product_workspace(m, n, row_bytes, gated, device):
     return ws.data_ptr(), size, ws
 
 
-def _int8_operand(q, scale, name, k=None, device=None):
-    p, ld = _row_matrix(q, name, torch.int8, None, device)
-    if q.size(1) == 0 or (k is not None and q.size(1) != k):
-        raise RuntimeError(f"{name}: expected rows of {k if k else 'some'} elements, got {q.size(1)}")
-    ps = _vector(scale, f"{name} scale", q.size(0), q.device)
-    return p, ld, ps
+def _product_output(out, name, shape, dtype, device):
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+        return out, out.data_ptr(), shape[1]
+    return (out, *_row_matrix(out, name, dtype, shape, device, output=True))
 
 
-def _int8_product(name, x, x_scale, weights, extra, out_dtype, out):
+def _int8_weight(w, scale, k, device):
+    pw, ldw = _row_matrix(w, "8-bit product: weight", torch.int8, None, device)
+    n, wk = w.shape
+    if wk != k or n == 0:
+        raise RuntimeError(f"8-bit product: weight of shape {[n, wk]} for rows of {k} elements")
+    ps = _vector(scale, "8-bit product: weight scale", n, device)
+    return (*_pieces(w, pw, ldw), ps, n)
+
+
+def _int8_rows_in(x, x_scale, out_dtype):
     if out_dtype not in ROW_DTYPES:
-        raise RuntimeError(f"{name}: output in fp32, bf16 or fp16, not {out_dtype}")
-    px, ldx, psx = _int8_operand(x, x_scale, f"{name}: x")
-    (m, k), dev = x.shape, x.device
-    n = weights[0][0].size(0)
-    given = []
-    for w, scale in weights:
-        pw, ldw, psw = _int8_operand(w, scale, f"{name}: weight", k, dev)
-        if w.size(0) != n or n == 0:
-            raise RuntimeError(f"{name}: weights of {w.size(0)} rows")
-        given.append((w, pw, ldw, psw))
-    out = _output(out, "out", (m, n), out_dtype, dev)
-    po, ldo = _row_matrix(out, f"{name}: out", out_dtype, (m, n), dev, output=True)
-    if m == 0:
-        return out
-    px, ldx, wide, keep = _pieces(x, px, ldx)
-    args, kept = [], [keep]
-    for w, pw, ldw, psw in given:
-        pw, ldw, _, keep = _pieces(w, pw, ldw)
-        args += [pw, ldw, psw]
-        kept.append(keep)
-    ws, ws_bytes, keep = _product_workspace(m, n, wide, len(weights) - 1, dev)
-    _call(f"sage_{name}", dev, px, ldx, psx, *args, extra(n, dev), m, n, wide, ROW_DTYPES[out_dtype], po, ldo, ws, ws_bytes)
-    return out
+        raise RuntimeError(f"8-bit product: output in fp32, bf16 or fp16, not {out_dtype}")
+    px, ldx = _row_matrix(x, "8-bit product: x", torch.int8)
+    m, k = x.shape
+    if k == 0:
+        raise RuntimeError("8-bit product: rows of no elements")
+    dev = x.device
+    return px, ldx, _vector(x_scale, "8-bit product: x scale", m, dev), m, k, dev
 
 
 def int8_linear(x, x_scale, weight, w_scale, bias=None, out_dtype=torch.float32, out=None):
     """out[m, n] = x_scale[m] * w_scale[n] * (x @ weight^T)[m, n] + bias[n] for int8 x [m, k] and weight
     [n, k] (k <= 131056: the integer sum is exact), fp32 scales and bias."""
-    return _int8_product("int8_linear", x, x_scale, [(weight, w_scale)],
-                         lambda n, dev: None if bias is None else _vector(bias, "int8_linear: bias", n, dev), out_dtype, out)
+    px, ldx, psx, m, k, dev = _int8_rows_in(x, x_scale, out_dtype)
+    pw, ldw, _, keep_w, psw, n = _int8_weight(weight, w_scale, k, dev)
+    pb = None if bias is None else _vector(bias, "int8_linear: bias", n, dev)
+    out, po, ldo = _product_output(out, "int8_linear: out", (m, n), out_dtype, dev)
+    if m > 0:
+        px, ldx, wide, keep_x = _pieces(x, px, ldx)
+        ws, ws_bytes, keep = _product_workspace(m, n, wide, 0, dev)
+        _call("sage_int8_linear", dev, px, ldx, psx, pw, ldw, psw, pb, m, n, wide, ROW_DTYPES[out_dtype], po, ldo,
+              ws, ws_bytes)
+    return out
 
 
 def int8_gated_linear(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation="silu", out_dtype=torch.float32, out=None):
     """activation(x @ w_gate^T) * (x @ w_up^T), both 8-bit products with token and channel scales."""
     act = _activation(activation)
-    return _int8_product("int8_gated_linear", x, x_scale, [(w_gate, gate_scale), (w_up, up_scale)], lambda n, dev: act,
-                         out_dtype, out)
+    act = _activation(activation)
+    px, ldx, psx, m, k, dev = _int8_rows_in(x, x_scale, out_dtype)
+    pg, ldg, _, keep_g, psg, n = _int8_weight(w_gate, gate_scale, k, dev)
+    pu, ldu, _, keep_u, psu, nu = _int8_weight(w_up, up_scale, k, dev)
+    if n != nu:
+        raise RuntimeError(f"int8_gated_linear: weights of {n} and {nu} rows")
+    out, po, ldo = _product_output(out, "int8_gated_linear: out", (m, n), out_dtype, dev)
+    if m > 0:
+        px, ldx, wide, keep_x = _pieces(x, px, ldx)
+        ws, ws_bytes, keep = _product_workspace(m, n, wide, 1, dev)
+        _call("sage_int8_gated_linear", dev, px, ldx, psx, pg, ldg, psg, pu, ldu, psu, act, m, n, wide,
+              ROW_DTYPES[out_dtype], po, ldo, ws, ws_bytes)
+    return out
 
 
-def _gated_inputs(x, w_gate, w_up, what):
-    px, ldx = _row_matrix(x, f"{what}: x")
-    (m, k), dev = x.shape, x.device
-    pg, ldg = _row_matrix(w_gate, f"{what}: w_gate", x.dtype, (w_gate.size(0), k) if isinstance(w_gate, torch.Tensor) else None, dev)
-    h = w_gate.size(0)
-    pu, ldu = _row_matrix(w_up, f"{what}: w_up", x.dtype, (h, k), dev)
-    if h == 0 or k == 0:
-        raise RuntimeError(f"{what}: weights of shape {[h, k]}")
+def _gated_inputs(x, w_gate, w_up):
+    px, ldx = _row_matrix(x, "gated_linear: x")
+    (m, k), dev, kind = x.shape, x.device, x.dtype
+    pg, ldg = _row_matrix(w_gate, "gated_linear: w_gate", kind, None, dev)
+    h, wk = w_gate.shape
+    if wk != k or h == 0 or k == 0:
+        raise RuntimeError(f"gated_linear: weights of shape {[h, wk]} for rows of {k} elements")
+    pu, ldu = _row_matrix(w_up, "gated_linear: w_up", kind, (h, k), dev)
     return px, ldx, pg, ldg, pu, ldu, m, h, k, dev
 
 
@@ -1582,10 +1608,9 @@ def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
     """activation(x @ w_gate^T) * (x @ w_up^T) for x [m, k], weights [h, k] of one dtype (fp32 / bf16 /
     fp16; fp32 sums).  Returns (out [m, h], saved): with save, saved [2, m, h] holds both products in
     fp32 for gated_linear_bwd, else None."""
-    px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up, "gated_linear_fwd")
+    px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up)
     act = _activation(activation)
-    out = _output(out, "out", (m, h), x.dtype, dev)
-    po, ldo = _row_matrix(out, "gated_linear_fwd: out", x.dtype, (m, h), dev, output=True)
+    out, po, ldo = _product_output(out, "gated_linear_fwd: out", (m, h), x.dtype, dev)
     saved = torch.empty((2, m, h), dtype=torch.float32, device=dev) if save else None
     if m == 0:
         return out, saved
@@ -1601,7 +1626,7 @@ def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
 def gated_linear_bwd(dh, x, w_gate, w_up, saved, activation="silu", need_dx=True, need_dw=True):
     """Gradients of gated_linear_fwd: (dx, dw_gate, dw_up); the two weight gradients are the halves of
     one [2 h, k] buffer."""
-    px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up, "gated_linear_bwd")
+    px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up)
     act = _activation(activation)
     pd, ldd = _row_matrix(dh, "gated_linear_bwd: dh", x.dtype, (m, h), dev)
     if not isinstance(saved, torch.Tensor) or saved.shape != (2, m, h) or saved.dtype != torch.float32 or \
