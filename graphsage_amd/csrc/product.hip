@@ -259,7 +259,7 @@ __device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool kGated>
-__global__ void __launch_bounds__(WM* WN* kWave) tile_kernel(Product p, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(WM* WN* kWave, 2) tile_kernel(Product p, int tiles_m, int tiles_n) {
   using S = TileShape<BM, BN, WM, WN, kGated>;
   using Acc = typename Mma<T>::Acc;
   __shared__ __attribute__((aligned(1024))) char a_lds0[BM * 128];
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(256) join_kernel(Product p, int tiles_m, int t
 }
 
 // ------------------------------------------------------------------------------- few rows
-// Up to 16 * MT rows of A against the whole of B: B is read once, straight into the registers that
+// 16 * MT rows of A (grid y: more of them) against the whole of B: B goes straight into the registers that
 // the MFMAs take, so the kernel is as fast as B's bytes arrive.  A block owns 16 columns (gated: 16 of
 // each B); its waves take k in runs of 256 bytes in turn and add their sums in LDS, in wave order.
 constexpr int kFewWaves = 8;
@@ -642,29 +642,47 @@ inline bool rows16(const void* p, int64_t ld_bytes) {
 }
 constexpr int64_t kMaxRowBytes = int64_t{1} << 23;     // the tile loads' offsets: 256 rows in 31 bits
 
-// How a product is cut: few rows; or tiles of `tile` x `tile` (gated: `tile` / 2 columns), k in `slices`.
+// How a product is cut: blocks of 64 rows and 16 columns (tile 0: few_rows_kernel), or tiles of `tile` x `tile`
+// (gated: `tile` / 2 columns), k in `slices`.
 struct Plan {
-  int tile, slices;      // tile 0: few_rows_kernel
+  int tile, slices;
   int64_t slice_bytes;
   size_t workspace;
 };
 
-inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated) {
+// The cut with the least estimated time.  The estimate, in microseconds, follows measurements of every cut at
+// m 32 to 2048 against 1024 x 1024, 4096 x 4096, 8192 x 2048 and 2048 x 8192 in 8 bits, bf16 and fp32 (its choice
+// is 1.2 % slower than the best cut there in the geometric mean, never more than 16 %):
+//   few rows: a block's bytes of k at 2.3 us a kilobyte-thousand (more with two Bs, and in fp32, where the MFMAs
+//     count), blocks in turns of one a CU;
+//   tiles: a step of 128 bytes of k takes a CU 1.6 us at 256 x 256 (1.2 while half of the chip is idle); at
+//     128 x 128 0.65 us alone and 1.0 us for the two that share a CU; fp32 is bound by its MFMAs (8, 2.1, 4.1 us);
+//   slices: one more launch, and their sums written and read.
+inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool fp32) {
   Plan best{0, 1, kbytes, 0};
-  if (m <= 64) return best;
+  if (m <= 16) return best;
   const int64_t steps = cdiv(kbytes, 128);
   double least = 1e300;
-  for (int tile : {256, 128}) {
+  if (m <= 512) {
+    const double byte = (fp32 ? 0.0025 : 0.0023) * (gated ? (fp32 ? 1.6 : 1.22) : 1.0) * (m <= 32 ? 0.68 : 1.0);
+    least = 4.0 + cdiv(cdiv(n, 16) * cdiv(m, 64), 256) * kbytes * byte;
+  }
+  for (int tile : {128, 256}) {
     const int64_t tiles = cdiv(m, tile) * cdiv(n, gated ? tile / 2 : tile);
-    // microseconds: a step of 128 bytes of k, a block's start and end, and how many blocks run at once
-    const double step = tile == 256 ? 1.5 : 0.9, ends = tile == 256 ? 6.0 : 4.0;
-    const int64_t at_once = tile == 256 ? 256 : 512;
-    for (int64_t slices = 1; slices <= 32 && slices <= steps; slices *= 2) {
-      const int64_t each = cdiv(steps, slices), used = cdiv(steps, each);
-      if (used != slices) continue;
-      const double bytes = static_cast<double>(slices) * tiles * tile * tile * 4;
-      double time = cdiv(tiles * slices, at_once) * (each * step + ends);
-      if (slices > 1) time += 4.0 + 2.0 * bytes / 4e6;      // written and read at 4 TB/s, one more launch
+    for (int64_t slices = 1; slices <= 32 && 2 * slices <= steps + 1; slices *= 2) {
+      const int64_t each = cdiv(steps, slices), blocks = tiles * slices;
+      if (cdiv(steps, each) != slices) continue;
+      double time;
+      if (tile == 128) {
+        const double alone = fp32 ? 2.1 : blocks <= 128 ? 0.65 : 0.72, pair = fp32 ? 4.1 : 1.0;
+        const int64_t turns = blocks / 512, rest = blocks % 512;
+        time = each * (turns * pair + (rest == 0 ? 0.0 : rest <= 256 ? alone : pair)) + 5.5 + 2.0 * (turns - (rest == 0 ? 1 : 0));
+      } else {
+        const int64_t turns = cdiv(blocks, 256);
+        time = each * turns * (fp32 ? 8.0 : blocks <= 128 ? 1.2 : 1.62) + 9.0 + 5.0 * (turns - 1);
+      }
+      const double bytes = static_cast<double>(blocks) * tile * tile * 4;
+      if (slices > 1) time += 6.0 + 2.0 * bytes / 7e6;
       if (time < least) {
         least = time;
         best = Plan{tile, static_cast<int>(slices), each * 128, slices > 1 ? static_cast<size_t>(bytes) : 0};
@@ -691,11 +709,11 @@ void launch_tiles(Product& p, const Plan& plan, int64_t tm, int64_t tn, hipStrea
 
 template <typename T, bool kGated>
 int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, const char* what) {
-  const Plan plan = plan_product(p.m, p.n, p.kbytes, kGated);
+  const Plan plan = plan_product(p.m, p.n, p.kbytes, kGated, std::is_same<T, float>::value);
   SAGE_REQUIRE(p.lda < kMaxRowBytes && p.ldb0 < kMaxRowBytes && p.ldb1 < kMaxRowBytes, SAGE_ELIMIT, "%s: rows more than %ld bytes apart",
                what, (long)kMaxRowBytes);
   if (plan.tile == 0) {
-    const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), 1);
+    const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), static_cast<unsigned>(cdiv(p.m, 64)));   // m <= 512
     if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
     else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
     else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
@@ -824,8 +842,8 @@ inline BwdLayout bwd_layout(int64_t m, int64_t h, int64_t k, int dtype) {
   l.wt = take(k * l.ld_w);
   // the two products run one after the other and share the room for their slices
   l.part = off;
-  const size_t for_dx = plan_product(m, k, l.ld_rows * size_of(dtype), false).workspace;
-  const size_t for_dw = plan_product(2 * h, k, l.ld_cols * size_of(dtype), false).workspace;
+  const size_t for_dx = plan_product(m, k, l.ld_rows * size_of(dtype), false, dtype == SAGE_F32).workspace;
+  const size_t for_dw = plan_product(2 * h, k, l.ld_cols * size_of(dtype), false, dtype == SAGE_F32).workspace;
   l.part_bytes = for_dx > for_dw ? for_dx : for_dw;
   l.bytes = off + l.part_bytes;
   return l;
@@ -894,9 +912,9 @@ extern "C" int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows
   return SAGE_OK;
 }
 
-extern "C" size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated) {
+extern "C" size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32) {
   if (m <= 0 || n <= 0 || row_bytes <= 0) return 0;
-  return plan_product(m, n, row_bytes, gated != 0).workspace;
+  return plan_product(m, n, row_bytes, gated != 0, fp32 != 0).workspace;
 }
 
 #define SAGE_INT8_CHECKS(what)                                                                                          \

@@ -1524,9 +1524,9 @@ def _pieces(t, p, ld):
     return out.data_ptr(), wide, wide, out
 
 
-def _product_workspace(m, n, row_bytes, gated, device):
-    """(pointer, bytes, owner) of what a product of few tiles splits k into; few rows take none."""
-    size = _lib.load().sage_product_workspace_bytes(m, n, row_bytes, gated) if m > 64 else 0
+def _product_workspace(m, n, row_bytes, gated, fp32, device):
+    """(pointer, bytes, owner) of what a product of few tiles splits k into; the fewest rows take none."""
+    size = _lib.load().sage_product_workspace_bytes(m, n, row_bytes, gated, fp32) if m > 16 else 0
     if size == 0:
         return None, 0, None
     ws = torch.empty(size, dtype=torch.uint8, device=device)
@@ -1569,7 +1569,7 @@ def int8_linear(x, x_scale, weight, w_scale, bias=None, out_dtype=torch.float32,
     out, po, ldo = _product_output(out, "int8_linear: out", (m, n), out_dtype, dev)
     if m > 0:
         px, ldx, wide, keep_x = _pieces(x, px, ldx)
-        ws, ws_bytes, keep = _product_workspace(m, n, wide, 0, dev)
+        ws, ws_bytes, keep = _product_workspace(m, n, wide, 0, 0, dev)
         _call("sage_int8_linear", dev, px, ldx, psx, pw, ldw, psw, pb, m, n, wide, ROW_DTYPES[out_dtype], po, ldo,
               ws, ws_bytes)
     return out
@@ -1587,7 +1587,7 @@ def int8_gated_linear(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation
     out, po, ldo = _product_output(out, "int8_gated_linear: out", (m, n), out_dtype, dev)
     if m > 0:
         px, ldx, wide, keep_x = _pieces(x, px, ldx)
-        ws, ws_bytes, keep = _product_workspace(m, n, wide, 1, dev)
+        ws, ws_bytes, keep = _product_workspace(m, n, wide, 1, 0, dev)
         _call("sage_int8_gated_linear", dev, px, ldx, psx, pg, ldg, psg, pu, ldu, psu, act, m, n, wide,
               ROW_DTYPES[out_dtype], po, ldo, ws, ws_bytes)
     return out
@@ -1617,7 +1617,7 @@ def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
     px, ldx, wide, keep_x = _pieces(x, px, ldx)
     pg, ldg, _, keep_g = _pieces(w_gate, pg, ldg)
     pu, ldu, _, keep_u = _pieces(w_up, pu, ldu)
-    ws, ws_bytes, keep = _product_workspace(m, h, wide * x.element_size(), 1, dev)
+    ws, ws_bytes, keep = _product_workspace(m, h, wide * x.element_size(), 1, x.dtype is torch.float32, dev)
     _call("sage_gated_linear_fwd", dev, px, ldx, pg, ldg, pu, ldu, act, m, h, wide, ROW_DTYPES[x.dtype], po, ldo,
           saved.data_ptr() if save else None, ws, ws_bytes)
     return out, saved

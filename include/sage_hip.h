@@ -794,8 +794,9 @@ int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows, sage_i64 
                   sage_i64 ld_out_bytes, void* stream);
 /* Workspace of a product below (starts on 16 bytes; 0 bytes: none, NULL): where an output has too few
  * tiles to fill the chip, k is split and the slices' sums meet there.  row_bytes is k times the
- * element's size; gated: two weights.  The operands' rows are less than 2^23 bytes apart. */
-size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated);
+ * element's size; gated: two weights; fp32: fp32 operands.  The operands' rows are less than 2^23 bytes
+ * apart. */
+size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32);
 /* out[m, n] = x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]; the sum is exact (32-bit
  * integers, k <= SAGE_INT8_MAX_K), the rest fp32, rounded once to out_dtype.  bias may be NULL. */
 int sage_int8_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w, sage_i64 ld_w,
