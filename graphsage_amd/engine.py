@@ -176,6 +176,8 @@ class SageTrainEngine:
     def __init__(self, model, sampler, features, labels, batch_size, lr=1e-3, betas=(0.9, 0.999),
                  eps=1e-8, weight_decay=0.0, world_size=1, process_group=None, overlap_gather=False,
                  keep_grads=False, group=4, unsup=False, force_collective=False):
+        if getattr(model, 'blocks', None) is not None:
+            raise NotImplementedError("engine: models with feed-forward blocks run on the module path")
         if model.aggregator not in _REDUCE:
             raise NotImplementedError(f"engine supports {sorted(_REDUCE)}, got {model.aggregator}")
         self.model = model

@@ -6,6 +6,7 @@ derives for the reference's unfused ops; tests compare both against the CPU orac
 """
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -194,6 +195,80 @@ class L2NormReLUFn(Function):
     def backward(ctx, dh):
         y, inv = ctx.saved_tensors
         return ops.l2norm_relu_bwd(dh.contiguous(), y, inv, ctx.relu), None
+
+
+class RmsNormFn(Function):
+    """(y, s): s = x + residual, y = s / rms(s) * weight.  Backward from the stored s, so nothing but it
+    and the weight is kept."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        ctx.set_materialize_grads(False)
+        y, s = ops.rms_norm_fwd(_rows(x), weight.contiguous(), None if residual is None else _rows(residual), eps)
+        ctx.save_for_backward(s, weight)
+        ctx.eps, ctx.shape, ctx.has_residual = eps, x.shape, residual is not None
+        return y.view(x.shape), (s.view(x.shape) if residual is not None else None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds):
+        s, weight = ctx.saved_tensors
+        need_dx = ctx.needs_input_grad[0] or (ctx.has_residual and ctx.needs_input_grad[2])
+        need_dw = ctx.needs_input_grad[1]
+        dx = dw = None
+        if dy is None:                   # only the sum was used: its gradient passes through
+            dx = ds
+        elif need_dx or need_dw:
+            dx, dw = ops.rms_norm_bwd(_rows(dy), s, weight.contiguous(), ctx.eps, None if ds is None else _rows(ds),
+                                      need_dx=need_dx, need_dw=need_dw)
+            dx = None if dx is None else dx.view(ctx.shape)
+        return dx, dw, (dx if ctx.has_residual else None), None
+
+
+class GatedLinearFn(Function):
+    """activation(x w_gate^T) * (x w_up^T); both products are kept in fp32 for the backward pass when a
+    gradient will be asked for."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, activation):
+        x2, w_gate, w_up = _rows(x), _rows(w_gate), _rows(w_up)
+        save = any(ctx.needs_input_grad)
+        out, saved = ops.gated_linear_fwd(x2, w_gate, w_up, activation, save=save)
+        if save:
+            ctx.save_for_backward(x2, w_gate, w_up, saved)
+        ctx.activation, ctx.shape = activation, x.shape
+        return out.view(*x.shape[:-1], out.size(1))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, w_gate, w_up, saved = ctx.saved_tensors
+        need_dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dx, dwg, dwu = ops.gated_linear_bwd(_rows(dout), x, w_gate, w_up, saved, ctx.activation,
+                                            need_dx=ctx.needs_input_grad[0], need_dw=need_dw)
+        return (None if dx is None else dx.view(ctx.shape), dwg if ctx.needs_input_grad[1] else None,
+                dwu if ctx.needs_input_grad[2] else None, None)
+
+
+def _rows(t):
+    """[..., n] as a matrix whose rows are contiguous (a copy only where they are not)."""
+    t = t.reshape(-1, t.size(-1)) if t.dim() != 2 else t
+    return t if t.stride(1) == 1 or t.size(1) <= 1 else t.contiguous()
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """s / sqrt(mean(s^2) + eps) * weight over the last dimension of x [..., n] (fp32, bf16, fp16; the weight
+    in x's dtype or fp32), s = x + residual.  Returns y, or (y, s) with a residual: s goes on as the next
+    residual."""
+    y, s = RmsNormFn.apply(x, weight, residual, eps)
+    return y if residual is None else (y, s)
+
+
+def gated_linear(x, w_gate, w_up, activation="silu"):
+    """activation(x @ w_gate^T) * (x @ w_up^T): the two projections of a gated feed-forward block, their
+    activation and product in one kernel.  x [..., k], weights [h, k], all of one dtype (fp32, bf16,
+    fp16); activation 'silu', 'gelu' (erf) or 'relu'."""
+    return GatedLinearFn.apply(x, w_gate, w_up, activation)
 
 
 def gather_reduce(x, plan_or_ptr, src=None, num_targets=None, reduce="mean", node_map=None):

@@ -1,3 +1,4 @@
+from .feed_forward import GatedFeedForward
 from .sage import SAGE
 
-__all__ = ["SAGE"]
+__all__ = ["SAGE", "GatedFeedForward"]

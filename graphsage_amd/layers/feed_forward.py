@@ -1,0 +1,88 @@
+"""Residual feed-forward block behind an aggregation (no counterpart in the reference, whose layers end at
+layers/sage.py:131-134):
+
+    s = x + residual;  out = s + down(act(gate(norm(s))) * up(norm(s)))
+
+norm: root mean square with a learned weight; gate, up, down: bias-free Linears.  The norm adds the
+residual as it reads x, and gate, up, activation and product are one kernel (functional.rms_norm,
+functional.gated_linear).
+
+quantize_() lays the three weights out in 8 bits, one scale a channel, for inference: the norm then
+writes 8 bits with a scale a row, and every product is an 8-bit one.  The 8-bit weights are those of the
+call's moment: train() and load_state_dict() drop them, any other change of the weights needs quantize_()
+again.  They serve calls in eval mode without gradients; every other call takes the fp32 weights.
+"""
+import torch
+
+from .. import functional as SF
+from .. import ops
+
+
+class GatedFeedForward(torch.nn.Module):
+    def __init__(self, channels: int, hidden_channels: int, activation: str = 'silu', eps: float = 1e-6):
+        super().__init__()
+        ops._activation(activation)
+        self.channels, self.hidden_channels = channels, hidden_channels
+        self.activation, self.eps = activation, eps
+        self.norm_weight = torch.nn.Parameter(torch.ones(channels))
+        self.gate = torch.nn.Linear(channels, hidden_channels, bias=False)
+        self.up = torch.nn.Linear(channels, hidden_channels, bias=False)
+        self.down = torch.nn.Linear(hidden_channels, channels, bias=False)
+        self._eight = None
+
+    def reset_parameters(self):
+        self._eight = None
+        with torch.no_grad():
+            self.norm_weight.fill_(1.0)
+        for layer in (self.gate, self.up, self.down):
+            layer.reset_parameters()
+
+    # ------------------------------------------------------------------ 8-bit weights
+    @torch.no_grad()
+    def quantize_(self):
+        self._eight = tuple(ops.quantize_rows(layer.weight, padded=True) for layer in (self.gate, self.up, self.down))
+        return self
+
+    def dequantize_(self):
+        self._eight = None
+        return self
+
+    @property
+    def quantized(self):
+        return self._eight is not None
+
+    def train(self, mode=True):
+        if mode:
+            self._eight = None
+        return super().train(mode)
+
+    def _apply(self, fn, *args, **kwargs):      # .to() and the like: the 8-bit copies stay behind
+        self._eight = None
+        return super()._apply(fn, *args, **kwargs)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._eight = None
+        return super()._load_from_state_dict(*args, **kwargs)
+
+    # ------------------------------------------------------------------ forward
+    def forward(self, x, residual=None):
+        if self._eight is not None and not self.training and not torch.is_grad_enabled():
+            return self._serve(x, residual)
+        if residual is None:
+            y, s = SF.rms_norm(x, self.norm_weight, eps=self.eps), x
+        else:
+            y, s = SF.rms_norm(x, self.norm_weight, residual, self.eps)
+        h = SF.gated_linear(y, self.gate.weight, self.up.weight, self.activation)
+        return s + SF.linear_concat(h, self.down.weight)
+
+    def _serve(self, x, residual):
+        (gate, gate_scale), (up, up_scale), (down, down_scale) = self._eight
+        y, y_scale, s = ops.rms_norm_int8(x, self.norm_weight, residual, self.eps, padded=True)
+        # bf16 between the two products: its rounding is a 128th of the 8-bit step that follows at the row's
+        # largest values, and halves the bytes
+        h = ops.int8_gated_linear(y, y_scale, gate, gate_scale, up, up_scale, self.activation, torch.bfloat16)
+        h, h_scale = ops.quantize_rows(h, padded=True)
+        return ops.int8_linear(h, h_scale, down, down_scale, out_dtype=s.dtype).add_(s)
+
+    def __repr__(self):
+        return f'{self.__class__.__name__}({self.channels}, {self.hidden_channels}, activation={self.activation})'

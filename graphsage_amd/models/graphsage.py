@@ -7,12 +7,16 @@ reference trainers/node_level_graphsage_trainers.py:40, models/graphsage.py:63):
 edge_index comes from UniformLoader (it carries the hop structure) and
 `prune_to_seeds` is True, layer i is evaluated only on the rows that can influence the seed
 rows — hop_nodes[L-1-i] targets — and forward returns [batch_size, C] instead of [N_b, C].
+
+ffn_channels (not in the reference) puts a residual feed-forward block (layers/feed_forward.py) of that
+width behind every layer but the last; from the second layer on the layer's own input is the residual, so
+that deeper stacks have a path around each aggregation.  quantize_() serves those blocks in 8 bits.
 """
 import torch
 
 from .. import functional as SF
 from .. import settings
-from ..layers import SAGE
+from ..layers import SAGE, GatedFeedForward
 
 
 def set_batch_size_attr(batch):
@@ -25,7 +29,7 @@ def set_batch_size_attr(batch):
 
 class GraphSAGE(torch.nn.Module):
     def __init__(self, in_channels: int, hidden_channels: int, aggregator: str = 'mean',
-                 num_layers: int = 2, out_channels=None):
+                 num_layers: int = 2, out_channels=None, ffn_channels=None, ffn_activation: str = 'silu'):
         super().__init__()
         self.aggregator = aggregator
         self.name = 'GraphSAGE-' + aggregator.upper()
@@ -37,6 +41,26 @@ class GraphSAGE(torch.nn.Module):
             [SAGE(hidden_channels, hidden_channels, aggregator) for _ in range(num_layers - 2)] +
             [SAGE(hidden_channels, out_channels, aggregator)]
         )
+        self.blocks = None
+        if ffn_channels is not None:
+            self.blocks = torch.nn.ModuleList([GatedFeedForward(hidden_channels, ffn_channels, ffn_activation)
+                                               for _ in range(len(self.layers) - 1)])
+
+    def quantize_(self):
+        """8-bit weights for the feed-forward blocks (see GatedFeedForward.quantize_); call in eval mode."""
+        if self.blocks is None:
+            raise RuntimeError("quantize_: the model has no feed-forward blocks (ffn_channels)")
+        if self.training:
+            raise RuntimeError("quantize_: call eval() first (train() drops the 8-bit weights)")
+        for block in self.blocks:
+            block.quantize_()
+        return self
+
+    def _feed_forward(self, i, x, x_in):
+        """Block i on layer i's output x; x_in is the layer's input, whose first rows are x's targets."""
+        if self.blocks is None or i >= len(self.blocks):
+            return x
+        return self.blocks[i](x, x_in[:x.size(0)] if i > 0 else None)
 
     def _targets(self, plan, i):
         """Rows of layer i's output that can reach the seed rows through the later layers."""
@@ -50,17 +74,18 @@ class GraphSAGE(torch.nn.Module):
                     and plan.num_src == x.size(0))
         if not prunable:
             for i, layer in enumerate(self.layers):
-                x = layer(x, edge_index)
+                x_in, x = x, layer(x, edge_index)
                 if i < len(self.layers) - 1:
                     # out of place: the normalise Function saved its output for backward (the
                     # reference's relu_() at models/graphsage.py:48 has the same values)
-                    x = x.relu()
+                    x = self._feed_forward(i, x.relu(), x_in)
             return x
         L = len(self.layers)
         for i, layer in enumerate(self.layers):
             t = self._targets(plan, i)
             n_src = plan.hop_nodes[min(L - i, len(plan.hop_nodes) - 1)]
-            x = layer.apply_plan(x, x, plan, t, relu=(i < L - 1), num_src_rows=min(n_src, x.size(0)))
+            x_in, x = x, layer.apply_plan(x, x, plan, t, relu=(i < L - 1), num_src_rows=min(n_src, x.size(0)))
+            x = self._feed_forward(i, x, x_in)
         return x
 
     def forward_batch(self, batch):
@@ -76,8 +101,9 @@ class GraphSAGE(torch.nn.Module):
         for i, layer in enumerate(self.layers):
             t = self._targets(plan, i)
             n_src = plan.hop_nodes[min(L - i, len(plan.hop_nodes) - 1)]
-            x = layer.apply_plan(x, x, plan, t, relu=(i < L - 1), node_map=node_map,
-                                 num_src_rows=n_src)
+            x_in, x = x, layer.apply_plan(x, x, plan, t, relu=(i < L - 1), node_map=node_map,
+                                          num_src_rows=n_src)
+            x = self._feed_forward(i, x, x_in)
             node_map = None
         return x
 

@@ -1533,11 +1533,35 @@ def _product_workspace(m, n, row_bytes, gated, fp32, device):
     return ws.data_ptr(), size, ws
 
 
-def _product_output(out, name, shape, dtype, device):
+def _product_output(out, name, shape, dtype, device, operands):
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=device)
         return out, out.data_ptr(), shape[1]
-    return (out, *_row_matrix(out, name, dtype, shape, device, output=True))
+    p, ld = _row_matrix(out, name, dtype, shape, device, output=True)
+    for t in operands:
+        if t is not None and _overlap(out, t):
+            raise RuntimeError(f"{name}: shares memory with an operand, which blocks still read when others write")
+    return out, p, ld
+
+
+def _span(t):
+    """(first byte, bytes to the end of the last row, row stride, row length) of a matrix or vector."""
+    size, rows = t.element_size(), t.size(0) if t.dim() == 2 else 1
+    ld = t.stride(0) * size if rows > 1 else t.size(-1) * size
+    return t.data_ptr(), (rows - 1) * ld + t.size(-1) * size, ld, t.size(-1) * size
+
+
+def _overlap(a, b):
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    pa, na, lda, wa = _span(a)
+    pb, nb, ldb, wb = _span(b)
+    if pa >= pb + nb or pb >= pa + na:
+        return False
+    if lda == ldb and lda > 0:               # columns of one buffer: apart if they are within every row
+        gap = (pb - pa) % lda
+        return gap < wa or gap + wb > lda
+    return True
 
 
 def _int8_weight(w, scale, k, device):
@@ -1566,7 +1590,7 @@ def int8_linear(x, x_scale, weight, w_scale, bias=None, out_dtype=torch.float32,
     px, ldx, psx, m, k, dev = _int8_rows_in(x, x_scale, out_dtype)
     pw, ldw, _, keep_w, psw, n = _int8_weight(weight, w_scale, k, dev)
     pb = None if bias is None else _vector(bias, "int8_linear: bias", n, dev)
-    out, po, ldo = _product_output(out, "int8_linear: out", (m, n), out_dtype, dev)
+    out, po, ldo = _product_output(out, "int8_linear: out", (m, n), out_dtype, dev, (x, x_scale, weight, w_scale, bias))
     if m > 0:
         px, ldx, wide, keep_x = _pieces(x, px, ldx)
         ws, ws_bytes, keep = _product_workspace(m, n, wide, 0, 0, dev)
@@ -1584,7 +1608,8 @@ def int8_gated_linear(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation
     pu, ldu, _, keep_u, psu, nu = _int8_weight(w_up, up_scale, k, dev)
     if n != nu:
         raise RuntimeError(f"int8_gated_linear: weights of {n} and {nu} rows")
-    out, po, ldo = _product_output(out, "int8_gated_linear: out", (m, n), out_dtype, dev)
+    out, po, ldo = _product_output(out, "int8_gated_linear: out", (m, n), out_dtype, dev,
+                                   (x, x_scale, w_gate, gate_scale, w_up, up_scale))
     if m > 0:
         px, ldx, wide, keep_x = _pieces(x, px, ldx)
         ws, ws_bytes, keep = _product_workspace(m, n, wide, 1, 0, dev)
@@ -1610,7 +1635,7 @@ def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
     fp32 for gated_linear_bwd, else None."""
     px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up)
     act = _activation(activation)
-    out, po, ldo = _product_output(out, "gated_linear_fwd: out", (m, h), x.dtype, dev)
+    out, po, ldo = _product_output(out, "gated_linear_fwd: out", (m, h), x.dtype, dev, (x, w_gate, w_up))
     saved = torch.empty((2, m, h), dtype=torch.float32, device=dev) if save else None
     if m == 0:
         return out, saved

@@ -337,3 +337,48 @@ def test_not_a_number_stays_in_its_row(dev):
             x[m - 1, 71] = float("nan")
             out, _ = ops.gated_linear_fwd(x, w, w)
             assert bool(torch.isnan(out[m - 1]).all()) and bool(torch.isfinite(out[:m - 1]).all())
+
+
+def test_refusals(dev):
+    """Wrong types, shapes, strides and outputs, before anything is launched."""
+    x, w = torch.zeros(4, 32, device=dev), torch.ones(32, device=dev)
+    q, s = torch.zeros(4, 32, dtype=torch.int8, device=dev), torch.ones(4, device=dev)
+    wide = torch.zeros(4, 64, device=dev)
+    half, saved = x.bfloat16(), torch.zeros(2, 4, 4, device=dev)
+    for call in (lambda: ops.rms_norm_fwd(x.double(), w), lambda: ops.rms_norm_fwd(x, w[:-1]), lambda: ops.rms_norm_fwd(x, w.bfloat16()),
+                 lambda: ops.rms_norm_fwd(x, None), lambda: ops.rms_norm_fwd(x.t(), w[:4]), lambda: ops.rms_norm_fwd(x, w, residual=half),
+                 lambda: ops.rms_norm_fwd(x, w, residual=wide), lambda: ops.rms_norm_fwd(x, w, sum_out=wide[:, :32]),
+                 lambda: ops.rms_norm_fwd(x, w, out=x[:1].expand(4, 32)), lambda: ops.rms_norm_fwd(x, w, out=half),
+                 lambda: ops.rms_norm_fwd(x[:, :0], w[:0]), lambda: ops.rms_norm_fwd(x[0], w), lambda: ops.rms_norm_fwd(x, w.cpu()),
+                 lambda: ops.rms_norm_bwd(half, x, w), lambda: ops.rms_norm_bwd(x, x, w, dsum=wide), lambda: ops.rms_norm_bwd(x, x, w, need_dx=False, need_dw=False),
+                 lambda: ops.rms_norm_int8(x, None), lambda: ops.quantize_rows(q), lambda: ops.dequantize_rows(q, s[:3]), lambda: ops.dequantize_rows(q, s, torch.float64),
+                 lambda: ops.int8_linear(x, s, q, s), lambda: ops.int8_linear(q, s[:2], q, s), lambda: ops.int8_linear(q, s, q[:, :16], s),
+                 lambda: ops.int8_linear(q, s, q, s, bias=w), lambda: ops.int8_linear(q, s, q, s, out_dtype=torch.int8),
+                 lambda: ops.int8_linear(q, s, q, s.half()), lambda: ops.int8_linear(q, s, q, s, out=wide), lambda: ops.int8_linear(q, s, q[:0], s[:0]),
+                 lambda: ops.int8_gated_linear(q, s, q, s, q[:2], s[:2]), lambda: ops.int8_gated_linear(q, s, q, s, q, s, activation="tanh"),
+                 lambda: ops.gated_linear_fwd(x, half, x), lambda: ops.gated_linear_fwd(x, x, x[:2]), lambda: ops.gated_linear_fwd(x, wide, wide),
+                 lambda: ops.gated_linear_fwd(x, x, x, activation="none"), lambda: ops.gated_linear_fwd(x, x, x, out=x[:, :4]),
+                 lambda: ops.gated_linear_fwd(wide[:, 32:], x, x, out=wide[:, 30:34]),
+                 lambda: ops.gated_linear_bwd(x, x, x, x, saved), lambda: ops.gated_linear_bwd(wide[:, :4], x, x, x, saved[:, :, :3]),
+                 lambda: ops.gated_linear_bwd(wide[:, :4], x, x, x, None), lambda: ops.gated_linear_bwd(wide[:, :4], x, x, x, saved, need_dx=False, need_dw=False)):
+        with pytest.raises(RuntimeError):
+            call()
+    ops.gated_linear_fwd(wide[:, 32:], x, x, out=wide[:, 28:32])       # columns of one buffer that lie apart
+
+
+def test_empty_inputs(dev):
+    for dtype in DTYPES:
+        x, w = torch.zeros(0, 24, dtype=dtype, device=dev), torch.ones(24, dtype=dtype, device=dev)
+        wg = torch.ones(5, 24, dtype=dtype, device=dev)
+        y, s = ops.rms_norm_fwd(x, w, residual=x)
+        assert y.shape == s.shape == (0, 24)
+        dx, dw = ops.rms_norm_bwd(y, s, w)
+        assert dx.shape == (0, 24) and not dw.any()
+        q, scale, _ = ops.rms_norm_int8(x, w)
+        assert q.shape == (0, 24) and scale.shape == (0,) and ops.dequantize_rows(q, scale).shape == (0, 24)
+        h, saved = ops.gated_linear_fwd(x, wg, wg, save=True)
+        assert h.shape == (0, 5)
+        dx, dwg, dwu = ops.gated_linear_bwd(h, x, wg, wg, saved)
+        assert dx.shape == (0, 24) and not dwg.any() and not dwu.any()
+        wq, ws = ops.quantize_rows(wg)
+        assert ops.int8_linear(q, scale, wq, ws).shape == (0, 5) and ops.int8_gated_linear(q, scale, wq, ws, wq, ws).shape == (0, 5)
