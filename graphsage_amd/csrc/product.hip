@@ -564,67 +564,76 @@ __global__ void __launch_bounds__(256) join_kernel(Product p, int tiles_m, int t
 
 // ------------------------------------------------------------------------------- few rows
 // 16 * MT rows of A (grid y: more of them) against the whole of B: B goes straight into the registers that
-// the MFMAs take, so the kernel is as fast as B's bytes arrive.  A block owns 16 columns (gated: 16 of
+// the MFMAs take, so the kernel is as fast as B's bytes arrive.  A block owns 16 * NT columns (gated: of
 // each B); its waves take k in runs of 256 bytes in turn and add their sums in LDS, in wave order.
 constexpr int kFewWaves = 8;
 
-template <typename T, int MT, bool kGated>
+template <typename T, int MT, bool kGated, int NT>
 __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_kernel(Product p) {
   using Acc = typename Mma<T>::Acc;
-  constexpr int NB = kGated ? 2 : 1;
-  __shared__ Acc lds[kFewWaves][MT * NB][kWave];
+  constexpr int NB = kGated ? 2 : 1, NC = NB * NT, U = 4;
+  __shared__ Acc lds[kFewWaves][MT * NC][kWave];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int l15 = lane & 15, q = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
-  const int64_t col = n0 + l15 < p.n ? n0 + l15 : p.n - 1;
-  const char* b[NB];
-  b[0] = p.b0 + col * p.ldb0 + q * 16;
-  if constexpr (kGated) b[1] = p.b1 + col * p.ldb1 + q * 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * NT), m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
+  const char* b[NC];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t col = n0 + t * 16 + l15 < p.n ? n0 + t * 16 + l15 : p.n - 1;
+    b[t * NB] = p.b0 + col * p.ldb0 + q * 16;
+    if constexpr (kGated) b[t * NB + 1] = p.b1 + col * p.ldb1 + q * 16;
+  }
   const char* a[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int64_t row = m0 + i * 16 + l15 < p.m ? m0 + i * 16 + l15 : p.m - 1;
     a[i] = p.a + row * p.lda + q * 16;
   }
-  Acc acc[MT][NB];
+  Acc acc[MT][NC];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[i][j] = Acc{};
+    for (int j = 0; j < NC; ++j) acc[i][j] = Acc{};
   const i32x4 none = {0, 0, 0, 0};
-  // four pieces of 64 bytes a turn: 256 contiguous bytes of a row, all loads before the first product
-  for (int64_t k = wave * 256; k < p.kbytes; k += kFewWaves * 256) {
-    i32x4 bv[4][NB], av[4][MT];
+  // U pieces of 64 bytes a turn: contiguous bytes of a row, all loads before the first product
+  for (int64_t k = wave * (U * 64); k < p.kbytes; k += kFewWaves * U * 64) {
+    i32x4 bv[U][NC], av[U][MT];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       const bool in = k + u * 64 + q * 16 < p.kbytes;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) bv[u][j] = in ? *reinterpret_cast<const i32x4*>(b[j] + k + u * 64) : none;
+      for (int j = 0; j < NC; ++j) bv[u][j] = in ? *reinterpret_cast<const i32x4*>(b[j] + k + u * 64) : none;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = k + u * 64 + q * 16 < p.kbytes;
 #pragma unroll
       for (int i = 0; i < MT; ++i) av[u][i] = in ? *reinterpret_cast<const i32x4*>(a[i] + k + u * 64) : none;
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = Mma<T>::mma(bv[u][j], av[u][i], acc[i][j]);
+        for (int j = 0; j < NC; ++j) acc[i][j] = Mma<T>::mma(bv[u][j], av[u][i], acc[i][j]);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) lds[wave][i * NB + j][lane] = acc[i][j];
+    for (int j = 0; j < NC; ++j) lds[wave][i * NC + j][lane] = acc[i][j];
   __syncthreads();
   using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
-  for (int i = wave; i < MT; i += kFewWaves) {
+  for (int o = wave; o < MT * NT; o += kFewWaves) {
+    const int i = o / NT, t = o % NT;
     Acc sum[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      sum[j] = lds[0][i * NB + j][lane];
+      const int at = i * NC + t * NB + j;
+      sum[j] = lds[0][at][lane];
 #pragma unroll
-      for (int w = 1; w < kFewWaves; ++w) sum[j] += lds[w][i * NB + j][lane];
+      for (int w = 1; w < kFewWaves; ++w) sum[j] += lds[w][at][lane];
     }
-    const int64_t row = m0 + i * 16 + l15, at = n0 + q * 4;
+    const int64_t row = m0 + i * 16 + l15, at = n0 + t * 16 + q * 4;
     E c[4], d[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -714,9 +723,14 @@ int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, con
                what, (long)kMaxRowBytes);
   if (plan.tile == 0) {
     const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), static_cast<unsigned>(cdiv(p.m, 64)));   // m <= 512
-    if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
-    else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
-    else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated>), grid, dim3(kFewWaves * kWave), 0, stream, p);
+    // 32 columns a block where 17 to 32 rows would otherwise be read for every 16 (8-bit pair of 8192 x 2048 against 24
+    // rows 10.9 -> 10.3 us, bf16 pair of 5632 x 2048 against 20 rows 19.1 -> 16.9; more or fewer pieces a turn and 32
+    // columns for other row counts measured the same or slower)
+    const dim3 half(static_cast<unsigned>(cdiv(p.n, 32)), 1), threads(kFewWaves * kWave);
+    if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated, 1>), grid, threads, 0, stream, p);
+    else if (p.m <= 32 && p.n >= 4096) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 2>), half, threads, 0, stream, p);
+    else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 1>), grid, threads, 0, stream, p);
+    else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated, 1>), grid, threads, 0, stream, p);
   } else {
     SAGE_REQUIRE(plan.workspace <= ws_bytes && (plan.workspace == 0 || rows16(ws, 0)), SAGE_EWORKSPACE,
                  "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, plan.workspace);

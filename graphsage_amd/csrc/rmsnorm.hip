@@ -329,8 +329,18 @@ struct NormBwdArgs {
 
 // A block goes over rows r, r + step, ...; dw's column sums stay in registers until its last row and are
 // written once, as the block's partial row (dweight_sum_kernel adds those in a fixed order).  A row's three
-// inputs are all loaded before the first is used, and kept in their own type.
-template <typename T, int kTPR, int kNV>
+// inputs are all loaded before the first is used, and they and the weight are kept in their own type and
+// widened where they are used: with the widened values kept as well a wave of 4 vectors a lane needs 241
+// registers, and half as many waves fit a CU.
+template <typename T>
+__device__ inline void narrow(Pack<T>& p) {
+  uint32_t w[4];
+  __builtin_memcpy(w, &p, 16);
+  asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));   // what was widened from it is not kept
+  __builtin_memcpy(&p, w, 16);
+}
+
+template <typename T, typename W, int kTPR, int kNV>
 __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_bwd_kernel(NormBwdArgs a) {
   constexpr int n = VecOf<T>::n;
   constexpr int kRows = kTPR > kRowBlock ? 1 : kRowBlock / kTPR;
@@ -339,14 +349,18 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
   __shared__ float lds_b[2][16];
   const int t = threadIdx.x % kTPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
-  float w[kNV][n];
+  constexpr int nw = VecOf<W>::n, kW = n / nw;         // an fp32 weight of 16-bit rows is two vectors
+  Pack<W> w[kNV][kW];
   float acc[kNV][n];
+  const W* wp = std::is_same<T, W>::value ? static_cast<const W*>(a.w) : reinterpret_cast<const W*>(a.w32);
 #pragma unroll
   for (int j = 0; j < kNV; ++j) {
-    load_weight<T>(static_cast<const T*>(a.w), a.w32, static_cast<int64_t>(j * kTPR + t) * n, a.dim, w[j]);
+#pragma unroll
+    for (int h = 0; h < kW; ++h) w[j][h] = load_pack<W>(wp, static_cast<int64_t>(j * kTPR + t) * n + h * nw, a.dim);
 #pragma unroll
     for (int i = 0; i < n; ++i) acc[j][i] = 0.f;
   }
+  auto weight = [&](int j, int i) { return to_f(w[j][i / nw].v[i % nw]); };
   int flip = 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; row < a.rows; row += step) {
     const T* sp = static_cast<const T*>(a.s) + row * a.ld_s;
@@ -370,8 +384,15 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
       for (int i = 0; i < n; ++i) {
         const float v = to_f(s[j].v[i]);
         ss += v * v;
-        dot += to_f(g[j].v[i]) * w[j][i] * v;
+        dot += to_f(g[j].v[i]) * weight(j, i) * v;
       }
+    }
+#pragma unroll
+    for (int j = 0; j < kNV; ++j) {
+      narrow(s[j]);
+      narrow(g[j]);
+#pragma unroll
+      for (int h = 0; h < kW; ++h) narrow(w[j][h]);
     }
     ss = wave_add(ss);
     dot = wave_add(dot);
@@ -402,7 +423,7 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
       for (int i = 0; i < n; ++i) {
         const float xh = to_f(s[j].v[i]) * rstd, gy = to_f(g[j].v[i]);
         acc[j][i] += gy * xh;
-        o[i] = rstd * (gy * w[j][i] - xh * c) + (dsp != nullptr ? to_f(d[j].v[i]) : 0.f);
+        o[i] = rstd * (gy * weight(j, i) - xh * c) + (dsp != nullptr ? to_f(d[j].v[i]) : 0.f);
       }
       if (a.dx != nullptr) store_vec<T>(dxp, static_cast<int64_t>(j * kTPR + t) * n, a.dim, o);
     }
@@ -425,8 +446,7 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
       __syncthreads();
     }
     for (int e = threadIdx.x; e < kTPR * kNV * n; e += kRowBlock) {
-      const int64_t col = static_cast<int64_t>((e / n / kTPR) * kTPR + e / n % kTPR) * n + e % n;
-      if (col < a.dim) part[col] = lds[((e / n / kTPR) * n + e % n) * kTPR + e / n % kTPR];
+      if (e < a.dim) part[e] = lds[(e / n / kTPR * n + e % n) * kTPR + e / n % kTPR];
     }
   } else {
 #pragma unroll
@@ -597,8 +617,13 @@ int norm_by_type(const NormArgs& a, int dtype, hipStream_t stream, const char* w
 }
 
 // Blocks of the backward pass: four for each of the 256 CUs at most, and one partial row of dw for each.
-inline int64_t bwd_blocks(int64_t rows, int64_t dim, int dtype) {
+// Rows of over 2048 vectors go through the long kernel (their sums would not fit the registers).
+inline RowShape bwd_shape(int64_t rows, int64_t dim, int dtype) {
   const RowShape s = row_shape(dim, dtype == SAGE_F32 ? 4 : 8, rows);
+  return s.threads * s.vectors > 2048 ? RowShape{0, 0} : s;
+}
+inline int64_t bwd_blocks(int64_t rows, int64_t dim, int dtype) {
+  const RowShape s = bwd_shape(rows, dim, dtype);
   const int64_t blocks = cdiv(rows, s.threads == 64 ? kRowBlock / kWave : 1);
   return blocks < 1024 ? blocks : 1024;
 }
@@ -606,10 +631,16 @@ inline int64_t bwd_blocks(int64_t rows, int64_t dim, int dtype) {
 template <typename T>
 void launch_norm_bwd(const NormBwdArgs& a, int dtype, hipStream_t stream) {
   const unsigned blocks = static_cast<unsigned>(bwd_blocks(a.rows, a.dim, dtype));
-  const bool held = with_row_shape(row_shape(a.dim, VecOf<T>::n, a.rows), [&](auto tpr, auto nv) {
+  const RowShape shape = bwd_shape(a.rows, a.dim, dtype);
+  const bool held = with_row_shape(shape, [&](auto tpr, auto nv) {
     constexpr int kTPR = decltype(tpr)::value, kNV = decltype(nv)::value;
     constexpr int threads = kTPR > kRowBlock ? kTPR : kRowBlock;
-    hipLaunchKernelGGL((rms_norm_bwd_kernel<T, kTPR, kNV>), dim3(blocks), dim3(threads), 0, stream, a);
+    if constexpr (kTPR * kNV <= 2048) {
+      if (a.w32 == nullptr)
+        hipLaunchKernelGGL((rms_norm_bwd_kernel<T, T, kTPR, kNV>), dim3(blocks), dim3(threads), 0, stream, a);
+      else if constexpr (!std::is_same<T, float>::value)
+        hipLaunchKernelGGL((rms_norm_bwd_kernel<T, float, kTPR, kNV>), dim3(blocks), dim3(threads), 0, stream, a);
+    }
   });
   if (!held) hipLaunchKernelGGL((rms_norm_bwd_long_kernel<T>), dim3(blocks), dim3(1024), 0, stream, a);
 }
