@@ -40,13 +40,20 @@ __device__ inline float to_f(T v) { return static_cast<float>(v); }
 template <typename T>
 __device__ inline T from_f(float v) { return static_cast<T>(v); }   // round to nearest even
 
-// a vector of a row, zeros behind its end
+// A vector of a row, zeros behind its end.  The last, partial one is the row's last n elements moved down (one
+// load; element by element where the row is shorter than a vector).
 template <typename T>
 __device__ inline Pack<T> load_pack(const T* p, int64_t at, int64_t dim) {
   constexpr int n = VecOf<T>::n;
   Pack<T> k;
   if (at + n <= dim) {
     k = *reinterpret_cast<const Pack<T>*>(p + at);
+  } else if (at < dim && dim >= n) {
+    k = *reinterpret_cast<const Pack<T>*>(p + (dim - n));
+    unsigned __int128 bits;
+    __builtin_memcpy(&bits, &k, 16);
+    bits >>= (at + n - dim) * (8 * sizeof(T));
+    __builtin_memcpy(&k, &bits, 16);
   } else {
 #pragma unroll
     for (int i = 0; i < n; ++i) k.v[i] = at + i < dim ? p[at + i] : static_cast<T>(0.f);
@@ -115,14 +122,14 @@ __device__ inline uint32_t wave_umax(uint32_t v) {
   return v;
 }
 
-// Sum and maximum over the kTPR threads of a row, given to all of them.  The order of the additions
+// Sum and maximum over the threads of a row (a wave, or the block), given to all of them.  The order of the additions
 // is fixed (lanes, then waves in order), so a row's result does not depend on the launch.
-template <int kTPR>
+template <bool kWaveRow>
 __device__ inline void row_reduce(float& sum, uint32_t& top, float* lds_sum, uint32_t* lds_top) {
   sum = wave_add(sum);
   top = wave_umax(top);
-  if constexpr (kTPR > kWave) {
-    constexpr int kWaves = kTPR / kWave;
+  if constexpr (!kWaveRow) {
+    const int waves = blockDim.x / kWave;
     const int wave = threadIdx.x / kWave;
     if ((threadIdx.x & (kWave - 1)) == 0) {
       lds_sum[wave] = sum;
@@ -131,8 +138,7 @@ __device__ inline void row_reduce(float& sum, uint32_t& top, float* lds_sum, uin
     __syncthreads();
     sum = 0.f;
     top = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < waves; ++i) {
       sum += lds_sum[i];
       top = max(top, lds_top[i]);
     }
@@ -184,16 +190,15 @@ struct NormArgs {
   int normalise;        // 0: rstd = 1 (quantisation alone)
 };
 
-// One row to kTPR threads; kNV vectors of 16 bytes a thread hold it.
-template <typename T, bool kInt8, int kTPR, int kNV>
-__global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_kernel(NormArgs a) {
+// A row to a wave (four rows a block) or to the block; kNV vectors of 16 bytes a thread hold it.
+template <typename T, bool kInt8, bool kWaveRow, int kNV>
+__global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024) rms_norm_kernel(NormArgs a) {
   constexpr int n = VecOf<T>::n;
-  constexpr int kRows = kTPR > kRowBlock ? 1 : kRowBlock / kTPR;
-  static_assert(kTPR == kWave || kRows == 1, "a block of several waves holds one row");
   __shared__ float lds_sum[16];
   __shared__ uint32_t lds_top[16];
-  const int t = threadIdx.x % kTPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR;
+  const int threads = kWaveRow ? kWave : blockDim.x;       // of a row
+  const int t = kWaveRow ? threadIdx.x % kWave : threadIdx.x;
+  const int64_t row = kWaveRow ? static_cast<int64_t>(blockIdx.x) * (kRowBlock / kWave) + threadIdx.x / kWave : blockIdx.x;
   if (row >= a.rows) return;     // whole waves, and never part of a block that meets at a barrier
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ld_r : nullptr;
@@ -204,14 +209,14 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
   {
     Pack<T> px[kNV], pr[kNV];     // all of a row's loads before the first use
 #pragma unroll
-    for (int j = 0; j < kNV; ++j) px[j] = load_pack<T>(x, static_cast<int64_t>(j * kTPR + t) * n, a.dim);
+    for (int j = 0; j < kNV; ++j) px[j] = load_pack<T>(x, static_cast<int64_t>(j * threads + t) * n, a.dim);
     if (r != nullptr) {
 #pragma unroll
-      for (int j = 0; j < kNV; ++j) pr[j] = load_pack<T>(r, static_cast<int64_t>(j * kTPR + t) * n, a.dim);
+      for (int j = 0; j < kNV; ++j) pr[j] = load_pack<T>(r, static_cast<int64_t>(j * threads + t) * n, a.dim);
     }
 #pragma unroll
     for (int j = 0; j < kNV; ++j)
-      load_weight<T>(static_cast<const T*>(a.w), a.w32, static_cast<int64_t>(j * kTPR + t) * n, a.dim, w[j]);
+      load_weight<T>(static_cast<const T*>(a.w), a.w32, static_cast<int64_t>(j * threads + t) * n, a.dim, w[j]);
 #pragma unroll
     for (int j = 0; j < kNV; ++j)
 #pragma unroll
@@ -228,9 +233,9 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
   if (a.sum != nullptr) {
     T* out = static_cast<T*>(a.sum) + row * a.ld_sum;
 #pragma unroll
-    for (int j = 0; j < kNV; ++j) store_vec<T>(out, static_cast<int64_t>(j * kTPR + t) * n, a.dim, s[j]);
+    for (int j = 0; j < kNV; ++j) store_vec<T>(out, static_cast<int64_t>(j * threads + t) * n, a.dim, s[j]);
   }
-  row_reduce<kTPR>(ss, top, lds_sum, lds_top);
+  row_reduce<kWaveRow>(ss, top, lds_sum, lds_top);
   const float rstd = a.normalise ? 1.f / sqrtf(ss / static_cast<float>(a.dim) + a.eps) : 1.f;
   if constexpr (kInt8) {
     const RowScale k = row_scale(top, rstd);
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
     int8_t* q = a.q + row * a.ld_q;
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
-      const int64_t at = static_cast<int64_t>(j * kTPR + t) * n;
+      const int64_t at = static_cast<int64_t>(j * threads + t) * n;
       Bytes<n> o;
 #pragma unroll
       for (int i = 0; i < n; ++i) o.v[i] = to_q(s[j][i] * w[j][i], k);
@@ -257,7 +262,7 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
       float o[n];
 #pragma unroll
       for (int i = 0; i < n; ++i) o[i] = s[j][i] * rstd * w[j][i];
-      store_vec<T>(y, static_cast<int64_t>(j * kTPR + t) * n, a.dim, o);
+      store_vec<T>(y, static_cast<int64_t>(j * threads + t) * n, a.dim, o);
     }
   }
 }
@@ -291,7 +296,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(NormArgs a) {
       if constexpr (kInt8) top = max(top, magnitude(s[i] * w[i]));
     }
   }
-  row_reduce<1024>(ss, top, lds_sum, lds_top);
+  row_reduce<false>(ss, top, lds_sum, lds_top);
   const float rstd = a.normalise ? 1.f / sqrtf(ss / static_cast<float>(a.dim) + a.eps) : 1.f;
   RowScale k{};
   if constexpr (kInt8) {
@@ -328,9 +333,9 @@ struct NormBwdArgs {
 };
 
 // A block goes over rows r, r + step, ...; dw's column sums stay in registers until its last row and are
-// written once, as the block's partial row (dweight_sum_kernel adds those in a fixed order).  A row's three
-// inputs are all loaded before the first is used, and they and the weight are kept in their own type and
-// widened where they are used: with the widened values kept as well a wave of 4 vectors a lane needs 241
+// written once, as the block's partial row (dweight_sum_kernel adds those in a fixed order).  The next
+// row's three inputs are under way while a row is computed, and they and the weight are kept in their own type
+// and widened where they are used: with the widened values kept as well a wave of 4 vectors a lane needs 241
 // registers, and half as many waves fit a CU.
 template <typename T>
 __device__ inline void narrow(Pack<T>& p) {
@@ -340,14 +345,14 @@ __device__ inline void narrow(Pack<T>& p) {
   __builtin_memcpy(&p, w, 16);
 }
 
-template <typename T, typename W, int kTPR, int kNV>
-__global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_bwd_kernel(NormBwdArgs a) {
+template <typename T, typename W, bool kWaveRow, int kNV>
+__global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024, 4) rms_norm_bwd_kernel(NormBwdArgs a) {
   constexpr int n = VecOf<T>::n;
-  constexpr int kRows = kTPR > kRowBlock ? 1 : kRowBlock / kTPR;
-  constexpr int kWaves = kTPR / kWave;
+  constexpr int kRows = kWaveRow ? kRowBlock / kWave : 1;
+  const int threads = kWaveRow ? kWave : blockDim.x, waves = blockDim.x / kWave;
   __shared__ float lds_a[2][16];
   __shared__ float lds_b[2][16];
-  const int t = threadIdx.x % kTPR;
+  const int t = kWaveRow ? threadIdx.x % kWave : threadIdx.x;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   constexpr int nw = VecOf<W>::n, kW = n / nw;         // an fp32 weight of 16-bit rows is two vectors
   Pack<W> w[kNV][kW];
@@ -356,27 +361,40 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
 #pragma unroll
   for (int j = 0; j < kNV; ++j) {
 #pragma unroll
-    for (int h = 0; h < kW; ++h) w[j][h] = load_pack<W>(wp, static_cast<int64_t>(j * kTPR + t) * n + h * nw, a.dim);
+    for (int h = 0; h < kW; ++h) w[j][h] = load_pack<W>(wp, static_cast<int64_t>(j * threads + t) * n + h * nw, a.dim);
 #pragma unroll
     for (int i = 0; i < n; ++i) acc[j][i] = 0.f;
   }
   auto weight = [&](int j, int i) { return to_f(w[j][i / nw].v[i % nw]); };
   int flip = 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; row < a.rows; row += step) {
+  Pack<T> s[kNV], g[kNV], d[kNV], s_next[kNV], g_next[kNV], d_next[kNV];
+  auto load_row = [&](int64_t row) {
     const T* sp = static_cast<const T*>(a.s) + row * a.ld_s;
     const T* yp = static_cast<const T*>(a.dy) + row * a.ld_dy;
-    const T* dsp = a.ds ? static_cast<const T*>(a.ds) + row * a.ld_ds : nullptr;
-    Pack<T> s[kNV], g[kNV], d[kNV];
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
-      const int64_t at = static_cast<int64_t>(j * kTPR + t) * n;
-      s[j] = load_pack<T>(sp, at, a.dim);
-      g[j] = load_pack<T>(yp, at, a.dim);
+      const int64_t at = static_cast<int64_t>(j * threads + t) * n;
+      s_next[j] = load_pack<T>(sp, at, a.dim);
+      g_next[j] = load_pack<T>(yp, at, a.dim);
     }
-    if (dsp != nullptr) {
+    if (a.ds != nullptr) {
+      const T* dsp = static_cast<const T*>(a.ds) + row * a.ld_ds;
 #pragma unroll
-      for (int j = 0; j < kNV; ++j) d[j] = load_pack<T>(dsp, static_cast<int64_t>(j * kTPR + t) * n, a.dim);
+      for (int j = 0; j < kNV; ++j) d_next[j] = load_pack<T>(dsp, static_cast<int64_t>(j * threads + t) * n, a.dim);
     }
+  };
+  int64_t row = kWaveRow ? static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kWave : blockIdx.x;
+  constexpr bool kAhead = kNV == 1;     // two rows of two vectors a thread would not fit the registers
+  if (kAhead && row < a.rows) load_row(row);
+  for (; row < a.rows; row += step) {
+    if (!kAhead) load_row(row);
+#pragma unroll
+    for (int j = 0; j < kNV; ++j) {
+      s[j] = s_next[j];
+      g[j] = g_next[j];
+      d[j] = d_next[j];
+    }
+    if (kAhead && row + step < a.rows) load_row(row + step);      // under way while this row is computed
     float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
@@ -396,7 +414,7 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
     }
     ss = wave_add(ss);
     dot = wave_add(dot);
-    if constexpr (kTPR > kWave) {
+    if constexpr (!kWaveRow) {
       // two sets of slots in turn: a wave that is a row ahead writes the other one
       const int wave = threadIdx.x / kWave;
       if ((threadIdx.x & (kWave - 1)) == 0) {
@@ -406,8 +424,7 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
       __syncthreads();
       ss = 0.f;
       dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
+      for (int i = 0; i < waves; ++i) {
         ss += lds_a[flip][i];
         dot += lds_b[flip][i];
       }
@@ -423,35 +440,35 @@ __global__ void __launch_bounds__(kTPR > kRowBlock ? kTPR : kRowBlock) rms_norm_
       for (int i = 0; i < n; ++i) {
         const float xh = to_f(s[j].v[i]) * rstd, gy = to_f(g[j].v[i]);
         acc[j][i] += gy * xh;
-        o[i] = rstd * (gy * weight(j, i) - xh * c) + (dsp != nullptr ? to_f(d[j].v[i]) : 0.f);
+        o[i] = rstd * (gy * weight(j, i) - xh * c) + (a.ds != nullptr ? to_f(d[j].v[i]) : 0.f);
       }
-      if (a.dx != nullptr) store_vec<T>(dxp, static_cast<int64_t>(j * kTPR + t) * n, a.dim, o);
+      if (a.dx != nullptr) store_vec<T>(dxp, static_cast<int64_t>(j * threads + t) * n, a.dim, o);
     }
   }
   if (a.part == nullptr) return;
   float* part = a.part + static_cast<int64_t>(blockIdx.x) * a.dim;
   if constexpr (kRows > 1) {
     // the block's rows' sums, added in wave order
-    __shared__ float lds[kTPR * kNV * n];
+    __shared__ float lds[kWave * kNV * n];
     for (int wave = 0; wave < kRows; ++wave) {
-      if (static_cast<int>(threadIdx.x) / kTPR == wave) {
+      if (static_cast<int>(threadIdx.x) / kWave == wave) {
 #pragma unroll
         for (int j = 0; j < kNV; ++j)
 #pragma unroll
           for (int i = 0; i < n; ++i) {
-            float* at = lds + (j * n + i) * kTPR + t;
+            float* at = lds + (j * n + i) * kWave + t;
             *at = (wave == 0 ? 0.f : *at) + acc[j][i];
           }
       }
       __syncthreads();
     }
-    for (int e = threadIdx.x; e < kTPR * kNV * n; e += kRowBlock) {
-      if (e < a.dim) part[e] = lds[(e / n / kTPR * n + e % n) * kTPR + e / n % kTPR];
+    for (int e = threadIdx.x; e < kWave * kNV * n; e += kRowBlock) {
+      if (e < a.dim) part[e] = lds[(e / n / kWave * n + e % n) * kWave + e / n % kWave];
     }
   } else {
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
-      const int64_t at = static_cast<int64_t>(j * kTPR + t) * n;
+      const int64_t at = static_cast<int64_t>(j * threads + t) * n;
 #pragma unroll
       for (int i = 0; i < n; ++i)
         if (at + i < a.dim) part[at + i] = acc[j][i];
@@ -568,40 +585,44 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, int64_
   }
 }
 
-// How a row of v vectors is split: threads and vectors a thread; {0, 0}: longer than the registers hold.
-// With many rows a wave takes a row of up to 256 vectors alone: no barrier, and 4 KB of each input under way
-// a wave.  With few (fewer than the chip's waves) a row's latency counts, and four waves share it.
+// How a row of v vectors is split: a wave (four rows a block) or a block of `threads` to a row, and vectors a
+// thread; no vectors: longer than the registers hold.
 struct RowShape {
   int threads, vectors;
+  bool wave;
 };
+inline RowShape block_row(int64_t v, int vectors) {
+  return {static_cast<int>(cdiv(v, kWave * vectors)) * kWave, vectors, false};
+}
+// With many rows a wave takes a row of up to 256 vectors alone: no barrier, and 4 KB of each input under way
+// a wave.  With few (fewer than the chip's waves) a row's latency counts: one vector a thread.
 inline RowShape row_shape(int64_t dim, int n, int64_t rows) {
   const int64_t v = cdiv(dim, n);
-  const int64_t alone = rows >= 2048 ? 256 : 64;
-  if (v <= alone) return {64, static_cast<int>(cdiv(v, 64))};
-  if (v <= 1024) return {256, static_cast<int>(cdiv(v, 256))};
-  if (v <= 2048) return {1024, 2};
-  if (v <= 4096) return {1024, 4};
-  return {0, 0};
+  if (v <= (rows >= 2048 ? 256 : 64)) return {kWave, static_cast<int>(cdiv(v, 64)), true};
+  if (v <= 1024 && rows < 2048) return block_row(v, 1);
+  if (v <= 2048) return block_row(v, 2);
+  if (v <= 4096) return block_row(v, 4);
+  return {1024, 0, false};
 }
 template <typename F>
-inline bool with_row_shape(RowShape s, F&& f) {
+inline bool with_row_shape(const RowShape& s, F&& f) {
   using std::integral_constant;
-#define SAGE_SHAPE(TPR, NV) \
-  if (s.threads == TPR && s.vectors == NV) { f(integral_constant<int, TPR>{}, integral_constant<int, NV>{}); return true; }
-  SAGE_SHAPE(64, 1) SAGE_SHAPE(64, 2) SAGE_SHAPE(64, 3) SAGE_SHAPE(64, 4)
-  SAGE_SHAPE(256, 1) SAGE_SHAPE(256, 2) SAGE_SHAPE(256, 3) SAGE_SHAPE(256, 4)
-  SAGE_SHAPE(1024, 2) SAGE_SHAPE(1024, 4)
+#define SAGE_SHAPE(WAVE, NV) \
+  if (s.wave == WAVE && s.vectors == NV) { f(integral_constant<bool, WAVE>{}, integral_constant<int, NV>{}); return true; }
+  SAGE_SHAPE(true, 1) SAGE_SHAPE(true, 2) SAGE_SHAPE(true, 3) SAGE_SHAPE(true, 4)
+  SAGE_SHAPE(false, 1) SAGE_SHAPE(false, 2) SAGE_SHAPE(false, 4)
 #undef SAGE_SHAPE
   return false;
 }
 
 template <typename T, bool kInt8>
 void launch_norm(const NormArgs& a, hipStream_t stream) {
-  const bool held = with_row_shape(row_shape(kInt8 ? a.q_cols : a.dim, VecOf<T>::n, a.rows), [&](auto tpr, auto nv) {
-    constexpr int kTPR = decltype(tpr)::value, kNV = decltype(nv)::value;
-    constexpr int threads = kTPR > kRowBlock ? kTPR : kRowBlock;
-    const int64_t blocks = cdiv(a.rows, threads / kTPR);
-    hipLaunchKernelGGL((rms_norm_kernel<T, kInt8, kTPR, kNV>), dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, stream, a);
+  const RowShape shape = row_shape(kInt8 ? a.q_cols : a.dim, VecOf<T>::n, a.rows);
+  const bool held = with_row_shape(shape, [&](auto wave, auto nv) {
+    constexpr bool kWaveRow = decltype(wave)::value;
+    const dim3 grid(static_cast<unsigned>(kWaveRow ? cdiv(a.rows, kRowBlock / kWave) : a.rows));
+    hipLaunchKernelGGL((rms_norm_kernel<T, kInt8, kWaveRow, decltype(nv)::value>), grid,
+                       dim3(kWaveRow ? kRowBlock : shape.threads), 0, stream, a);
   });
   if (!held)
     hipLaunchKernelGGL((rms_norm_long_kernel<T, kInt8>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, stream, a);
@@ -616,30 +637,37 @@ int norm_by_type(const NormArgs& a, int dtype, hipStream_t stream, const char* w
   return SAGE_OK;
 }
 
-// Blocks of the backward pass: four for each of the 256 CUs at most, and one partial row of dw for each.
-// Rows of over 2048 vectors go through the long kernel (their sums would not fit the registers).
-inline RowShape bwd_shape(int64_t rows, int64_t dim, int dtype) {
-  const RowShape s = row_shape(dim, dtype == SAGE_F32 ? 4 : 8, rows);
-  return s.threads * s.vectors > 2048 ? RowShape{0, 0} : s;
+// The backward pass: one vector a thread with the next row's under way (16381 x 2047 bf16, all of it: four vectors
+// a lane of a wave 90 us; with the next row under way as well they leave one wave a SIMD, 147; two vectors
+// a thread 102, their registers spill), two where a block is too short; rows of over 2048 vectors go through the
+// long kernel.  As many blocks as run at once (20 waves a CU in 16 bits, 32 in fp32), so that none is left over.
+inline RowShape bwd_shape(int64_t dim, int dtype) {
+  const int64_t v = cdiv(dim, dtype == SAGE_F32 ? 4 : 8);
+  if (v <= 64) return {kWave, 1, true};
+  if (v <= 1024) return block_row(v, 1);
+  if (v <= 2048) return block_row(v, 2);
+  return {1024, 0, false};
 }
 inline int64_t bwd_blocks(int64_t rows, int64_t dim, int dtype) {
-  const RowShape s = bwd_shape(rows, dim, dtype);
-  const int64_t blocks = cdiv(rows, s.threads == 64 ? kRowBlock / kWave : 1);
-  return blocks < 1024 ? blocks : 1024;
+  const RowShape s = bwd_shape(dim, dtype);
+  const int64_t blocks = s.wave ? cdiv(rows, kRowBlock / kWave) : rows;
+  const int64_t most = 256 * ((dtype == SAGE_F32 ? 32 : 20) / (s.wave ? kRowBlock / kWave : s.threads / kWave));
+  return blocks < most ? blocks : most;
 }
 
 template <typename T>
 void launch_norm_bwd(const NormBwdArgs& a, int dtype, hipStream_t stream) {
   const unsigned blocks = static_cast<unsigned>(bwd_blocks(a.rows, a.dim, dtype));
-  const RowShape shape = bwd_shape(a.rows, a.dim, dtype);
-  const bool held = with_row_shape(shape, [&](auto tpr, auto nv) {
-    constexpr int kTPR = decltype(tpr)::value, kNV = decltype(nv)::value;
-    constexpr int threads = kTPR > kRowBlock ? kTPR : kRowBlock;
-    if constexpr (kTPR * kNV <= 2048) {
+  const RowShape shape = bwd_shape(a.dim, dtype);
+  const bool held = with_row_shape(shape, [&](auto wave, auto nv) {
+    constexpr bool kWaveRow = decltype(wave)::value;
+    constexpr int kNV = decltype(nv)::value;
+    const dim3 threads(kWaveRow ? kRowBlock : shape.threads);
+    if constexpr (kNV == 1 || (kNV == 2 && !kWaveRow)) {
       if (a.w32 == nullptr)
-        hipLaunchKernelGGL((rms_norm_bwd_kernel<T, T, kTPR, kNV>), dim3(blocks), dim3(threads), 0, stream, a);
+        hipLaunchKernelGGL((rms_norm_bwd_kernel<T, T, kWaveRow, kNV>), dim3(blocks), threads, 0, stream, a);
       else if constexpr (!std::is_same<T, float>::value)
-        hipLaunchKernelGGL((rms_norm_bwd_kernel<T, float, kTPR, kNV>), dim3(blocks), dim3(threads), 0, stream, a);
+        hipLaunchKernelGGL((rms_norm_bwd_kernel<T, float, kWaveRow, kNV>), dim3(blocks), threads, 0, stream, a);
     }
   });
   if (!held) hipLaunchKernelGGL((rms_norm_bwd_long_kernel<T>), dim3(blocks), dim3(1024), 0, stream, a);
