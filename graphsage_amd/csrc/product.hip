@@ -89,7 +89,8 @@ struct Product {
   const char* b1;       // second B of a gated product
   int64_t lda, ldb0, ldb1;   // row strides in bytes
   int64_t m, n;         // outputs (n: of each B)
-  int64_t kbytes;       // row length in bytes, a multiple of 16
+  int64_t kbytes;       // rows along k: their length in bytes, a multiple of 16
+  int64_t depth;        // rows of k: how many (of each B, where b1 follows b0)
   void* out;
   int64_t ldo;          // in elements
   int out_dtype;
@@ -98,9 +99,11 @@ struct Product {
   const float* sb0;
   const float* sb1;
   const float* bias;
+  int64_t fold, fold_rows;   // two outputs below each other: row fold + r is row fold_rows + r, fold_rows .. fold - 1 none
   float* saved;         // gated, training: pre-activations [2, m, n] in fp32
+  // k in runs of 64 bytes: all of it; before b1's begin; before the first that k does not fill; of a slice
+  int64_t runs, part_runs, whole_runs, slice_runs;
   i32x4* partial;       // k split over blockIdx.y: the slices' sums, as the waves hold them
-  int64_t slice_bytes;  // of a row, a multiple of 128
 };
 
 template <int n, typename T>
@@ -133,6 +136,10 @@ __device__ inline void store_out(const Product& p, int64_t row, int64_t col, con
 template <typename T, int n, typename S>
 __device__ inline void finish(const Product& p, int64_t row, int64_t col, const S (&c)[n]) {
   if (row >= p.m || col >= p.n) return;
+  if (p.fold > p.fold_rows) {
+    if (row >= p.fold) row -= p.fold - p.fold_rows;
+    else if (row >= p.fold_rows) return;
+  }
   float v[n];
   if constexpr (std::is_same<T, int8_t>::value) {
     const float sa = p.sa[row];
@@ -186,27 +193,31 @@ __device__ inline void finish_gated(const Product& p, int64_t row, int64_t col, 
 __device__ const i32x4 kZeroPiece = {0, 0, 0, 0};
 
 // ------------------------------------------------------------------------------- tiles
-// BM x BN outputs a block (gated: BN / 2 of each B), waves WM x WN, K-steps of 128 bytes.  Both
-// tiles go straight from memory to LDS (global_load_lds, 16 bytes a lane, no registers), one step
-// ahead of the MFMAs, in two buffers that are separate arrays so that the compiler's waits for one
-// do not cover the other.
+// kTile x kTile outputs a block (gated: kTile / 2 of each B), 2 x 4 waves at 256 and 2 x 2 at 128, so that a wave
+// has 64 slots of B and 128 or 64 rows of A.
 //
-// LDS rows are 128 bytes; piece c of row r lies at c ^ ((r >> 1) & 7), so that the 16 rows of an MFMA
-// operand fall on all 64 banks.  The order of B's rows in LDS is chosen so that a lane ends with 16
-// (gated: 8) consecutive columns of its row of C: slot 16 j + i of a wave's 64 holds column
-// 16 (i / 4) + 4 j + i % 4.
-template <int BM, int BN, int WM, int WN, bool kGated>
+// An operand's rows lie along k (its tile: kTile rows of 64 bytes of k a run), or they are rows of k whose elements
+// are the outputs' rows or columns (kAT, kBT: 64 / sizeof(T) rows of kTile elements a run), as the weights' gradients
+// and dx want them; both fill kTile * 64 bytes of LDS a run.  Tiles go straight from memory to LDS
+// (global_load_lds, 16 bytes a lane, no registers); LDS holds four runs in a ring, separate arrays so that the
+// compiler's waits for one do not cover the others.
+//
+// LDS order: rows along k: piece c (of 4) of row r lies at c ^ ((r >> 2) & 3), so that the 16 rows of an MFMA operand
+// fall on all banks.  Rows of k, 16 bits: the operand is read with the transposing read (a group of 16 lanes takes
+// 4 rows x 16 elements and each lane leaves with a column's 4), and the 32 bytes c of row r lie at c ^ f,
+// f = r & 3 | (r >> 3 & 1) << 2, so that the 8 rows of half a wave fall on all banks.  fp32: four plain reads, and the
+// 64 bytes c of row r lie at c ^ (r >> 2 & 3).
+//
+// B's slots: where its rows lie along k, slot 16 j + i of a wave's 64 holds column 16 (i / 4) + 4 j + i % 4 (gated: 8,
+// 32 of each B), so that a lane ends with 16 (gated: 8) consecutive columns of its row of C; else column 16 j + i.
+template <int kTile, bool kGated>
 struct TileShape {
-  static constexpr int kThreads = WM * WN * kWave;
-  static constexpr int kRowsM = BM / WM;             // rows of C a wave computes
-  static constexpr int kColsN = BN / WN;             // slots of B
-  static_assert(kColsN == 64, "the column order is written for 64 slots a wave");
-  static constexpr int kMI = kRowsM / 16, kNI = kColsN / 16;
-  static constexpr int kLoadA = BM * 128 / 16 / kThreads, kLoadB = BN * 128 / 16 / kThreads;
-  static constexpr int kColsOut = kGated ? BN / 2 : BN;
+  static constexpr int kThreads = kTile == 256 ? 512 : 256;
+  static constexpr int WM = 2, WN = kTile / 64;
+  static constexpr int kMI = kTile / WM / 16, kNI = 4;
+  static constexpr int kColsOut = kGated ? kTile / 2 : kTile;
 };
 
-// column (within the block's) that B slot s holds, and which B
 template <bool kGated>
 __device__ inline int slot_column(int s, int* which) {
   const int wn = s >> 6, j = (s >> 4) & 3, i = s & 15;
@@ -236,10 +247,10 @@ __device__ inline void tile_place(int tile, int tiles_m, int tiles_n, int* tm, i
   *tn = in / rows;
 }
 
-// C^T layout of the MFMA (B's rows are its first operand): lane l holds row l & 15, and of slot group j
-// columns 4 (l >> 4) + 0..3, which the slot order makes consecutive over j.
-template <typename T, typename S, bool kGated, typename Acc>
-__device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[S::kNI]) {
+// C^T layout of the MFMA (B's slots are its first operand): lane l holds row l & 15, and of slot group j
+// slots 4 (l >> 4) + 0..3.
+template <typename T, bool kGated, bool kBT, typename Acc>
+__device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[4]) {
   using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
   const int l15 = lane & 15, q = lane >> 4;
   if constexpr (kGated) {
@@ -250,6 +261,14 @@ __device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int
       u[e] = acc[2 + (e >> 2)][e & 3];
     }
     finish_gated<T, 8>(p, m0 + row + l15, n0 + wn * 32 + q * 8, g, u);
+  } else if constexpr (kBT) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      E c[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[e] = acc[j][e];
+      finish<T, 4>(p, m0 + row + l15, n0 + wn * 64 + j * 16 + q * 4, c);
+    }
   } else {
     E c[16];
 #pragma unroll
@@ -258,73 +277,138 @@ __device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool kGated>
-__global__ void __launch_bounds__(WM* WN* kWave, 2) tile_kernel(Product p, int tiles_m, int tiles_n) {
-  using S = TileShape<BM, BN, WM, WN, kGated>;
+// Where a lane's two loads of an operand's run come from, as offsets of 32 bits from the tile's first row (strides are
+// below 2^23 bytes), and which of them lie behind the end of k.
+template <typename T, int kTile, bool kTransposed>
+struct Lanes {
+  static constexpr int kThreads = kTile == 256 ? 512 : 256;
+  uint32_t off[2];
+  int at[2];      // rows along k: byte of the run; rows of k: row of the run
+
+  // rows along k: `of(r)` is the operand's row for LDS row r
+  template <typename F>
+  __device__ void along(int wave, int lane, uint32_t ld, F&& of) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      at[j] = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+      off[j] = static_cast<uint32_t>(of(j * (kThreads / 4) + wave * 16 + (lane >> 2))) * ld + at[j];
+    }
+  }
+  // rows of k; `last`: the last piece of 16 bytes that the row has (what is behind it is not stored)
+  __device__ void across(int wave, int lane, uint32_t ld, int last) {
+    constexpr int kPieces = kTile * static_cast<int>(sizeof(T)) / 16;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int index = j * kThreads + wave * kWave + lane, r = index / kPieces, to = index % kPieces;
+      int from;
+      if constexpr (sizeof(T) == 2) from = ((to >> 1) ^ ((r & 3) | ((r >> 3 & 1) << 2))) << 1 | (to & 1);
+      else from = to ^ ((r >> 2 & 3) << 2);
+      at[j] = r;
+      off[j] = static_cast<uint32_t>(r) * ld + (from < last ? from : last) * 16;
+    }
+  }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds16_t;
+
+// An MFMA operand: 16 rows or slots (those of the 16 that begin at 16 * c) by 64 bytes of k
+template <typename T, int kTile, bool kTransposed>
+__device__ inline i32x4 operand(const char* tile, int c, int lane) {
+  const int l15 = lane & 15, q = lane >> 4;
+  if constexpr (!kTransposed) {
+    return *reinterpret_cast<const i32x4*>(tile + (c * 16 + l15) * 64 + (q ^ ((l15 >> 2) & 3)) * 16);
+  } else if constexpr (sizeof(T) == 2) {
+    constexpr int kRow = kTile * 2;
+    const int r = l15 >> 2;            // rows 8 q + r and 8 q + 4 + r
+    const char* at = tile + (8 * q + r) * kRow + ((c ^ (r | ((q & 1) << 2))) * 32 + (l15 & 3) * 8);
+    union {
+      s16x4 half[2];
+      i32x4 whole;
+    } v;
+    v.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16_t)(at));
+    v.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16_t)(at + 4 * kRow));
+    return v.whole;
+  } else {
+    constexpr int kRow = kTile * 4;
+    const char* at = tile + 4 * q * kRow + ((c ^ q) * 64 + l15 * 4);
+    i32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const int*>(at + e * kRow);
+    return v;
+  }
+}
+
+// The ring: run u lies in stage u % 4.  Before run u is read, run u + 3 is fetched into the place of run u - 1, whose
+// readers have met since; at most 8 loads a wave (runs u + 2 and u + 3) are under way when run u + 1 is next.
+//
+// At 256, two waves share a SIMD, one of each half of the block (wave / 4), and the halves run half a phase apart:
+// while one half's waves read their operands from LDS, the other's multiply.  Run u is read in phase 2 u by the first
+// half and in phase 2 u + 1 by the second, and multiplied in the phase after; every phase ends at a barrier of the
+// whole block (the second half passes one more before its first phase, the first half one more behind its last).
+// Run u - 1 was last read in phase 2 u - 1, and its reads had landed (lgkmcnt(0)) before the barrier that ended it, so
+// run u + 3 may be fetched from phase 2 u on; run u + 1 is first read in phase 2 u + 2, and at the end of their reading
+// phases 2 u and 2 u + 1 both halves have waited for their loads of it.
+//
+// At 128, two blocks share a CU instead, and a run is one phase: wait, meet, fetch, read, multiply.
+template <typename T, int kTile, bool kGated, bool kAT, bool kBT>
+__global__ void __launch_bounds__(kTile == 256 ? 512 : 256, 2) tile_kernel(Product p, int tiles_m, int tiles_n) {
+  using S = TileShape<kTile, kGated>;
   using Acc = typename Mma<T>::Acc;
-  __shared__ __attribute__((aligned(1024))) char a_lds0[BM * 128];
-  __shared__ __attribute__((aligned(1024))) char b_lds0[BN * 128];
-  __shared__ __attribute__((aligned(1024))) char a_lds1[BM * 128];
-  __shared__ __attribute__((aligned(1024))) char b_lds1[BN * 128];
+  constexpr int kHalf = kTile * 64, kRows = 64 / static_cast<int>(sizeof(T));
+  static_assert(!(kGated && (kAT || kBT)) && (!kAT || kBT), "the forms that are used");
+  __shared__ __attribute__((aligned(1024))) char stage0[2 * kHalf];
+  __shared__ __attribute__((aligned(1024))) char stage1[2 * kHalf];
+  __shared__ __attribute__((aligned(1024))) char stage2[2 * kHalf];
+  __shared__ __attribute__((aligned(1024))) char stage3[2 * kHalf];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int total = tiles_m * tiles_n;
   const int tile = xcd_tile(blockIdx.x, total);
   int tm, tn;
   tile_place(tile, tiles_m, tiles_n, &tm, &tn);
-  const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * S::kColsOut;
+  const int64_t m0 = static_cast<int64_t>(tm) * kTile, n0 = static_cast<int64_t>(tn) * S::kColsOut;
 
-  // a lane's pieces: row (of 8 a wave and load) and piece of the row, permuted as LDS holds them; as
-  // offsets of 32 bits from the tile's first row (a row's stride is below 2^23 bytes)
-  constexpr int kRowsLoad = S::kThreads / 8;        // rows a load of the whole block fills
-  const int64_t k_first = static_cast<int64_t>(blockIdx.y) * p.slice_bytes;
-  const int64_t kbytes = p.kbytes - k_first < p.slice_bytes ? p.kbytes - k_first : p.slice_bytes;
-  const char* a_base = p.a + m0 * p.lda + k_first;
-  const char* b_base0 = p.b0 + n0 * p.ldb0 + k_first;
-  const char* b_base1 = kGated ? p.b1 + n0 * p.ldb1 + k_first : nullptr;
-  const int rows_left = p.m - m0 < BM ? static_cast<int>(p.m - m0) : BM;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * p.slice_runs;         // runs of this block
+  const int64_t runs = p.runs - first < p.slice_runs ? p.runs - first : p.slice_runs;
+  const bool up = kGated && ((wave >> 1) & 1);          // slots 32 to 63 of each 64 are the second B's
+  const uint32_t lda = static_cast<uint32_t>(p.lda), ldb = static_cast<uint32_t>(up ? p.ldb1 : p.ldb0);
+  const int rows_left = p.m - m0 < kTile ? static_cast<int>(p.m - m0) : kTile;
   const int cols_left = p.n - n0 < S::kColsOut ? static_cast<int>(p.n - n0) : S::kColsOut;
-  const uint32_t lda = static_cast<uint32_t>(p.lda), ldb0 = static_cast<uint32_t>(p.ldb0), ldb1 = static_cast<uint32_t>(p.ldb1);
-  uint32_t oa[S::kLoadA], ob[S::kLoadB];
-  // the load's rows are a multiple of 16, so every load of a lane takes the same piece of its row
-  static_assert(kRowsLoad % 16 == 0, "the piece of a lane");
-  const int lane_row = wave * 8 + (lane >> 3);
-  const int piece_at = ((lane & 7) ^ ((lane_row >> 1) & 7)) * 16;
-#pragma unroll
-  for (int j = 0; j < S::kLoadA; ++j) {
-    const int r = j * kRowsLoad + lane_row;
-    oa[j] = static_cast<uint32_t>(r < rows_left ? r : rows_left - 1) * lda + piece_at;     // rows behind the last are not stored
+  Lanes<T, kTile, kAT> la;
+  Lanes<T, kTile, kBT> lb;
+  // rows and columns behind the last repeat it: their outputs are not stored
+  if constexpr (kAT) la.across(wave, lane, lda, (rows_left * static_cast<int>(sizeof(T)) - 1) / 16);
+  else la.along(wave, lane, lda, [&](int r) { return r < rows_left ? r : rows_left - 1; });
+  if constexpr (kBT) {
+    lb.across(wave, lane, ldb, (cols_left * static_cast<int>(sizeof(T)) - 1) / 16);
+  } else {
+    lb.along(wave, lane, ldb, [&](int r) {
+      int which;
+      const int c = slot_column<kGated>(r, &which);
+      return c < cols_left ? c : cols_left - 1;
+    });
   }
-#pragma unroll
-  for (int j = 0; j < S::kLoadB; ++j) {
-    int which;
-    const int c = slot_column<kGated>(j * kRowsLoad + lane_row, &which);
-    ob[j] = static_cast<uint32_t>(c < cols_left ? c : cols_left - 1) * (which ? ldb1 : ldb0) + piece_at;
-  }
+  const char* a_base = kAT ? p.a + m0 * sizeof(T) : p.a + m0 * p.lda;
+  const char* b_base = kBT ? p.b0 + n0 * sizeof(T) : up ? p.b1 + n0 * p.ldb1 : p.b0 + n0 * p.ldb0;
+  const char* b_base1 = kBT ? p.b1 + n0 * sizeof(T) : nullptr;
   const char* zero = reinterpret_cast<const char*>(&kZeroPiece);
-  auto b_base = [&](int j) {      // a wave's 8 rows of a load are all of one B
-    if constexpr (!kGated) return b_base0;
-    return (((j * kRowsLoad + wave * 8) >> 5) & 1) ? b_base1 : b_base0;
-  };
-  auto fetch = [&](char* a_lds, char* b_lds, int64_t k0) {
-    const int64_t left = kbytes - k0;
-    if (left >= 128) {
+  // kWhole: every element of the run is there; else pieces and rows behind the end of k are zeros (and runs behind
+  // the last are all zeros: the number of loads under way is always the same)
+  auto fetch = [&](char* stage, int64_t run, auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;
+    const int64_t u = first + run;
+    const bool second = kBT && u >= p.part_runs;
+    const int64_t ub = second ? u - p.part_runs : u;
+    const char* a = a_base + (kAT ? u * kRows * p.lda : u * 64);
+    const char* b = (second ? b_base1 : b_base) + (kBT ? ub * kRows * p.ldb0 : u * 64);
+    const int64_t left_a = kAT ? p.depth - u * kRows : p.kbytes - u * 64, left_b = kBT ? p.depth - ub * kRows : p.kbytes - u * 64;
 #pragma unroll
-      for (int j = 0; j < S::kLoadA; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(a_base + k0 + oa[j]), (lptr_t)(a_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
-#pragma unroll
-      for (int j = 0; j < S::kLoadB; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(b_base(j) + k0 + ob[j]), (lptr_t)(b_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
-    } else {
-      const bool in = piece_at < left;
-#pragma unroll
-      for (int j = 0; j < S::kLoadA; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(in ? a_base + k0 + oa[j] : zero),
-                                         (lptr_t)(a_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
-#pragma unroll
-      for (int j = 0; j < S::kLoadB; ++j)
-        __builtin_amdgcn_global_load_lds((gptr_t)(in ? b_base(j) + k0 + ob[j] : zero),
-                                         (lptr_t)(b_lds + (j * kRowsLoad + wave * 8) * 128), 16, 0, 0);
+    for (int j = 0; j < 2; ++j) {
+      const bool in_a = kWhole || la.at[j] < left_a, in_b = kWhole || lb.at[j] < left_b;
+      char* to = stage + (j * S::kThreads + wave * kWave) * 16;
+      __builtin_amdgcn_global_load_lds((gptr_t)(in_a ? a + la.off[j] : zero), (lptr_t)(to), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gptr_t)(in_b ? b + lb.off[j] : zero), (lptr_t)(to + kHalf), 16, 0, 0);
     }
   };
 
@@ -333,16 +417,13 @@ __global__ void __launch_bounds__(WM* WN* kWave, 2) tile_kernel(Product p, int t
   for (int i = 0; i < S::kMI; ++i)
 #pragma unroll
     for (int j = 0; j < S::kNI; ++j) acc[i][j] = Acc{};
-  const int wm = wave / WN, wn = wave % WN;
-  const int l15 = lane & 15, q = lane >> 4, swz = (l15 >> 1) & 7;
-  const int a_row = (wm * S::kRowsM + l15) * 128, b_row = (wn * 64 + l15) * 128;
+  const int wm = wave / S::WN, wn = wave % S::WN;
   i32x4 a[S::kMI], b[S::kNI];
-  auto read = [&](const char* a_lds, const char* b_lds, int h) {
-    const int piece = ((h * 4 + q) ^ swz) * 16;
+  auto read = [&](const char* stage) {
 #pragma unroll
-    for (int j = 0; j < S::kNI; ++j) b[j] = *reinterpret_cast<const i32x4*>(b_lds + b_row + j * 2048 + piece);
+    for (int j = 0; j < S::kNI; ++j) b[j] = operand<T, kTile, kBT>(stage + kHalf, wn * S::kNI + j, lane);
 #pragma unroll
-    for (int i = 0; i < S::kMI; ++i) a[i] = *reinterpret_cast<const i32x4*>(a_lds + a_row + i * 2048 + piece);
+    for (int i = 0; i < S::kMI; ++i) a[i] = operand<T, kTile, kAT>(stage, wm * S::kMI + i, lane);
   };
   auto multiply = [&]() {
 #pragma unroll
@@ -350,119 +431,6 @@ __global__ void __launch_bounds__(WM* WN* kWave, 2) tile_kernel(Product p, int t
 #pragma unroll
       for (int j = 0; j < S::kNI; ++j) acc[i][j] = Mma<T>::mma(b[j], a[i], acc[i][j]);
   };
-
-  const int64_t steps = (kbytes + 127) / 128;
-  fetch(a_lds0, b_lds0, 0);
-  __syncthreads();
-  auto both = [&](const char* a_lds, const char* b_lds) {
-    read(a_lds, b_lds, 0);
-    multiply();
-    __builtin_amdgcn_sched_barrier(0);      // one half's operands in registers at a time
-    read(a_lds, b_lds, 1);
-    multiply();
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  for (int64_t pair = 0; pair < steps / 2; ++pair) {
-    fetch(a_lds1, b_lds1, (2 * pair + 1) * 128);
-    both(a_lds0, b_lds0);
-    __syncthreads();
-    if (2 * pair + 2 < steps) fetch(a_lds0, b_lds0, (2 * pair + 2) * 128);
-    both(a_lds1, b_lds1);
-    __syncthreads();
-  }
-  if (steps & 1) both(a_lds0, b_lds0);
-
-  if (p.partial != nullptr) {
-    i32x4* to = p.partial + (((static_cast<int64_t>(blockIdx.y) * total + tile) * (WM * WN) + wave) * (S::kMI * S::kNI)) * kWave + lane;
-#pragma unroll
-    for (int i = 0; i < S::kMI; ++i)
-#pragma unroll
-      for (int j = 0; j < S::kNI; ++j) to[(i * S::kNI + j) * kWave] = __builtin_bit_cast(i32x4, acc[i][j]);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < S::kMI; ++i) finish_rows<T, S, kGated>(p, m0, n0, wm * S::kRowsM + i * 16, wn, lane, acc[i]);
-}
-
-// The 256 x 256 tile of 8 waves (2 x 4), where the products are large enough for the matrix cores to be
-// the bound.  Two waves share a SIMD, one of each half of the block (wave / 4), and the halves run half a
-// phase apart: while one half's waves read their operands from LDS, the other's multiply.
-//
-// k goes in runs of 64 bytes, of which LDS holds four in a ring (32 KB each: 256 rows of A, 256 slots of B).
-// Run u is read in phase 2 u by the first half and in phase 2 u + 1 by the second, and multiplied in the phase
-// after; every phase ends at a barrier of the whole block (the second half passes one more before its first
-// phase, the first half one more behind its last).  Before it reads run u a half fetches run u + 3: into the
-// ring's place of run u - 1, which was last read in phase 2 u - 1, whose reads had landed (lgkmcnt(0)) before
-// the barrier that ended it.  Run u + 1 is first read in phase 2 u + 2: at the end of their reading phases 2 u
-// and 2 u + 1 both halves have waited until no more than the 8 loads of runs u + 2 and u + 3 are under way.  So
-// a load has four phases, over 2000 cycles, to arrive.
-//
-// LDS rows are 64 bytes; piece c of row r lies at c ^ ((r >> 2) & 3): the 16 rows of an operand fall on all banks.
-template <typename T, bool kGated>
-__global__ void __launch_bounds__(512) tile256_kernel(Product p, int tiles_m, int tiles_n) {
-  using S = TileShape<256, 256, 2, 4, kGated>;
-  using Acc = typename Mma<T>::Acc;
-  constexpr int kStage = 2 * 256 * 64;
-  __shared__ __attribute__((aligned(1024))) char stage0[kStage];
-  __shared__ __attribute__((aligned(1024))) char stage1[kStage];
-  __shared__ __attribute__((aligned(1024))) char stage2[kStage];
-  __shared__ __attribute__((aligned(1024))) char stage3[kStage];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int total = tiles_m * tiles_n;
-  const int tile = xcd_tile(blockIdx.x, total);
-  int tm, tn;
-  tile_place(tile, tiles_m, tiles_n, &tm, &tn);
-  const int64_t m0 = static_cast<int64_t>(tm) * 256, n0 = static_cast<int64_t>(tn) * S::kColsOut;
-
-  // a lane fetches one piece of each of two rows of A and two slots of B a run
-  const int64_t k_first = static_cast<int64_t>(blockIdx.y) * p.slice_bytes;
-  const int64_t kbytes = p.kbytes - k_first < p.slice_bytes ? p.kbytes - k_first : p.slice_bytes;
-  const bool up = kGated && ((wave >> 1) & 1);          // slots 32 to 63 of each 64 are the second B's
-  const uint32_t lda = static_cast<uint32_t>(p.lda), ldb = static_cast<uint32_t>(up ? p.ldb1 : p.ldb0);
-  const char* a_base = p.a + m0 * p.lda + k_first;
-  const char* b_base = (up ? p.b1 + n0 * p.ldb1 : p.b0 + n0 * p.ldb0) + k_first;
-  const int rows_left = p.m - m0 < 256 ? static_cast<int>(p.m - m0) : 256;
-  const int cols_left = p.n - n0 < S::kColsOut ? static_cast<int>(p.n - n0) : S::kColsOut;
-  const int piece_at = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
-  uint32_t oa[2], ob[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = j * 128 + wave * 16 + (lane >> 2);
-    oa[j] = static_cast<uint32_t>(r < rows_left ? r : rows_left - 1) * lda + piece_at;       // rows behind the last are not stored
-    int which;
-    const int c = slot_column<kGated>(r, &which);
-    ob[j] = static_cast<uint32_t>(c < cols_left ? c : cols_left - 1) * ldb + piece_at;
-  }
-  const char* zero = reinterpret_cast<const char*>(&kZeroPiece);
-  auto fetch = [&](char* stage, int64_t run) {          // a run that the row fills
-    const int64_t k0 = run * 64;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      __builtin_amdgcn_global_load_lds((gptr_t)(a_base + k0 + oa[j]), (lptr_t)(stage + (j * 128 + wave * 16) * 64), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gptr_t)(b_base + k0 + ob[j]), (lptr_t)(stage + 16384 + (j * 128 + wave * 16) * 64), 16, 0, 0);
-    }
-  };
-  auto fetch_last = [&](char* stage, int64_t run) {     // one that it may not fill
-    const int64_t k0 = run * 64;
-    const bool in = piece_at < kbytes - k0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      __builtin_amdgcn_global_load_lds((gptr_t)(in ? a_base + k0 + oa[j] : zero), (lptr_t)(stage + (j * 128 + wave * 16) * 64), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gptr_t)(in ? b_base + k0 + ob[j] : zero),
-                                       (lptr_t)(stage + 16384 + (j * 128 + wave * 16) * 64), 16, 0, 0);
-    }
-  };
-
-  Acc acc[S::kMI][S::kNI];
-#pragma unroll
-  for (int i = 0; i < S::kMI; ++i)
-#pragma unroll
-    for (int j = 0; j < S::kNI; ++j) acc[i][j] = Acc{};
-  const int half = wave >> 2, wn = wave & 3;
-  const int l15 = lane & 15, q = lane >> 4;
-  const int a_at = (half * 128 + l15) * 64 + (q ^ ((l15 >> 2) & 3)) * 16;
-  const int b_at = 16384 + (wn * 64 + l15) * 64 + (q ^ ((l15 >> 2) & 3)) * 16;
   auto meet = [&]() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
@@ -477,53 +445,69 @@ __global__ void __launch_bounds__(512) tile256_kernel(Product p, int tiles_m, in
     __builtin_amdgcn_s_waitcnt(0x0078);        // vmcnt(8) lgkmcnt(0)
     asm volatile("" ::: "memory");
   };
-  const int64_t runs = (kbytes + 63) / 64;
-  // run u in `now`, run u + 3 into `then`; kAll: the row fills it (else zeros behind its end, so that the
-  // number of loads under way is always the same)
-  auto run_step = [&](const char* now, char* then, int64_t u, auto all) {
-    constexpr bool kAll = decltype(all)::value;
-    i32x4 a[S::kMI], b[S::kNI];
-    if constexpr (kAll) fetch(then, u + 3);
-    else fetch_last(then, u + 3);
-#pragma unroll
-    for (int j = 0; j < S::kNI; ++j) b[j] = *reinterpret_cast<const i32x4*>(now + b_at + j * 1024);
-#pragma unroll
-    for (int i = 0; i < S::kMI; ++i) a[i] = *reinterpret_cast<const i32x4*>(now + a_at + i * 1024);
+  const int half = wave >> 2;
+  auto run_step = [&](const char* now, char* then, int64_t u, auto whole) {
+    if constexpr (kTile == 256) {
+      fetch(then, u + 3, whole);
+      read(now);
+      wait_loads();
+      meet();
+      __builtin_amdgcn_s_setprio(1);
+      multiply();
+      __builtin_amdgcn_s_setprio(0);
+      meet();
+    } else {
+      wait_loads();
+      meet();
+      fetch(then, u + 3, whole);
+      read(now);
+      multiply();
+    }
+  };
+  fetch(stage0, 0, std::false_type{});
+  fetch(stage1, 1, std::false_type{});
+  fetch(stage2, 2, std::false_type{});
+  if constexpr (kTile == 256) {
     wait_loads();
     meet();
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int i = 0; i < S::kMI; ++i)
-#pragma unroll
-      for (int j = 0; j < S::kNI; ++j) acc[i][j] = Mma<T>::mma(b[j], a[i], acc[i][j]);
-    __builtin_amdgcn_s_setprio(0);
-    meet();
-  };
-  fetch_last(stage0, 0);
-  fetch_last(stage1, 1);
-  fetch_last(stage2, 2);
-  wait_loads();
-  meet();
-  if (half) meet();
+    if (half) meet();
+  }
   int64_t u = 0;
-  const int64_t whole = kbytes / 64;                     // runs that the row fills
+  const int64_t whole = p.whole_runs - first < runs ? p.whole_runs - first : runs;     // runs before the first that is not
   for (; u + 7 <= whole; u += 4) {
     run_step(stage0, stage3, u, std::true_type{});
     run_step(stage1, stage0, u + 1, std::true_type{});
     run_step(stage2, stage1, u + 2, std::true_type{});
     run_step(stage3, stage2, u + 3, std::true_type{});
   }
-  for (; u < runs; u += 4) {
+  for (; runs - u > 7; u += 4) {
     run_step(stage0, stage3, u, std::false_type{});
-    if (u + 1 < runs) run_step(stage1, stage0, u + 1, std::false_type{});
-    if (u + 2 < runs) run_step(stage2, stage1, u + 2, std::false_type{});
-    if (u + 3 < runs) run_step(stage3, stage2, u + 3, std::false_type{});
+    run_step(stage1, stage0, u + 1, std::false_type{});
+    run_step(stage2, stage1, u + 2, std::false_type{});
+    run_step(stage3, stage2, u + 3, std::false_type{});
   }
-  if (!half) meet();
+  // the last one to seven, in a row: left early from inside a loop, the compiler would see ways back to its head on
+  // which loads are under way that are not, and wait for them
+  do {
+    run_step(stage0, stage3, u, std::false_type{});
+    if (u + 1 >= runs) break;
+    run_step(stage1, stage0, u + 1, std::false_type{});
+    if (u + 2 >= runs) break;
+    run_step(stage2, stage1, u + 2, std::false_type{});
+    if (u + 3 >= runs) break;
+    run_step(stage3, stage2, u + 3, std::false_type{});
+    if (u + 4 >= runs) break;
+    run_step(stage0, stage3, u + 4, std::false_type{});
+    if (u + 5 >= runs) break;
+    run_step(stage1, stage0, u + 5, std::false_type{});
+    if (u + 6 >= runs) break;
+    run_step(stage2, stage1, u + 6, std::false_type{});
+  } while (false);
+  if (kTile == 256 && !half) meet();
   __builtin_amdgcn_s_waitcnt(0x0070);        // no load is under way into LDS when the block gives it back
 
   if (p.partial != nullptr) {
-    i32x4* to = p.partial + ((static_cast<int64_t>(blockIdx.y) * total + tile) * 8 + wave) * (S::kMI * S::kNI) * kWave + lane;
+    i32x4* to = p.partial + ((static_cast<int64_t>(blockIdx.y) * total + tile) * (S::WM * S::WN) + wave) * (S::kMI * S::kNI) * kWave + lane;
 #pragma unroll
     for (int i = 0; i < S::kMI; ++i)
 #pragma unroll
@@ -531,25 +515,25 @@ __global__ void __launch_bounds__(512) tile256_kernel(Product p, int tiles_m, in
     return;
   }
 #pragma unroll
-  for (int i = 0; i < S::kMI; ++i) finish_rows<T, S, kGated>(p, m0, n0, half * 128 + i * 16, wn, lane, acc[i]);
+  for (int i = 0; i < S::kMI; ++i) finish_rows<T, kGated, kBT>(p, m0, n0, (wm * S::kMI + i) * 16, wn, lane, acc[i]);
 }
 
 // The slices' sums of a split product, added in order by waves that each take the 16 rows that one wave
 // of the tile kernel holds in acc[i], and finished as there.
-template <typename T, int BM, int BN, int WM, int WN, bool kGated>
+template <typename T, int kTile, bool kGated, bool kBT>
 __global__ void __launch_bounds__(256) join_kernel(Product p, int tiles_m, int tiles_n, int slices) {
-  using S = TileShape<BM, BN, WM, WN, kGated>;
+  using S = TileShape<kTile, kGated>;
   using Acc = typename Mma<T>::Acc;
   const int lane = threadIdx.x & (kWave - 1);
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;   // (tile, wave, i)
-  const int64_t total = static_cast<int64_t>(tiles_m) * tiles_n, per_tile = WM * WN * S::kMI;
+  const int64_t total = static_cast<int64_t>(tiles_m) * tiles_n, per_tile = S::WM * S::WN * S::kMI;
   if (unit >= total * per_tile) return;
   const int tile = static_cast<int>(unit / per_tile), in_tile = static_cast<int>(unit - tile * per_tile);
   const int wave = in_tile / S::kMI, i = in_tile - wave * S::kMI;
   int tm, tn;
   tile_place(tile, tiles_m, tiles_n, &tm, &tn);
-  const i32x4* from = p.partial + ((static_cast<int64_t>(tile) * (WM * WN) + wave) * S::kMI + i) * S::kNI * kWave + lane;
-  const int64_t stride = total * (WM * WN) * S::kMI * S::kNI * kWave;
+  const i32x4* from = p.partial + ((static_cast<int64_t>(tile) * (S::WM * S::WN) + wave) * S::kMI + i) * S::kNI * kWave + lane;
+  const int64_t stride = total * (S::WM * S::WN) * S::kMI * S::kNI * kWave;
   Acc acc[S::kNI];
 #pragma unroll
   for (int j = 0; j < S::kNI; ++j) acc[j] = __builtin_bit_cast(Acc, from[j * kWave]);
@@ -558,8 +542,8 @@ __global__ void __launch_bounds__(256) join_kernel(Product p, int tiles_m, int t
 #pragma unroll
     for (int j = 0; j < S::kNI; ++j) acc[j] += __builtin_bit_cast(Acc, from[j * kWave]);
   }
-  finish_rows<T, S, kGated>(p, static_cast<int64_t>(tm) * BM, static_cast<int64_t>(tn) * S::kColsOut,
-                            wave / WN * S::kRowsM + i * 16, wave % WN, lane, acc);
+  finish_rows<T, kGated, kBT>(p, static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * S::kColsOut,
+                              (wave / S::WN * S::kMI + i) * 16, wave % S::WN, lane, acc);
 }
 
 // ------------------------------------------------------------------------------- few rows
@@ -655,7 +639,7 @@ constexpr int64_t kMaxRowBytes = int64_t{1} << 23;     // the tile loads' offset
 // (gated: `tile` / 2 columns), k in `slices`.
 struct Plan {
   int tile, slices;
-  int64_t slice_bytes;
+  int64_t slice_runs;
   size_t workspace;
 };
 
@@ -667,12 +651,12 @@ struct Plan {
 //   tiles: a step of 128 bytes of k takes a CU 1.6 us at 256 x 256 (1.2 while half of the chip is idle); at
 //     128 x 128 0.65 us alone and 1.0 us for the two that share a CU; fp32 is bound by its MFMAs (8, 2.1, 4.1 us);
 //   slices: one more launch, and their sums written and read.
-inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool fp32) {
-  Plan best{0, 1, kbytes, 0};
-  if (m <= 16) return best;
+inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool fp32, bool few) {
+  Plan best{0, 1, cdiv(kbytes, 64), 0};
+  if (few && m <= 16) return best;
   const int64_t steps = cdiv(kbytes, 128);
   double least = 1e300;
-  if (m <= 512) {
+  if (few && m <= 512) {
     const double byte = (fp32 ? 0.0025 : 0.0023) * (gated ? (fp32 ? 1.6 : 1.22) : 1.0) * (m <= 32 ? 0.68 : 1.0);
     least = 4.0 + cdiv(cdiv(n, 16) * cdiv(m, 64), 256) * kbytes * byte;
   }
@@ -694,53 +678,57 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool 
       if (slices > 1) time += 6.0 + 2.0 * bytes / 7e6;
       if (time < least) {
         least = time;
-        best = Plan{tile, static_cast<int>(slices), each * 128, slices > 1 ? static_cast<size_t>(bytes) : 0};
+        best = Plan{tile, static_cast<int>(slices), each * 2, slices > 1 ? static_cast<size_t>(bytes) : 0};
       }
     }
   }
   return best;
 }
 
-template <typename T, bool kGated, int kTile, int WM, int WN>
-void launch_tiles(Product& p, const Plan& plan, int64_t tm, int64_t tn, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(tm * tn), plan.slices);
-  if constexpr (kTile == 256)
-    hipLaunchKernelGGL((tile256_kernel<T, kGated>), grid, dim3(512), 0, stream, p, static_cast<int>(tm), static_cast<int>(tn));
-  else
-    hipLaunchKernelGGL((tile_kernel<T, kTile, kTile, WM, WN, kGated>), grid, dim3(WM * WN * kWave), 0, stream, p,
-                       static_cast<int>(tm), static_cast<int>(tn));
+template <typename T, int kTile, bool kGated, bool kAT, bool kBT>
+void launch_tiles(const Product& p, const Plan& plan, int64_t tm, int64_t tn, hipStream_t stream) {
+  hipLaunchKernelGGL((tile_kernel<T, kTile, kGated, kAT, kBT>), dim3(static_cast<unsigned>(tm * tn), plan.slices),
+                     dim3(TileShape<kTile, kGated>::kThreads), 0, stream, p, static_cast<int>(tm), static_cast<int>(tn));
   if (plan.slices > 1) {
     const int64_t units = tm * tn * (kTile * kTile / (16 * 64));
-    hipLaunchKernelGGL((join_kernel<T, kTile, kTile, WM, WN, kGated>), dim3(static_cast<unsigned>(cdiv(units, 4))), dim3(256), 0,
-                       stream, p, static_cast<int>(tm), static_cast<int>(tn), plan.slices);
+    hipLaunchKernelGGL((join_kernel<T, kTile, kGated, kBT>), dim3(static_cast<unsigned>(cdiv(units, 4))), dim3(256), 0, stream, p,
+                       static_cast<int>(tm), static_cast<int>(tn), plan.slices);
   }
 }
 
-template <typename T, bool kGated>
-int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, const char* what) {
-  const Plan plan = plan_product(p.m, p.n, p.kbytes, kGated, std::is_same<T, float>::value);
+template <typename T, bool kGated, bool kAT, bool kBT>
+int launch_planned(Product p, const Plan& plan, void* ws, size_t ws_bytes, hipStream_t stream, const char* what) {
   SAGE_REQUIRE(p.lda < kMaxRowBytes && p.ldb0 < kMaxRowBytes && p.ldb1 < kMaxRowBytes, SAGE_ELIMIT, "%s: rows more than %ld bytes apart",
                what, (long)kMaxRowBytes);
-  if (plan.tile == 0) {
-    const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), static_cast<unsigned>(cdiv(p.m, 64)));   // m <= 512
-    // 32 columns a block where 17 to 32 rows would otherwise be read for every 16 (8-bit pair of 8192 x 2048 against 24
-    // rows 10.9 -> 10.3 us, bf16 pair of 5632 x 2048 against 20 rows 19.1 -> 16.9; more or fewer pieces a turn and 32
-    // columns for other row counts measured the same or slower)
-    const dim3 half(static_cast<unsigned>(cdiv(p.n, 32)), 1), threads(kFewWaves * kWave);
-    if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated, 1>), grid, threads, 0, stream, p);
-    else if (p.m <= 32 && p.n >= 4096) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 2>), half, threads, 0, stream, p);
-    else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 1>), grid, threads, 0, stream, p);
-    else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated, 1>), grid, threads, 0, stream, p);
-  } else {
-    SAGE_REQUIRE(plan.workspace <= ws_bytes && (plan.workspace == 0 || rows16(ws, 0)), SAGE_EWORKSPACE,
-                 "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, plan.workspace);
-    const int64_t tm = cdiv(p.m, plan.tile), tn = cdiv(p.n, kGated ? plan.tile / 2 : plan.tile);
-    SAGE_REQUIRE(tm * tn < (int64_t{1} << 24), SAGE_ELIMIT, "%s: %ld output tiles", what, (long)(tm * tn));
-    p.slice_bytes = plan.slice_bytes;
-    p.partial = plan.slices > 1 ? static_cast<i32x4*>(ws) : nullptr;
-    if (plan.tile == 256) launch_tiles<T, kGated, 256, 2, 4>(p, plan, tm, tn, stream);
-    else launch_tiles<T, kGated, 128, 2, 2>(p, plan, tm, tn, stream);
-  }
+  SAGE_REQUIRE(plan.workspace <= ws_bytes && (plan.workspace == 0 || rows16(ws, 0)), SAGE_EWORKSPACE,
+               "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, plan.workspace);
+  const int64_t tm = cdiv(p.m, plan.tile), tn = cdiv(p.n, kGated ? plan.tile / 2 : plan.tile);
+  SAGE_REQUIRE(tm * tn < (int64_t{1} << 24), SAGE_ELIMIT, "%s: %ld output tiles", what, (long)(tm * tn));
+  p.slice_runs = plan.slice_runs;
+  p.partial = plan.slices > 1 ? static_cast<i32x4*>(ws) : nullptr;
+  if (plan.tile == 256) launch_tiles<T, 256, kGated, kAT, kBT>(p, plan, tm, tn, stream);
+  else launch_tiles<T, 128, kGated, kAT, kBT>(p, plan, tm, tn, stream);
+  SAGE_CHECK_LAUNCH(what);
+  return SAGE_OK;
+}
+
+// rows of both operands along k
+template <typename T, bool kGated>
+int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, const char* what) {
+  const Plan plan = plan_product(p.m, p.n, p.kbytes, kGated, std::is_same<T, float>::value, true);
+  p.runs = cdiv(p.kbytes, 64);
+  p.part_runs = p.runs;
+  p.whole_runs = p.kbytes / 64;
+  if (plan.tile != 0) return launch_planned<T, kGated, false, false>(p, plan, ws, ws_bytes, stream, what);
+  const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), static_cast<unsigned>(cdiv(p.m, 64)));   // m <= 512
+  // 32 columns a block where 17 to 32 rows would otherwise be read for every 16 (8-bit pair of 8192 x 2048 against 24
+  // rows 10.9 -> 10.3 us, bf16 pair of 5632 x 2048 against 20 rows 19.1 -> 16.9; more or fewer pieces a turn and 32
+  // columns for other row counts measured the same or slower)
+  const dim3 half(static_cast<unsigned>(cdiv(p.n, 32)), 1), threads(kFewWaves * kWave);
+  if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated, 1>), grid, threads, 0, stream, p);
+  else if (p.m <= 32 && p.n >= 4096) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 2>), half, threads, 0, stream, p);
+  else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 1>), grid, threads, 0, stream, p);
+  else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated, 1>), grid, threads, 0, stream, p);
   SAGE_CHECK_LAUNCH(what);
   return SAGE_OK;
 }
@@ -757,63 +745,46 @@ int product_by_type(const Product& p, int dtype, void* ws, size_t ws_bytes, hipS
 }
 
 // ------------------------------------------------------------------------------- backward pass
-// dg = dh * u * act'(g), du = dh * act(g) for a 64 x 64 piece, each rounded once to the operands' type
-// (the matrix cores take no wider one), written as rows [m, 2 h] for dx and, turned over in LDS, as
-// rows [2 h, m] for the weights' gradients.  Columns between a row's end and its stride are zeros.
+// dg = dh * u * act'(g), du = dh * act(g), each rounded once to the operands' type (the matrix cores take no wider
+// one), as the rows [dg, zeros to wide, du, zeros to wide] that both products read: along h for dx, across for the
+// weights' gradients.  Bound by HBM: 8 bytes of g and u and one element of dh read, two elements written.
 template <typename T>
 __global__ void __launch_bounds__(256) gate_bwd_kernel(const T* dh, int64_t ld_dh, const float* saved, int act, int64_t m,
-                                                       int64_t h, T* rows, int64_t ld_rows, T* cols, int64_t ld_cols) {
-  __shared__ T lds[2][64][65];
+                                                       int64_t h, int64_t wide, T* out) {
   constexpr bool kExact = std::is_same<T, float>::value;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 64, h0 = static_cast<int64_t>(blockIdx.x) * 64;
-  const int c = threadIdx.x & 63, r0 = threadIdx.x >> 6;
-#pragma unroll 4
-  for (int r = r0; r < 64; r += 4) {
-    const int64_t row = m0 + r, col = h0 + c;
-    T dg = static_cast<T>(0.f), du = static_cast<T>(0.f);
-    if (row < m && col < h) {
-      const float g = saved[row * h + col], u = saved[(m + row) * h + col];
-      const float d = static_cast<float>(dh[row * ld_dh + col]);
-      dg = static_cast<T>(d * u * act_slope<kExact>(g, act));
-      du = static_cast<T>(d * act_value<kExact>(g, act));
-      if (rows != nullptr) {
-        rows[row * ld_rows + col] = dg;
-        rows[row * ld_rows + h + col] = du;
+  const int64_t per = wide / 4, total = m * per;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / per, col = (i - row * per) * 4;
+    float g[4], u[4], d[4];
+    if (col + 4 <= h) {
+      const Run<4, float> rg = *reinterpret_cast<const Run<4, float>*>(saved + row * h + col);
+      const Run<4, float> ru = *reinterpret_cast<const Run<4, float>*>(saved + (m + row) * h + col);
+      const Run<4, T> rd = *reinterpret_cast<const Run<4, T>*>(dh + row * ld_dh + col);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        g[e] = rg.v[e];
+        u[e] = ru.v[e];
+        d[e] = static_cast<float>(rd.v[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = col + e < h;
+        g[e] = in ? saved[row * h + col + e] : 0.f;
+        u[e] = in ? saved[(m + row) * h + col + e] : 0.f;
+        d[e] = in ? static_cast<float>(dh[row * ld_dh + col + e]) : 0.f;
       }
     }
-    lds[0][r][c] = dg;
-    lds[1][r][c] = du;
-  }
-  // the padding behind column 2 h of a row
-  if (rows != nullptr && blockIdx.x == gridDim.x - 1 && c < ld_rows - 2 * h)
-    for (int r = r0; r < 64; r += 4)
-      if (m0 + r < m) rows[(m0 + r) * ld_rows + 2 * h + c] = static_cast<T>(0.f);
-  if (cols == nullptr) return;
-  __syncthreads();
-#pragma unroll 4
-  for (int r = r0; r < 64; r += 4) {
-    const int64_t col = h0 + r, row = m0 + c;     // zeros where row >= m
-    if (col < h && row < ld_cols) {
-      cols[col * ld_cols + row] = lds[0][c][r];
-      cols[(h + col) * ld_cols + row] = lds[1][c][r];
+    Run<4, T> dg, du;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dg.v[e] = static_cast<T>(d[e] * u[e] * act_slope<kExact>(g[e], act));
+      du.v[e] = static_cast<T>(d[e] * act_value<kExact>(g[e], act));
     }
+    T* to = out + row * 2 * wide + col;
+    *reinterpret_cast<Run<4, T>*>(to) = dg;
+    *reinterpret_cast<Run<4, T>*>(to + wide) = du;
   }
-}
-
-// out[c, at + r] = in[r, c], zeros for rows between `rows` and `padded`
-template <typename T>
-__global__ void __launch_bounds__(256) transpose_kernel(const T* in, int64_t ld_in, int64_t rows, int64_t cols, T* out,
-                                                        int64_t ld_out, int64_t at, int64_t padded) {
-  __shared__ T lds[64][65];
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, c0 = static_cast<int64_t>(blockIdx.x) * 64;
-  const int x = threadIdx.x & 63, y0 = threadIdx.x >> 6;
-#pragma unroll 4
-  for (int y = y0; y < 64; y += 4)
-    lds[y][x] = r0 + y < rows && c0 + x < cols ? in[(r0 + y) * ld_in + c0 + x] : static_cast<T>(0.f);
-  __syncthreads();
-#pragma unroll 4
-  for (int y = y0; y < 64; y += 4)
-    if (c0 + y < cols && r0 + x < padded) out[(c0 + y) * ld_out + at + r0 + x] = lds[x][y];
 }
 
 __global__ void __launch_bounds__(256) pad_rows_kernel(const uint8_t* in, int64_t ld_in, int64_t row_bytes, uint8_t* out,
@@ -834,74 +805,57 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const uint8_t* in, int64_
   *reinterpret_cast<i32x4*>(out + row * ld_out + at) = __builtin_bit_cast(i32x4, k);
 }
 
+// The backward pass's workspace: [m, 2 wide] of dg and du, and the room for slices, which its two products, one
+// after the other, share.
 struct BwdLayout {
-  int64_t ld_rows, ld_cols, ld_w;          // in elements
-  size_t rows, cols, xt, wt, part, part_bytes, bytes;        // offsets
+  int64_t wide;                // h in whole runs
+  Plan dx, dw;
+  size_t part, part_bytes, bytes;
 };
 inline BwdLayout bwd_layout(int64_t m, int64_t h, int64_t k, int dtype) {
-  const int64_t piece = 16 / size_of(dtype);
+  const int64_t size = size_of(dtype), each = 64 / size;
   BwdLayout l;
-  l.ld_rows = static_cast<int64_t>(align_up(static_cast<size_t>(2 * h), static_cast<size_t>(piece)));
-  l.ld_cols = static_cast<int64_t>(align_up(static_cast<size_t>(m), static_cast<size_t>(piece)));
-  l.ld_w = l.ld_rows;
-  size_t off = 0;
-  auto take = [&](int64_t elements) {
-    const size_t at = off;
-    off = align_up(off + static_cast<size_t>(elements) * size_of(dtype), 256);
-    return at;
-  };
-  l.rows = take(m * l.ld_rows);
-  l.cols = take(2 * h * l.ld_cols);
-  l.xt = take(k * l.ld_cols);
-  l.wt = take(k * l.ld_w);
-  // the two products run one after the other and share the room for their slices
-  l.part = off;
-  const size_t for_dx = plan_product(m, k, l.ld_rows * size_of(dtype), false, dtype == SAGE_F32).workspace;
-  const size_t for_dw = plan_product(2 * h, k, l.ld_cols * size_of(dtype), false, dtype == SAGE_F32).workspace;
-  l.part_bytes = for_dx > for_dw ? for_dx : for_dw;
-  l.bytes = off + l.part_bytes;
+  l.wide = cdiv(h, each) * each;
+  l.dx = plan_product(m, k, 2 * l.wide * size, false, dtype == SAGE_F32, false);
+  l.dw = plan_product(l.wide + h, k, m * size, false, dtype == SAGE_F32, false);
+  l.part = align_up(static_cast<size_t>(m * 2 * l.wide * size), 256);
+  l.part_bytes = l.dx.workspace > l.dw.workspace ? l.dx.workspace : l.dw.workspace;
+  l.bytes = l.part + l.part_bytes;
   return l;
 }
 
 template <typename T>
-int gated_bwd(const void* dh, int64_t ld_dh, const void* x, int64_t ld_x, const void* wg, int64_t ld_g, const void* wu,
-              int64_t ld_u, const float* saved, int act, int64_t m, int64_t h, int64_t k, int dtype, void* dx,
-              int64_t ld_dx, void* dw, char* ws, hipStream_t st, const char* what) {
+int gated_bwd(const void* dh, int64_t ld_dh, const void* x, int64_t ld_x, const void* wg, const void* wu, int64_t ld_w,
+              const float* saved, int act, int64_t m, int64_t h, int64_t k, int dtype, void* dx, int64_t ld_dx, void* dw,
+              char* ws, hipStream_t st, const char* what) {
   const BwdLayout l = bwd_layout(m, h, k, dtype);
-  T* rows = reinterpret_cast<T*>(ws + l.rows);
-  T* cols = reinterpret_cast<T*>(ws + l.cols);
-  T* xt = reinterpret_cast<T*>(ws + l.xt);
-  T* wt = reinterpret_cast<T*>(ws + l.wt);
-  auto grid64 = [](int64_t c, int64_t r) { return dim3(static_cast<unsigned>(cdiv(c, 64)), static_cast<unsigned>(cdiv(r, 64))); };
-  hipLaunchKernelGGL((gate_bwd_kernel<T>), grid64(h, m), dim3(256), 0, st, static_cast<const T*>(dh), ld_dh, saved, act, m, h,
-                     dx != nullptr ? rows : nullptr, l.ld_rows, dw != nullptr ? cols : nullptr, l.ld_cols);
+  constexpr int64_t kRows = 64 / sizeof(T);
+  const int64_t units = cdiv(m * (l.wide / 4), 256);
+  hipLaunchKernelGGL((gate_bwd_kernel<T>), dim3(static_cast<unsigned>(units < 16384 ? units : 16384)), dim3(256), 0, st,
+                     static_cast<const T*>(dh), ld_dh, saved, act, m, h, l.wide, reinterpret_cast<T*>(ws));
   SAGE_CHECK_LAUNCH(what);
   if (dx != nullptr) {
-    // [k, 2 h]: the rows of B for dx[m, k] = sum over both halves of dgu[m, :] w[:, k]
-    hipLaunchKernelGGL((transpose_kernel<T>), grid64(k, h), dim3(256), 0, st, static_cast<const T*>(wg), ld_g, h, k, wt, l.ld_w,
-                       int64_t{0}, h);
-    SAGE_CHECK_LAUNCH(what);
-    hipLaunchKernelGGL((transpose_kernel<T>), grid64(k, l.ld_w - h), dim3(256), 0, st, static_cast<const T*>(wu), ld_u, h, k, wt,
-                       l.ld_w, h, l.ld_w - h);
-    SAGE_CHECK_LAUNCH(what);
+    // dx[m, k]: k runs over dg's columns against w_gate's rows, then over du's against w_up's
     Product p{};
-    p.a = reinterpret_cast<const char*>(rows); p.lda = l.ld_rows * sizeof(T);
-    p.b0 = reinterpret_cast<const char*>(wt); p.ldb0 = l.ld_w * sizeof(T);
-    p.m = m; p.n = k; p.kbytes = l.ld_rows * sizeof(T);
+    p.a = ws; p.lda = 2 * l.wide * sizeof(T);
+    p.b0 = static_cast<const char*>(wg); p.b1 = static_cast<const char*>(wu); p.ldb0 = p.ldb1 = ld_w * sizeof(T);
+    p.m = m; p.n = k; p.kbytes = 2 * l.wide * sizeof(T); p.depth = h;
+    p.part_runs = l.wide / kRows; p.runs = 2 * p.part_runs;
+    p.whole_runs = h % kRows == 0 ? p.runs : h / kRows;
     p.out = dx; p.ldo = ld_dx; p.out_dtype = dtype;
-    const int rc = launch_product<T, false>(p, ws + l.part, l.part_bytes, st, what);
+    const int rc = launch_planned<T, false, false, true>(p, l.dx, ws + l.part, l.part_bytes, st, what);
     if (rc != SAGE_OK) return rc;
   }
   if (dw != nullptr) {
-    hipLaunchKernelGGL((transpose_kernel<T>), grid64(k, l.ld_cols), dim3(256), 0, st, static_cast<const T*>(x), ld_x, m, k, xt,
-                       l.ld_cols, int64_t{0}, l.ld_cols);
-    SAGE_CHECK_LAUNCH(what);
+    // [dw_gate; dw_up]: dg's and du's columns at once; the rows of those between h and wide are not stored, and the
+    // last row is du's last column, wide + h - 1
     Product p{};
-    p.a = reinterpret_cast<const char*>(cols); p.lda = l.ld_cols * sizeof(T);
-    p.b0 = reinterpret_cast<const char*>(xt); p.ldb0 = l.ld_cols * sizeof(T);
-    p.m = 2 * h; p.n = k; p.kbytes = l.ld_cols * sizeof(T);
+    p.a = ws; p.lda = 2 * l.wide * sizeof(T);
+    p.b0 = static_cast<const char*>(x); p.ldb0 = ld_x * sizeof(T);
+    p.m = l.wide + h; p.n = k; p.depth = m; p.fold = l.wide; p.fold_rows = h;
+    p.runs = cdiv(m, kRows); p.part_runs = INT64_MAX; p.whole_runs = m / kRows;
     p.out = dw; p.ldo = k; p.out_dtype = dtype;
-    return launch_product<T, false>(p, ws + l.part, l.part_bytes, st, what);
+    return launch_planned<T, false, true, true>(p, l.dw, ws + l.part, l.part_bytes, st, what);
   }
   return SAGE_OK;
 }
@@ -928,7 +882,7 @@ extern "C" int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows
 
 extern "C" size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32) {
   if (m <= 0 || n <= 0 || row_bytes <= 0) return 0;
-  return plan_product(m, n, row_bytes, gated != 0, fp32 != 0).workspace;
+  return plan_product(m, n, row_bytes, gated != 0, fp32 != 0, true).workspace;
 }
 
 #define SAGE_INT8_CHECKS(what)                                                                                          \
@@ -1006,9 +960,11 @@ extern "C" int sage_gated_linear_bwd(const void* dh, sage_i64 ld_dh, const void*
   SAGE_REQUIRE(known_act(activation), SAGE_EINVAL, "sage_gated_linear_bwd: unknown activation %d", activation);
   SAGE_REQUIRE(m > 0 && h > 0 && k > 0, SAGE_EINVAL, "sage_gated_linear_bwd: bad shape m %ld h %ld k %ld", (long)m, (long)h, (long)k);
   SAGE_REQUIRE(dh && x && w_gate && w_up && saved && (dx || dw), SAGE_EINVAL, "sage_gated_linear_bwd: NULL pointer");
-  SAGE_REQUIRE(ld_dh >= 0 && ld_x >= 0 && ld_g >= 0 && ld_u >= 0 && (dx == nullptr || ld_dx >= k), SAGE_EINVAL,
-               "sage_gated_linear_bwd: row stride below the width");
-  SAGE_REQUIRE(cdiv(m, 64) < 65536 && cdiv(2 * h, 64) < 65536, SAGE_ELIMIT, "sage_gated_linear_bwd: m %ld h %ld", (long)m, (long)h);
+  const int64_t size = size_of(dtype), row_bytes = static_cast<int64_t>(align_up(static_cast<size_t>(k * size), 16));
+  SAGE_REQUIRE(ld_dh >= 0 && (dx == nullptr || ld_dx >= k), SAGE_EINVAL, "sage_gated_linear_bwd: row stride below the width");
+  SAGE_REQUIRE(rows16(x, ld_x * size) && rows16(w_gate, ld_g * size) && rows16(w_up, ld_u * size) && ld_x * size >= row_bytes &&
+                   ld_g * size >= row_bytes && ld_g == ld_u,
+               SAGE_EINVAL, "sage_gated_linear_bwd: rows are whole pieces of 16 bytes (sage_pad_rows), both weights' strides the same");
   SAGE_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
                    workspace_bytes >= sage_gated_linear_bwd_workspace_bytes(m, h, k, dtype),
                SAGE_EWORKSPACE, "sage_gated_linear_bwd: workspace of %zu bytes", workspace_bytes);
@@ -1016,8 +972,8 @@ extern "C" int sage_gated_linear_bwd(const void* dh, sage_i64 ld_dh, const void*
   hipStream_t st = static_cast<hipStream_t>(stream);
   const char* what = "sage_gated_linear_bwd";
   if (dtype == SAGE_F32)
-    return gated_bwd<float>(dh, ld_dh, x, ld_x, w_gate, ld_g, w_up, ld_u, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
+    return gated_bwd<float>(dh, ld_dh, x, ld_x, w_gate, w_up, ld_g, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
   if (dtype == SAGE_BF16)
-    return gated_bwd<__bf16>(dh, ld_dh, x, ld_x, w_gate, ld_g, w_up, ld_u, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
-  return gated_bwd<_Float16>(dh, ld_dh, x, ld_x, w_gate, ld_g, w_up, ld_u, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
+    return gated_bwd<__bf16>(dh, ld_dh, x, ld_x, w_gate, w_up, ld_g, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
+  return gated_bwd<_Float16>(dh, ld_dh, x, ld_x, w_gate, w_up, ld_g, saved, activation, m, h, k, dtype, dx, ld_dx, dw, ws, st, what);
 }

@@ -1511,11 +1511,11 @@ def rms_norm_bwd(dy, s, weight, eps=1e-6, dsum=None, need_dx=True, need_dw=True)
     return dx, dw
 
 
-def _pieces(t, p, ld):
+def _pieces(t, p, ld, copy=False):
     """The matrix itself if its rows are whole pieces of 16 bytes that start on 16 bytes, else a
     zero-filled copy that is: (pointer, row stride in elements, columns, what must stay alive)."""
     size, (rows, cols) = t.element_size(), t.shape
-    if p % 16 == 0 and ld * size % 16 == 0 and cols * size % 16 == 0 and ld * size < 1 << 23:
+    if not copy and p % 16 == 0 and ld * size % 16 == 0 and cols * size % 16 == 0 and ld * size < 1 << 23:
         return p, ld, cols, t
     each = 16 // size
     wide = (cols + each - 1) // each * each
@@ -1664,6 +1664,12 @@ def gated_linear_bwd(dh, x, w_gate, w_up, saved, activation="silu", need_dx=True
         dw = torch.zeros((2 * h, k), dtype=x.dtype, device=dev) if need_dw else None
     else:
         dw = torch.empty((2 * h, k), dtype=x.dtype, device=dev) if need_dw else None
+        px, ldx, _, keep_x = _pieces(x, px, ldx)
+        pg, ldg, _, keep_g = _pieces(w_gate, pg, ldg)
+        pu, ldu, _, keep_u = _pieces(w_up, pu, ldu)
+        if ldg != ldu:                       # the weights' rows go on from one to the other at one stride
+            pg, ldg, _, keep_g = _pieces(keep_g, pg, ldg, copy=True)
+            pu, ldu, _, keep_u = _pieces(keep_u, pu, ldu, copy=True)
         ws_bytes = _lib.load().sage_gated_linear_bwd_workspace_bytes(m, h, k, ROW_DTYPES[x.dtype])
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         _call("sage_gated_linear_bwd", dev, pd, ldd, px, ldx, pg, ldg, pu, ldu, saved.data_ptr(), act, m, h, k,

@@ -10,8 +10,7 @@ import math
 import pytest
 import torch
 
-from graphsage_amd import functional as SF
-from graphsage_amd import ops
+from graphsage_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -337,6 +336,31 @@ def test_not_a_number_stays_in_its_row(dev):
             x[m - 1, 71] = float("nan")
             out, _ = ops.gated_linear_fwd(x, w, w)
             assert bool(torch.isnan(out[m - 1]).all()) and bool(torch.isfinite(out[:m - 1]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,h,k", [(1, 1, 8), (1, 130, 208), (3, 17, 40), (40, 33, 24), (70, 130, 136), (300, 515, 200), (129, 257, 264)])
+def test_backward_writes_its_outputs_only(dev, dtype, m, h, k):
+    """dx and dw in the middle of buffers whose other elements stay as they were (widths that are no whole
+    runs, rows that fill no tile), and the workspace's next bytes too."""
+    rng = gen(dev, m + h + k)
+    x, wg, wu, dh = normal(rng, m, k, dtype=dtype), normal(rng, h, k, dtype=dtype), normal(rng, h, k, dtype=dtype), normal(rng, m, h, dtype=dtype)
+    _, saved = ops.gated_linear_fwd(x, wg, wu, save=True)
+    want = ops.gated_linear_bwd(dh, x, wg, wu, saved)
+    room = 256 * max(k, 64)
+    dx = torch.full((m * k + 2 * room,), 3.0, dtype=dtype, device=dev)
+    dw = torch.full((2 * h * k + 2 * room,), 3.0, dtype=dtype, device=dev)
+    kind = ops.ROW_DTYPES[dtype]
+    size = _lib.load().sage_gated_linear_bwd_workspace_bytes(m, h, k, kind)
+    ws = torch.full((size + (1 << 20),), 77, dtype=torch.uint8, device=dev)
+    one = x.element_size()
+    ops._call("sage_gated_linear_bwd", dev, dh.data_ptr(), h, x.data_ptr(), k, wg.data_ptr(), k, wu.data_ptr(), k, saved.data_ptr(), 0,
+              m, h, k, kind, dx.data_ptr() + room * one, k, dw.data_ptr() + room * one, ws.data_ptr(), size)
+    assert torch.equal(dx[room:-room].view(m, k), want[0])
+    assert torch.equal(dw[room:-room].view(2 * h, k), torch.cat(want[1:]))
+    assert bool((dx[:room] == 3).all()) and bool((dx[-room:] == 3).all())
+    assert bool((dw[:room] == 3).all()) and bool((dw[-room:] == 3).all())
+    assert bool((ws[size:] == 77).all())
 
 
 def test_refusals(dev):
