@@ -132,14 +132,30 @@ __device__ inline void store_out(const Product& p, int64_t row, int64_t col, con
   else store_run<n>(static_cast<float*>(p.out) + at, left, v);
 }
 
+// two values in T's 16 bits, the first in the low half
+template <typename T>
+__device__ inline uint32_t pack16(float a, float b) {
+  const T r[2] = {static_cast<T>(a), static_cast<T>(b)};
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+// n values, zeros behind the `left` that are there
+template <int n>
+__device__ inline void load_run(const float* p, int64_t left, float (&v)[n]) {
+  if (left >= n) {
+    const Run<n, float> r = *reinterpret_cast<const Run<n, float>*>(p);
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = r.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = i < left ? p[i] : 0.f;
+  }
+}
+
 // n consecutive columns of one row, from the sums of one B
 template <typename T, int n, typename S>
 __device__ inline void finish(const Product& p, int64_t row, int64_t col, const S (&c)[n]) {
   if (row >= p.m || col >= p.n) return;
-  if (p.fold > p.fold_rows) {
-    if (row >= p.fold) row -= p.fold - p.fold_rows;
-    else if (row >= p.fold_rows) return;
-  }
   float v[n];
   if constexpr (std::is_same<T, int8_t>::value) {
     const float sa = p.sa[row];
@@ -208,8 +224,9 @@ __device__ const i32x4 kZeroPiece = {0, 0, 0, 0};
 // f = r & 3 | (r >> 3 & 1) << 2, so that the 8 rows of half a wave fall on all banks.  fp32: four plain reads, and the
 // 64 bytes c of row r lie at c ^ (r >> 2 & 3).
 //
-// B's slots: where its rows lie along k, slot 16 j + i of a wave's 64 holds column 16 (i / 4) + 4 j + i % 4 (gated: 8,
-// 32 of each B), so that a lane ends with 16 (gated: 8) consecutive columns of its row of C; else column 16 j + i.
+// A wave's 64 slots of B are 64 columns, gated 32 of the first B and the same 32 of the second.  Where B's rows lie
+// along k, any column may be any slot: slot 16 j + i is column 4 i + j (gated 2 i + j % 2 of B j / 2), so that the 16
+// lanes that the MFMA leaves a row of C in hold 4 (2) consecutive columns each.
 template <int kTile, bool kGated>
 struct TileShape {
   static constexpr int kThreads = kTile == 256 ? 512 : 256;
@@ -221,12 +238,8 @@ struct TileShape {
 template <bool kGated>
 __device__ inline int slot_column(int s, int* which) {
   const int wn = s >> 6, j = (s >> 4) & 3, i = s & 15;
-  if constexpr (kGated) {
-    *which = j >> 1;
-    return wn * 32 + (i >> 2) * 8 + (j & 1) * 4 + (i & 3);
-  }
-  *which = 0;
-  return wn * 64 + (i >> 2) * 16 + j * 4 + (i & 3);
+  *which = kGated ? j >> 1 : 0;
+  return kGated ? wn * 32 + 2 * i + (j & 1) : wn * 64 + 4 * i + j;
 }
 
 // The tile of a block: each XCD (blockIdx modulo 8) takes a contiguous run of them, so that its L2 holds what
@@ -247,34 +260,107 @@ __device__ inline void tile_place(int tile, int tiles_m, int tiles_n, int* tm, i
   *tn = in / rows;
 }
 
-// C^T layout of the MFMA (B's slots are its first operand): lane l holds row l & 15, and of slot group j
-// slots 4 (l >> 4) + 0..3.
-template <typename T, bool kGated, bool kBT, typename Acc>
-__device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[4]) {
-  using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
-  const int l15 = lane & 15, q = lane >> 4;
-  if constexpr (kGated) {
-    E g[8], u[8];
+// 16 rows of C from one wave's sums, B along k.  The MFMA's rows are A's: lane l holds, of slot group j, slot l & 15 of
+// rows 4 (l >> 4) + 0..3, which the slot order makes consecutive columns over j: a store is 256 bytes of a row in fp32
+// and 128 in 16 bits (gated 128 and 64).  (With B's slots as the MFMA's rows and 16 consecutive columns a lane, a lane's
+// 16 bytes lay 64 apart: a product of 8192 x 8192 pairs over 2048 in bf16 that keeps both sums took 726 us.)
+template <typename T, bool kGated, typename Acc>
+__device__ inline void finish_along(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[4]) {
+  constexpr int n = kGated ? 2 : 4;
+  const int64_t col = n0 + (wn * 16 + (lane & 15)) * n, left = p.n - col, r0 = m0 + row + (lane >> 4) * 4;
+  if (left <= 0) return;
+  float s0[n], s1[n], bias[n];
+  if constexpr (std::is_same<T, int8_t>::value) {
+    load_run<n>(p.sb0 + col, left, s0);
+    if constexpr (kGated) load_run<n>(p.sb1 + col, left, s1);
+    if (p.bias != nullptr) load_run<n>(p.bias + col, left, bias);
+  }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      g[e] = acc[e >> 2][e & 3];
-      u[e] = acc[2 + (e >> 2)][e & 3];
+  for (int e = 0; e < 4; ++e) {
+    const int64_t r = r0 + e;
+    if (r >= p.m) break;
+    float v[n], u[n];
+    if constexpr (std::is_same<T, int8_t>::value) {
+      const float sa = p.sa[r];
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        v[j] = static_cast<float>(acc[j][e]) * (sa * s0[j]) + (p.bias != nullptr ? bias[j] : 0.f);
+        if constexpr (kGated) u[j] = static_cast<float>(acc[2 + j][e]) * (sa * s1[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        v[j] = acc[j][e];
+        if constexpr (kGated) u[j] = acc[2 + j][e];
+      }
+      if constexpr (kGated) {
+        if (p.saved != nullptr) {
+          store_run<n>(p.saved + r * p.n + col, left, v);
+          store_run<n>(p.saved + (p.m + r) * p.n + col, left, u);
+        }
+      }
     }
-    finish_gated<T, 8>(p, m0 + row + l15, n0 + wn * 32 + q * 8, g, u);
-  } else if constexpr (kBT) {
+    if constexpr (kGated) {
+#pragma unroll
+      for (int j = 0; j < n; ++j)
+        v[j] = (p.out_dtype == SAGE_F32 ? act_value<true>(v[j], p.act) : act_value<false>(v[j], p.act)) * u[j];
+    }
+    store_out<n>(p, r, col, v);
+  }
+}
+
+// The same where B's rows are rows of k, whose slots are columns in order.  There B's slots are the MFMA's rows: lane l
+// holds row l & 15, and of slot group j slots 4 q + 0..3, q = l >> 4.  In 16 bits two groups trade halves between the
+// lanes of odd and even q first, and lane q stores 8 consecutive columns, 8 (q >> 1) and on, of group j + (q & 1)
+// (dx and dw of 8192 x 8192 over 2048 in bf16 486 -> 436 us).
+template <typename T, typename Acc>
+__device__ inline void finish_across(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[4]) {
+  const int q = lane >> 4;
+  int64_t r = m0 + row + (lane & 15);
+  bool kept = r < p.m;
+  const int64_t col0 = n0 + wn * 64;
+  if (p.fold > p.fold_rows) {
+    if (r >= p.fold) r -= p.fold - p.fold_rows;
+    else kept = kept && r < p.fold_rows;
+  }
+  if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      E c[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] = acc[j][e];
-      finish<T, 4>(p, m0 + row + l15, n0 + wn * 64 + j * 16 + q * 4, c);
+      const int64_t col = col0 + j * 16 + q * 4;
+      const float v[4] = {acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
+      if (kept && col < p.n) store_run<4>(static_cast<float*>(p.out) + r * p.ldo + col, p.n - col, v);
     }
   } else {
-    E c[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) c[e] = acc[e >> 2][e & 3];
-    finish<T, 16>(p, m0 + row + l15, n0 + wn * 64 + q * 16, c);
+    for (int j = 0; j < 4; j += 2) {
+      uint32_t all[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const auto t = __builtin_amdgcn_permlane16_swap(pack16<T>(acc[j][2 * e], acc[j][2 * e + 1]),
+                                                        pack16<T>(acc[j + 1][2 * e], acc[j + 1][2 * e + 1]), false, false);
+        all[e] = t[0];
+        all[2 + e] = t[1];
+      }
+      const int64_t col = col0 + (j + (q & 1)) * 16 + (q >> 1) * 8, left = p.n - col;
+      uint16_t* to = static_cast<uint16_t*>(p.out) + r * p.ldo + col;
+      if (kept && left >= 8) {
+        Run<8, uint16_t> run;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) run.v[e] = static_cast<uint16_t>(all[e >> 1] >> (16 * (e & 1)));
+        *reinterpret_cast<Run<8, uint16_t>*>(to) = run;
+      } else if (kept) {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (e < left) to[e] = static_cast<uint16_t>(all[e >> 1] >> (16 * (e & 1)));
+      }
+    }
   }
+}
+
+template <typename T, bool kGated, bool kBT, typename Acc>
+__device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[4]) {
+  if constexpr (kBT) finish_across<T>(p, m0, n0, row, wn, lane, acc);
+  else finish_along<T, kGated>(p, m0, n0, row, wn, lane, acc);
 }
 
 // Where a lane's two loads of an operand's run come from, as offsets of 32 bits from the tile's first row (strides are
@@ -429,7 +515,7 @@ __global__ void __launch_bounds__(kTile == 256 ? 512 : 256, 2) tile_kernel(Produ
 #pragma unroll
     for (int i = 0; i < S::kMI; ++i)
 #pragma unroll
-      for (int j = 0; j < S::kNI; ++j) acc[i][j] = Mma<T>::mma(b[j], a[i], acc[i][j]);
+      for (int j = 0; j < S::kNI; ++j) acc[i][j] = kBT ? Mma<T>::mma(b[j], a[i], acc[i][j]) : Mma<T>::mma(a[i], b[j], acc[i][j]);
   };
   auto meet = [&]() {
     __builtin_amdgcn_sched_barrier(0);
