@@ -262,13 +262,14 @@ __device__ inline void tile_place(int tile, int tiles_m, int tiles_n, int* tm, i
 
 // 16 rows of C from one wave's sums, B along k.  The MFMA's rows are A's: lane l holds, of slot group j, slot l & 15 of
 // rows 4 (l >> 4) + 0..3, which the slot order makes consecutive columns over j: a store is 256 bytes of a row in fp32
-// and 128 in 16 bits (gated 128 and 64).  (With B's slots as the MFMA's rows and 16 consecutive columns a lane, a lane's
-// 16 bytes lay 64 apart: a product of 8192 x 8192 pairs over 2048 in bf16 that keeps both sums took 726 us.)
-template <typename T, bool kGated, typename Acc>
-__device__ inline void finish_along(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[4]) {
+// and 128 in 16 bits (gated 128 and 64).  kFull: all of the block's rows and columns are there; kAct, kOut: the
+// activation and the output's type, or -1: known at run time.
+template <typename T, bool kGated, bool kFull, int kAct, int kOut, typename Acc>
+__device__ inline void finish_along(const Product& p, int64_t r0, int64_t col, const Acc (&acc)[4]) {
   constexpr int n = kGated ? 2 : 4;
-  const int64_t col = n0 + (wn * 16 + (lane & 15)) * n, left = p.n - col, r0 = m0 + row + (lane >> 4) * 4;
-  if (left <= 0) return;
+  const int64_t left = kFull ? n : p.n - col;
+  if (!kFull && left <= 0) return;
+  const int act = kAct < 0 ? p.act : kAct, out_dtype = kOut < 0 ? p.out_dtype : kOut;
   float s0[n], s1[n], bias[n];
   if constexpr (std::is_same<T, int8_t>::value) {
     load_run<n>(p.sb0 + col, left, s0);
@@ -278,7 +279,7 @@ __device__ inline void finish_along(const Product& p, int64_t m0, int64_t n0, in
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int64_t r = r0 + e;
-    if (r >= p.m) break;
+    if (!kFull && r >= p.m) break;
     float v[n], u[n];
     if constexpr (std::is_same<T, int8_t>::value) {
       const float sa = p.sa[r];
@@ -303,9 +304,12 @@ __device__ inline void finish_along(const Product& p, int64_t m0, int64_t n0, in
     if constexpr (kGated) {
 #pragma unroll
       for (int j = 0; j < n; ++j)
-        v[j] = (p.out_dtype == SAGE_F32 ? act_value<true>(v[j], p.act) : act_value<false>(v[j], p.act)) * u[j];
+        v[j] = (out_dtype == SAGE_F32 ? act_value<true>(v[j], act) : act_value<false>(v[j], act)) * u[j];
     }
-    store_out<n>(p, r, col, v);
+    const int64_t at = r * p.ldo + col;
+    if (out_dtype == SAGE_BF16) store_run<n>(static_cast<__bf16*>(p.out) + at, left, v);
+    else if (out_dtype == SAGE_F16) store_run<n>(static_cast<_Float16*>(p.out) + at, left, v);
+    else store_run<n>(static_cast<float*>(p.out) + at, left, v);
   }
 }
 
@@ -357,10 +361,35 @@ __device__ inline void finish_across(const Product& p, int64_t m0, int64_t n0, i
   }
 }
 
-template <typename T, bool kGated, bool kBT, typename Acc>
-__device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, const Acc (&acc)[4]) {
-  if constexpr (kBT) finish_across<T>(p, m0, n0, row, wn, lane, acc);
-  else finish_along<T, kGated>(p, m0, n0, row, wn, lane, acc);
+// kRows x 64 slots of C from a wave's sums (kMI groups of 16 rows).  One activation and output type is compiled by
+// itself for blocks that are all there: the choices, made for every run of columns, took longer than the values.
+template <typename T, bool kGated, bool kBT, int kMI, typename Acc>
+__device__ inline void finish_rows(const Product& p, int64_t m0, int64_t n0, int row, int wn, int lane, bool full, const Acc (&acc)[kMI][4]) {
+  if constexpr (kBT) {
+#pragma unroll
+    for (int i = 0; i < kMI; ++i) finish_across<T>(p, m0, n0, row + i * 16, wn, lane, acc[i]);
+  } else {
+    constexpr int n = kGated ? 2 : 4;
+    const int64_t r0 = m0 + row + (lane >> 4) * 4, col = n0 + (wn * 16 + (lane & 15)) * n;
+    auto all = [&](auto is_full, auto act, auto out) {
+#pragma unroll
+      for (int i = 0; i < kMI; ++i)
+        finish_along<T, kGated, decltype(is_full)::value, decltype(act)::value, decltype(out)::value>(p, r0 + i * 16, col, acc[i]);
+    };
+    using any = std::integral_constant<int, -1>;
+    using silu = std::integral_constant<int, SAGE_ACT_SILU>;
+    if constexpr (std::is_same<T, int8_t>::value) {
+      if (full && (!kGated || p.act == SAGE_ACT_SILU) && p.out_dtype == SAGE_BF16)
+        all(std::true_type{}, silu{}, std::integral_constant<int, SAGE_BF16>{});
+      else if (full && (!kGated || p.act == SAGE_ACT_SILU) && p.out_dtype == SAGE_F32)
+        all(std::true_type{}, silu{}, std::integral_constant<int, SAGE_F32>{});
+      else all(std::false_type{}, any{}, any{});
+    } else {
+      using out = std::integral_constant<int, std::is_same<T, float>::value ? SAGE_F32 : std::is_same<T, __bf16>::value ? SAGE_BF16 : SAGE_F16>;
+      if (full && p.act == SAGE_ACT_SILU) all(std::true_type{}, silu{}, out{});
+      else all(std::false_type{}, any{}, out{});
+    }
+  }
 }
 
 // Where a lane's two loads of an operand's run come from, as offsets of 32 bits from the tile's first row (strides are
@@ -600,8 +629,7 @@ __global__ void __launch_bounds__(kTile == 256 ? 512 : 256, 2) tile_kernel(Produ
       for (int j = 0; j < S::kNI; ++j) to[(i * S::kNI + j) * kWave] = __builtin_bit_cast(i32x4, acc[i][j]);
     return;
   }
-#pragma unroll
-  for (int i = 0; i < S::kMI; ++i) finish_rows<T, kGated, kBT>(p, m0, n0, (wm * S::kMI + i) * 16, wn, lane, acc[i]);
+  finish_rows<T, kGated, kBT, S::kMI>(p, m0, n0, wm * S::kMI * 16, wn, lane, rows_left == kTile && cols_left == S::kColsOut, acc);
 }
 
 // The slices' sums of a split product, added in order by waves that each take the 16 rows that one wave
@@ -620,16 +648,17 @@ __global__ void __launch_bounds__(256) join_kernel(Product p, int tiles_m, int t
   tile_place(tile, tiles_m, tiles_n, &tm, &tn);
   const i32x4* from = p.partial + ((static_cast<int64_t>(tile) * (S::WM * S::WN) + wave) * S::kMI + i) * S::kNI * kWave + lane;
   const int64_t stride = total * (S::WM * S::WN) * S::kMI * S::kNI * kWave;
-  Acc acc[S::kNI];
+  Acc acc[1][S::kNI];
 #pragma unroll
-  for (int j = 0; j < S::kNI; ++j) acc[j] = __builtin_bit_cast(Acc, from[j * kWave]);
+  for (int j = 0; j < S::kNI; ++j) acc[0][j] = __builtin_bit_cast(Acc, from[j * kWave]);
   for (int s = 1; s < slices; ++s) {
     from += stride;
 #pragma unroll
-    for (int j = 0; j < S::kNI; ++j) acc[j] += __builtin_bit_cast(Acc, from[j * kWave]);
+    for (int j = 0; j < S::kNI; ++j) acc[0][j] += __builtin_bit_cast(Acc, from[j * kWave]);
   }
-  finish_rows<T, kGated, kBT>(p, static_cast<int64_t>(tm) * kTile, static_cast<int64_t>(tn) * S::kColsOut,
-                              (wave / S::WN * S::kMI + i) * 16, wave % S::WN, lane, acc);
+  const int64_t m0 = static_cast<int64_t>(tm) * kTile, n0 = static_cast<int64_t>(tn) * S::kColsOut;
+  finish_rows<T, kGated, kBT, 1>(p, m0, n0, (wave / S::WN * S::kMI + i) * 16, wave % S::WN, lane,
+                                 m0 + kTile <= p.m && n0 + S::kColsOut <= p.n, acc);
 }
 
 // ------------------------------------------------------------------------------- few rows

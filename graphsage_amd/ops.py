@@ -1346,7 +1346,7 @@ def _call(name, device, *args):
     a call tape, which keeps pointers only, does not take them."""
     if _lib._tape is not None:
         raise RuntimeError(f"{name}: not recordable on a call tape (capture a graph instead)")
-    fn, index = getattr(_lib.load(), name), device.index
+    fn, index = getattr(_lib._lib or _lib.load(), name), device.index
     if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
@@ -1358,35 +1358,38 @@ def _call(name, device, *args):
 
 def _row_matrix(t, name, dtype=None, shape=None, device=None, output=False):
     """2-D device matrix with contiguous rows -> (pointer, row stride in elements)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    try:
+        (rows, cols), (ld, inner), kind = t.shape, t.stride(), t.dtype
+    except (AttributeError, ValueError, TypeError):
+        raise RuntimeError(f"{name}: expected a 2-D CUDA (HIP) tensor, got "
+                           f"{tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}") from None
+    if not t.is_cuda:
         raise RuntimeError(f"{name}: expected a CUDA (HIP) tensor; graphsage_amd has no CPU path")
-    size = t.shape
-    if len(size) != 2:
-        raise RuntimeError(f"{name}: expected a 2-D tensor, got shape {tuple(size)}")
-    kind = t.dtype
     if kind is not dtype and (dtype is not None or kind not in ROW_DTYPES):
         raise RuntimeError(f"{name}: expected {dtype or 'fp32, bf16 or fp16'}, got {kind}")
-    if shape is not None and size != shape:
-        raise RuntimeError(f"{name}: expected shape {list(shape)}, got {list(size)}")
+    if shape is not None and (rows, cols) != shape:
+        raise RuntimeError(f"{name}: expected shape {list(shape)}, got {[rows, cols]}")
     if device is not None and t.device != device:
         raise RuntimeError(f"{name}: on {t.device}, the other operands on {device}")
-    ld, inner = t.stride()
-    rows, cols = size
     if inner != 1 and cols > 1:
         raise RuntimeError(f"{name}: expected contiguous rows, got strides {t.stride()}")
-    if rows <= 1 and ld < cols:
-        ld = cols
-    if output and ld < cols:
-        raise RuntimeError(f"{name}: the rows of an output must not overlap")
+    if ld < cols:
+        if rows <= 1:
+            ld = cols
+        elif output:
+            raise RuntimeError(f"{name}: the rows of an output must not overlap")
     return t.data_ptr(), ld
 
 
-def _vector(t, name, n, device, dtypes=(torch.float32,)):
+_FP32 = (torch.float32,)
+
+
+def _vector(t, name, n, device, dtypes=_FP32):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name}: expected a CUDA (HIP) tensor; graphsage_amd has no CPU path")
     if t.dtype not in dtypes:
         raise RuntimeError(f"{name}: expected dtype {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+    if t.shape != (n,) or not t.is_contiguous():
         raise RuntimeError(f"{name}: expected {n} contiguous elements, got shape {tuple(t.shape)}")
     if t.device != device:
         raise RuntimeError(f"{name}: on {t.device}, the other operands on {device}")
@@ -1421,7 +1424,7 @@ def _like(t, out, name):
     """`out`, checked against t's shape and dtype, or a new tensor: (tensor, pointer, row stride)."""
     if out is not None:
         return (out, *_row_matrix(out, name, t.dtype, t.shape, t.device, output=True))
-    out = t.new_empty(t.shape)
+    out = torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
     return out, out.data_ptr(), t.shape[1]
 
 
