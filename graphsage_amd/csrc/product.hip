@@ -763,13 +763,12 @@ struct Plan {
   size_t workspace;
 };
 
-// The cut with the least estimated time.  The estimate, in microseconds, follows measurements of every cut at
-// m 32 to 2048 against 1024 x 1024, 4096 x 4096, 8192 x 2048 and 2048 x 8192 in 8 bits, bf16 and fp32 (its choice
-// is 1.2 % slower than the best cut there in the geometric mean, never more than 16 %):
-//   few rows: a block's bytes of k at 2.3 us a kilobyte-thousand (more with two Bs, and in fp32, where the MFMAs
-//     count), blocks in turns of one a CU;
-//   tiles: a step of 128 bytes of k takes a CU 1.6 us at 256 x 256 (1.2 while half of the chip is idle); at
-//     128 x 128 0.65 us alone and 1.0 us for the two that share a CU; fp32 is bound by its MFMAs (8, 2.1, 4.1 us);
+// The cut with the least estimated time.  The estimate, in microseconds, is fitted to measurements of every cut at m
+// 24 to 8000 against weights of 256 x 256 to 8192 x 2048 and 2048 x 8192 in 8 bits, bf16 pairs and fp32 pairs: its
+// choice is 0.4 % slower than the best cut there in the geometric mean, and 18 % at most.
+//   few rows: a block's bytes of k at 2.2 us a thousand (more with two Bs), blocks in turns of one a CU;
+//   tiles: a step of 128 bytes of k takes a CU 1.5 us at 256 x 256 (1.4 while half of the chip is idle), at
+//     128 x 128 0.57 us alone and 1.2 us for the two that share a CU; fp32 is bound by its MFMAs (8, 2.15, 4.4 us);
 //   slices: one more launch, and their sums written and read.
 inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool fp32, bool few) {
   Plan best{0, 1, cdiv(kbytes, 64), 0};
@@ -777,8 +776,8 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool 
   const int64_t steps = cdiv(kbytes, 128);
   double least = 1e300;
   if (few && m <= 512) {
-    const double byte = (fp32 ? 0.0025 : 0.0023) * (gated ? (fp32 ? 1.6 : 1.22) : 1.0) * (m <= 32 ? 0.68 : 1.0);
-    least = 4.0 + cdiv(cdiv(n, 16) * cdiv(m, 64), 256) * kbytes * byte;
+    const double byte = 0.0022 * (gated ? (fp32 ? 1.9 : 1.4) : 1.0) * (m <= 32 ? 0.61 : 1.0);
+    least = 4.1 + cdiv(cdiv(n, 16) * cdiv(m, 64), 256) * kbytes * byte;
   }
   for (int tile : {128, 256}) {
     const int64_t tiles = cdiv(m, tile) * cdiv(n, gated ? tile / 2 : tile);
@@ -787,15 +786,15 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool 
       if (cdiv(steps, each) != slices) continue;
       double time;
       if (tile == 128) {
-        const double alone = fp32 ? 2.1 : blocks <= 128 ? 0.65 : 0.72, pair = fp32 ? 4.1 : 1.0;
+        const double alone = fp32 ? 2.15 : blocks <= 128 ? 0.56 : 0.58, pair = fp32 ? 4.4 : 1.2;
         const int64_t turns = blocks / 512, rest = blocks % 512;
-        time = each * (turns * pair + (rest == 0 ? 0.0 : rest <= 256 ? alone : pair)) + 5.5 + 2.0 * (turns - (rest == 0 ? 1 : 0));
+        time = each * (turns * pair + (rest == 0 ? 0.0 : rest <= 256 ? alone : pair)) + 7.7 + 2.0 * (turns - (rest == 0 ? 1 : 0));
       } else {
         const int64_t turns = cdiv(blocks, 256);
-        time = each * turns * (fp32 ? 8.0 : blocks <= 128 ? 1.2 : 1.62) + 9.0 + 5.0 * (turns - 1);
+        time = each * turns * (fp32 ? 8.0 : blocks <= 128 ? 1.4 : 1.5) + 12.0 + 7.5 * (turns - 1);
       }
       const double bytes = static_cast<double>(blocks) * tile * tile * 4;
-      if (slices > 1) time += 6.0 + 2.0 * bytes / 7e6;
+      if (slices > 1) time += 4.2 + 2.0 * bytes / 7.5e6;
       if (time < least) {
         least = time;
         best = Plan{tile, static_cast<int>(slices), each * 2, slices > 1 ? static_cast<size_t>(bytes) : 0};
