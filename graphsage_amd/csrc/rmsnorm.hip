@@ -357,11 +357,22 @@ __global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024, 4) rms_norm_bwd_k
   constexpr int nw = VecOf<W>::n, kW = n / nw;         // an fp32 weight of 16-bit rows is two vectors
   Pack<W> w[kNV][kW];
   float acc[kNV][n];
+  // a lane's vectors begin at `at`; the row's last is its last n elements, of which the first `skip` are the lane
+  // before's as well: both store the same dx there, one counts them (vectors behind the row: skip = n)
+  int64_t at[kNV];
+  int skip[kNV];
+#pragma unroll
+  for (int j = 0; j < kNV; ++j) {
+    at[j] = static_cast<int64_t>(j * threads + t) * n;
+    const int64_t over = at[j] + n - a.dim;
+    skip[j] = over <= 0 ? 0 : over < n ? static_cast<int>(over) : n;
+    if (skip[j] > 0) at[j] = a.dim - n;
+  }
   const W* wp = std::is_same<T, W>::value ? static_cast<const W*>(a.w) : reinterpret_cast<const W*>(a.w32);
 #pragma unroll
   for (int j = 0; j < kNV; ++j) {
 #pragma unroll
-    for (int h = 0; h < kW; ++h) w[j][h] = load_pack<W>(wp, static_cast<int64_t>(j * threads + t) * n + h * nw, a.dim);
+    for (int h = 0; h < kW; ++h) w[j][h] = *reinterpret_cast<const Pack<W>*>(wp + at[j] + h * nw);
 #pragma unroll
     for (int i = 0; i < n; ++i) acc[j][i] = 0.f;
   }
@@ -373,14 +384,15 @@ __global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024, 4) rms_norm_bwd_k
     const T* yp = static_cast<const T*>(a.dy) + row * a.ld_dy;
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
-      const int64_t at = static_cast<int64_t>(j * threads + t) * n;
-      s_next[j] = load_pack<T>(sp, at, a.dim);
-      g_next[j] = load_pack<T>(yp, at, a.dim);
+      if (skip[j] == n) continue;
+      s_next[j] = *reinterpret_cast<const Pack<T>*>(sp + at[j]);
+      g_next[j] = *reinterpret_cast<const Pack<T>*>(yp + at[j]);
     }
     if (a.ds != nullptr) {
       const T* dsp = static_cast<const T*>(a.ds) + row * a.ld_ds;
 #pragma unroll
-      for (int j = 0; j < kNV; ++j) d_next[j] = load_pack<T>(dsp, static_cast<int64_t>(j * threads + t) * n, a.dim);
+      for (int j = 0; j < kNV; ++j)
+        if (skip[j] < n) d_next[j] = *reinterpret_cast<const Pack<T>*>(dsp + at[j]);
     }
   };
   int64_t row = kWaveRow ? static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kWave : blockIdx.x;
@@ -400,9 +412,9 @@ __global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024, 4) rms_norm_bwd_k
     for (int j = 0; j < kNV; ++j) {
 #pragma unroll
       for (int i = 0; i < n; ++i) {
-        const float v = to_f(s[j].v[i]);
+        const float v = i < skip[j] ? 0.f : to_f(s[j].v[i]);
         ss += v * v;
-        dot += to_f(g[j].v[i]) * weight(j, i) * v;
+        dot += i < skip[j] ? 0.f : to_f(g[j].v[i]) * weight(j, i) * v;
       }
     }
 #pragma unroll
@@ -442,7 +454,7 @@ __global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024, 4) rms_norm_bwd_k
         acc[j][i] += gy * xh;
         o[i] = rstd * (gy * weight(j, i) - xh * c) + (a.ds != nullptr ? to_f(d[j].v[i]) : 0.f);
       }
-      if (a.dx != nullptr) store_vec<T>(dxp, static_cast<int64_t>(j * threads + t) * n, a.dim, o);
+      if (a.dx != nullptr && skip[j] < n) store_vec<T>(dxp, at[j], a.dim, o);
     }
   }
   if (a.part == nullptr) return;
@@ -456,22 +468,22 @@ __global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024, 4) rms_norm_bwd_k
         for (int j = 0; j < kNV; ++j)
 #pragma unroll
           for (int i = 0; i < n; ++i) {
-            float* at = lds + (j * n + i) * kWave + t;
-            *at = (wave == 0 ? 0.f : *at) + acc[j][i];
+            float* to = lds + (j * n + i) * kWave + t;
+            *to = (wave == 0 ? 0.f : *to) + acc[j][i];
           }
       }
       __syncthreads();
     }
     for (int e = threadIdx.x; e < kWave * kNV * n; e += kRowBlock) {
-      if (e < a.dim) part[e] = lds[(e / n / kWave * n + e % n) * kWave + e / n % kWave];
+      const int place = e / n, over = static_cast<int>((place + 1) * n - a.dim);       // > 0 for the row's last vector
+      if (e < a.dim) part[e] = lds[(place / kWave * n + e % n + (over > 0 ? over : 0)) * kWave + place % kWave];
     }
   } else {
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
-      const int64_t at = static_cast<int64_t>(j * threads + t) * n;
 #pragma unroll
       for (int i = 0; i < n; ++i)
-        if (at + i < a.dim) part[at + i] = acc[j][i];
+        if (i >= skip[j]) part[at[j] + i] = acc[j][i];
     }
   }
 }
@@ -642,7 +654,9 @@ int norm_by_type(const NormArgs& a, int dtype, hipStream_t stream, const char* w
 // a thread 102, their registers spill), two where a block is too short; rows of over 2048 vectors go through the
 // long kernel.  As many blocks as run at once (20 waves a CU in 16 bits, 32 in fp32), so that none is left over.
 inline RowShape bwd_shape(int64_t dim, int dtype) {
-  const int64_t v = cdiv(dim, dtype == SAGE_F32 ? 4 : 8);
+  const int n = dtype == SAGE_F32 ? 4 : 8;
+  const int64_t v = cdiv(dim, n);
+  if (dim < n) return {1024, 0, false};
   if (v <= 64) return {kWave, 1, true};
   if (v <= 1024) return block_row(v, 1);
   if (v <= 2048) return block_row(v, 2);
