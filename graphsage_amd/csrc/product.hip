@@ -749,6 +749,43 @@ __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_kernel(Product p) {
   }
 }
 
+// Up to 16 rows against a pair of Bs: a block owns 8 columns of each, whose rows are the 16 slots of one MFMA operand
+// (0 to 7 the first B's, 8 to 15 the second's), so that there are twice as many blocks to share out over the CUs.
+template <typename T, int U>
+__global__ void __launch_bounds__(kFewWaves* kWave) few_rows_pair_kernel(Product p) {
+  using Acc = typename Mma<T>::Acc;
+  __shared__ Acc lds[kFewWaves][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int l15 = lane & 15, q = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 8;
+  const int64_t col = n0 + (l15 & 7) < p.n ? n0 + (l15 & 7) : p.n - 1, row = l15 < p.m ? l15 : p.m - 1;
+  const char* b = (l15 < 8 ? p.b0 + col * p.ldb0 : p.b1 + col * p.ldb1) + q * 16;
+  const char* a = p.a + row * p.lda + q * 16;
+  const i32x4 none = {0, 0, 0, 0};
+  Acc acc = Acc{};
+  for (int64_t k = wave * (U * 64); k < p.kbytes; k += kFewWaves * U * 64) {
+    i32x4 bv[U], av[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) bv[u] = k + u * 64 + q * 16 < p.kbytes ? *reinterpret_cast<const i32x4*>(b + k + u * 64) : none;
+#pragma unroll
+    for (int u = 0; u < U; ++u) av[u] = k + u * 64 + q * 16 < p.kbytes ? *reinterpret_cast<const i32x4*>(a + k + u * 64) : none;
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc = Mma<T>::mma(bv[u], av[u], acc);
+  }
+  lds[wave][lane] = acc;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;      // lane: row l15, slots 4 q + 0..3 of the first B; 32 lanes on the second's
+  Acc g = lds[0][lane], u = lds[0][lane + 32];
+#pragma unroll
+  for (int w = 1; w < kFewWaves; ++w) {
+    g += lds[w][lane];
+    u += lds[w][lane + 32];
+  }
+  using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
+  const E c[4] = {g[0], g[1], g[2], g[3]}, d[4] = {u[0], u[1], u[2], u[3]};
+  finish_gated<T, 4>(p, l15, n0 + q * 4, c, d);
+}
+
 // ------------------------------------------------------------------------------- launch
 inline bool rows16(const void* p, int64_t ld_bytes) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld_bytes & 15) == 0 && ld_bytes >= 0;
@@ -844,6 +881,17 @@ int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, con
   // rows 10.9 -> 10.3 us, bf16 pair of 5632 x 2048 against 20 rows 19.1 -> 16.9; more or fewer pieces a turn and 32
   // columns for other row counts measured the same or slower)
   const dim3 half(static_cast<unsigned>(cdiv(p.n, 32)), 1), threads(kFewWaves * kWave);
+  if constexpr (kGated) {
+    // 8 columns a block where the busiest CU then gets fewer of them (bf16, 4 rows: 5632 x 2048 14.6 -> 12.9 us, 1024 x 1024
+    // 5.0 -> 4.3, 1000 x 4000 9.7 -> 7.0; 8192 x 2048, where it does not, 16.4 -> 16.7)
+    if (p.m <= 16 && cdiv(cdiv(p.n, 8), 256) < 2 * cdiv(cdiv(p.n, 16), 256)) {
+      const dim3 eight(static_cast<unsigned>(cdiv(p.n, 8)));
+      if (p.kbytes >= kFewWaves * 512) hipLaunchKernelGGL((few_rows_pair_kernel<T, 8>), eight, threads, 0, stream, p);
+      else hipLaunchKernelGGL((few_rows_pair_kernel<T, 4>), eight, threads, 0, stream, p);
+      SAGE_CHECK_LAUNCH(what);
+      return SAGE_OK;
+    }
+  }
   if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated, 1>), grid, threads, 0, stream, p);
   else if (p.m <= 32 && p.n >= 4096) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 2>), half, threads, 0, stream, p);
   else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 1>), grid, threads, 0, stream, p);

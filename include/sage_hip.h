@@ -781,7 +781,7 @@ int sage_dequantize_rows(const int8_t* q, sage_i64 ld_q, const float* scale, sag
 /* Backward of sage_rms_norm_fwd from the stored sum: xh = sum * rstd, c = mean(dy * weight * xh),
  * dx = rstd * (dy * weight - xh * c) + dsum (the gradient of x and of the residual alike),
  * dweight = sum over rows of dy * xh (fixed order, fp32 sums; in the weight's type).
- * dsum, and one of dx and dweight, may be NULL. */
+ * dsum, and one of dx and dweight, may be NULL; dx shares no memory with an input. */
 size_t sage_rms_norm_bwd_workspace_bytes(sage_i64 rows, sage_i64 dim, int dtype);
 int sage_rms_norm_bwd(const void* dy, sage_i64 ld_dy, const void* sum, sage_i64 ld_sum, const void* weight,
                       int weight_dtype, const void* dsum, sage_i64 ld_dsum, sage_i64 rows, sage_i64 dim, int dtype,
