@@ -672,7 +672,40 @@ __global__ void __launch_bounds__(256) join_kernel(Product p, int tiles_m, int t
 // each B); its waves take k in runs of 256 bytes in turn and add their sums in LDS, in wave order.
 constexpr int kFewWaves = 8;
 
-template <typename T, int MT, bool kGated, int NT>
+// 16 bytes of a row of T at `at`, zeros behind its end.  kRagged: rows of any length and alignment (at least 16 bytes).
+// In a wave's last turn a row's last piece is its last 16 bytes moved down.  Rows that start inside a 4-byte word are read
+// as the words that hold them (at most the 3 bytes before and behind them that share a word with theirs), shifted into
+// place: bf16, 4 rows against a pair of 5632 x 2047 23 us, 40 as loads that cross words, 32 through padded copies.
+template <typename T, bool kRagged>
+__device__ inline i32x4 load_piece(const char* row, int64_t at, int64_t kbytes, bool last) {
+  const i32x4 none = {0, 0, 0, 0};
+  if constexpr (!kRagged) return at < kbytes ? *reinterpret_cast<const i32x4*>(row + at) : none;
+  struct __attribute__((packed, aligned(4))) Words {
+    i32x4 v;
+  };
+  const int64_t from = at + 16 <= kbytes ? at : kbytes - 16;
+  i32x4 v;
+  if constexpr (sizeof(T) == 4) {
+    v = reinterpret_cast<const Words*>(row + from)->v;
+  } else {
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row + from) & 3);
+    const char* word = row + from - off;
+    const i32x4 lo = reinterpret_cast<const Words*>(word)->v;
+    const uint32_t next = *reinterpret_cast<const uint32_t*>(word + (off ? 16 : 12));   // no word behind a row that ends with one
+    const uint32_t w[5] = {static_cast<uint32_t>(lo[0]), static_cast<uint32_t>(lo[1]), static_cast<uint32_t>(lo[2]), static_cast<uint32_t>(lo[3]), next};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = static_cast<int>(__builtin_amdgcn_alignbyte(w[i + 1], w[i], off));
+  }
+  if (last) {
+    unsigned __int128 bits = __builtin_bit_cast(unsigned __int128, v);
+    const int64_t over = at - from;
+    bits = over < 16 ? bits >> (over * 8) : 0;
+    v = __builtin_bit_cast(i32x4, bits);
+  }
+  return v;
+}
+
+template <typename T, int MT, bool kGated, int NT, bool kRagged>
 __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_kernel(Product p) {
   using Acc = typename Mma<T>::Acc;
   constexpr int NB = kGated ? 2 : 1, NC = NB * NT, U = 4;
@@ -684,36 +717,32 @@ __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_kernel(Product p) {
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int64_t col = n0 + t * 16 + l15 < p.n ? n0 + t * 16 + l15 : p.n - 1;
-    b[t * NB] = p.b0 + col * p.ldb0 + q * 16;
-    if constexpr (kGated) b[t * NB + 1] = p.b1 + col * p.ldb1 + q * 16;
+    b[t * NB] = p.b0 + col * p.ldb0;
+    if constexpr (kGated) b[t * NB + 1] = p.b1 + col * p.ldb1;
   }
   const char* a[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int64_t row = m0 + i * 16 + l15 < p.m ? m0 + i * 16 + l15 : p.m - 1;
-    a[i] = p.a + row * p.lda + q * 16;
+    a[i] = p.a + row * p.lda;
   }
   Acc acc[MT][NC];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NC; ++j) acc[i][j] = Acc{};
-  const i32x4 none = {0, 0, 0, 0};
   // U pieces of 64 bytes a turn: contiguous bytes of a row, all loads before the first product
   for (int64_t k = wave * (U * 64); k < p.kbytes; k += kFewWaves * U * 64) {
+    const bool last = k + U * 64 > p.kbytes;
     i32x4 bv[U][NC], av[U][MT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = k + u * 64 + q * 16 < p.kbytes;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < NC; ++j) bv[u][j] = in ? *reinterpret_cast<const i32x4*>(b[j] + k + u * 64) : none;
-    }
+      for (int j = 0; j < NC; ++j) bv[u][j] = load_piece<T, kRagged>(b[j], k + u * 64 + q * 16, p.kbytes, last);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = k + u * 64 + q * 16 < p.kbytes;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) av[u][i] = in ? *reinterpret_cast<const i32x4*>(a[i] + k + u * 64) : none;
-    }
+      for (int i = 0; i < MT; ++i) av[u][i] = load_piece<T, kRagged>(a[i], k + u * 64 + q * 16, p.kbytes, last);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -751,7 +780,7 @@ __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_kernel(Product p) {
 
 // Up to 16 rows against a pair of Bs: a block owns 8 columns of each, whose rows are the 16 slots of one MFMA operand
 // (0 to 7 the first B's, 8 to 15 the second's), so that there are twice as many blocks to share out over the CUs.
-template <typename T, int U>
+template <typename T, int U, bool kRagged>
 __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_pair_kernel(Product p) {
   using Acc = typename Mma<T>::Acc;
   __shared__ Acc lds[kFewWaves][kWave];
@@ -759,16 +788,16 @@ __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_pair_kernel(Product
   const int l15 = lane & 15, q = lane >> 4;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 8;
   const int64_t col = n0 + (l15 & 7) < p.n ? n0 + (l15 & 7) : p.n - 1, row = l15 < p.m ? l15 : p.m - 1;
-  const char* b = (l15 < 8 ? p.b0 + col * p.ldb0 : p.b1 + col * p.ldb1) + q * 16;
-  const char* a = p.a + row * p.lda + q * 16;
-  const i32x4 none = {0, 0, 0, 0};
+  const char* b = l15 < 8 ? p.b0 + col * p.ldb0 : p.b1 + col * p.ldb1;
+  const char* a = p.a + row * p.lda;
   Acc acc = Acc{};
   for (int64_t k = wave * (U * 64); k < p.kbytes; k += kFewWaves * U * 64) {
+    const bool last = k + U * 64 > p.kbytes;
     i32x4 bv[U], av[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) bv[u] = k + u * 64 + q * 16 < p.kbytes ? *reinterpret_cast<const i32x4*>(b + k + u * 64) : none;
+    for (int u = 0; u < U; ++u) bv[u] = load_piece<T, kRagged>(b, k + u * 64 + q * 16, p.kbytes, last);
 #pragma unroll
-    for (int u = 0; u < U; ++u) av[u] = k + u * 64 + q * 16 < p.kbytes ? *reinterpret_cast<const i32x4*>(a + k + u * 64) : none;
+    for (int u = 0; u < U; ++u) av[u] = load_piece<T, kRagged>(a, k + u * 64 + q * 16, p.kbytes, last);
 #pragma unroll
     for (int u = 0; u < U; ++u) acc = Mma<T>::mma(bv[u], av[u], acc);
   }
@@ -868,6 +897,29 @@ int launch_planned(Product p, const Plan& plan, void* ws, size_t ws_bytes, hipSt
   return SAGE_OK;
 }
 
+template <typename T, bool kGated, bool kRagged>
+void launch_few_rows(const Product& p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), static_cast<unsigned>(cdiv(p.m, 64))), threads(kFewWaves * kWave);   // m <= 512
+  if constexpr (kGated) {
+    // 8 columns a block where the busiest CU then gets fewer of them (bf16, 4 rows: 5632 x 2048 14.6 -> 12.8 us, 1024 x 1024
+    // 5.0 -> 4.2, 1000 x 4000 9.7 -> 7.0; 8192 x 2048, where it does not, 16.4 -> 16.7)
+    if (p.m <= 16 && cdiv(cdiv(p.n, 8), 256) < 2 * cdiv(cdiv(p.n, 16), 256)) {
+      const dim3 eight(static_cast<unsigned>(cdiv(p.n, 8)));
+      if (p.kbytes >= kFewWaves * 512) hipLaunchKernelGGL((few_rows_pair_kernel<T, 8, kRagged>), eight, threads, 0, stream, p);
+      else hipLaunchKernelGGL((few_rows_pair_kernel<T, 4, kRagged>), eight, threads, 0, stream, p);
+      return;
+    }
+  }
+  // 32 columns a block where 17 to 32 rows would otherwise be read for every 16 (8-bit pair of 8192 x 2048 against 24
+  // rows 10.9 -> 10.3 us, bf16 pair of 5632 x 2048 against 20 rows 19.1 -> 16.9; more or fewer pieces a turn and 32
+  // columns for other row counts measured the same or slower)
+  if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated, 1, kRagged>), grid, threads, 0, stream, p);
+  else if (p.m <= 32 && p.n >= 4096)
+    hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 2, kRagged>), dim3(static_cast<unsigned>(cdiv(p.n, 32))), threads, 0, stream, p);
+  else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 1, kRagged>), grid, threads, 0, stream, p);
+  else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated, 1, kRagged>), grid, threads, 0, stream, p);
+}
+
 // rows of both operands along k
 template <typename T, bool kGated>
 int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, const char* what) {
@@ -876,26 +928,9 @@ int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, con
   p.part_runs = p.runs;
   p.whole_runs = p.kbytes / 64;
   if (plan.tile != 0) return launch_planned<T, kGated, false, false>(p, plan, ws, ws_bytes, stream, what);
-  const dim3 grid(static_cast<unsigned>(cdiv(p.n, 16)), static_cast<unsigned>(cdiv(p.m, 64)));   // m <= 512
-  // 32 columns a block where 17 to 32 rows would otherwise be read for every 16 (8-bit pair of 8192 x 2048 against 24
-  // rows 10.9 -> 10.3 us, bf16 pair of 5632 x 2048 against 20 rows 19.1 -> 16.9; more or fewer pieces a turn and 32
-  // columns for other row counts measured the same or slower)
-  const dim3 half(static_cast<unsigned>(cdiv(p.n, 32)), 1), threads(kFewWaves * kWave);
-  if constexpr (kGated) {
-    // 8 columns a block where the busiest CU then gets fewer of them (bf16, 4 rows: 5632 x 2048 14.6 -> 12.9 us, 1024 x 1024
-    // 5.0 -> 4.3, 1000 x 4000 9.7 -> 7.0; 8192 x 2048, where it does not, 16.4 -> 16.7)
-    if (p.m <= 16 && cdiv(cdiv(p.n, 8), 256) < 2 * cdiv(cdiv(p.n, 16), 256)) {
-      const dim3 eight(static_cast<unsigned>(cdiv(p.n, 8)));
-      if (p.kbytes >= kFewWaves * 512) hipLaunchKernelGGL((few_rows_pair_kernel<T, 8>), eight, threads, 0, stream, p);
-      else hipLaunchKernelGGL((few_rows_pair_kernel<T, 4>), eight, threads, 0, stream, p);
-      SAGE_CHECK_LAUNCH(what);
-      return SAGE_OK;
-    }
-  }
-  if (p.m <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1, kGated, 1>), grid, threads, 0, stream, p);
-  else if (p.m <= 32 && p.n >= 4096) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 2>), half, threads, 0, stream, p);
-  else if (p.m <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2, kGated, 1>), grid, threads, 0, stream, p);
-  else hipLaunchKernelGGL((few_rows_kernel<T, 4, kGated, 1>), grid, threads, 0, stream, p);
+  const bool whole = p.kbytes % 16 == 0 && rows16(p.a, p.lda) && rows16(p.b0, p.ldb0) && rows16(p.b1, p.ldb1);
+  if (whole) launch_few_rows<T, kGated, false>(p, stream);
+  else launch_few_rows<T, kGated, true>(p, stream);
   SAGE_CHECK_LAUNCH(what);
   return SAGE_OK;
 }
@@ -1050,6 +1085,10 @@ extern "C" int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows
   return SAGE_OK;
 }
 
+extern "C" int sage_product_any_rows(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32) {
+  return m > 0 && n > 0 && row_bytes >= 16 && plan_product(m, n, row_bytes, gated != 0, fp32 != 0, true).tile == 0;
+}
+
 extern "C" size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32) {
   if (m <= 0 || n <= 0 || row_bytes <= 0) return 0;
   return plan_product(m, n, row_bytes, gated != 0, fp32 != 0, true).workspace;
@@ -1066,8 +1105,8 @@ extern "C" int sage_int8_linear(const int8_t* x, sage_i64 ld_x, const float* x_s
   SAGE_INT8_CHECKS("sage_int8_linear");
   if (m == 0) return SAGE_OK;
   SAGE_REQUIRE(x && x_scale && w && w_scale && out, SAGE_EINVAL, "sage_int8_linear: NULL pointer");
-  SAGE_REQUIRE(k % 16 == 0 && rows16(x, ld_x) && rows16(w, ld_w) && ld_out >= n, SAGE_EINVAL,
-               "sage_int8_linear: rows are whole pieces of 16 bytes (sage_pad_rows) and outputs do not overlap");
+  SAGE_REQUIRE(((k % 16 == 0 && rows16(x, ld_x) && rows16(w, ld_w)) || sage_product_any_rows(m, n, k, 0, 0)) && ld_x >= 0 &&
+                   ld_w >= 0 && ld_out >= n, SAGE_EINVAL, "sage_int8_linear: rows are whole pieces of 16 bytes (sage_pad_rows) and outputs do not overlap");
   Product p{};
   p.a = reinterpret_cast<const char*>(x); p.lda = ld_x;
   p.b0 = reinterpret_cast<const char*>(w); p.ldb0 = ld_w;
@@ -1085,8 +1124,8 @@ extern "C" int sage_int8_gated_linear(const int8_t* x, sage_i64 ld_x, const floa
   SAGE_REQUIRE(known_act(activation), SAGE_EINVAL, "sage_int8_gated_linear: unknown activation %d", activation);
   if (m == 0) return SAGE_OK;
   SAGE_REQUIRE(x && x_scale && w_gate && gate_scale && w_up && up_scale && out, SAGE_EINVAL, "sage_int8_gated_linear: NULL pointer");
-  SAGE_REQUIRE(k % 16 == 0 && rows16(x, ld_x) && rows16(w_gate, ld_g) && rows16(w_up, ld_u) && ld_out >= n, SAGE_EINVAL,
-               "sage_int8_gated_linear: rows are whole pieces of 16 bytes (sage_pad_rows) and outputs do not overlap");
+  SAGE_REQUIRE(((k % 16 == 0 && rows16(x, ld_x) && rows16(w_gate, ld_g) && rows16(w_up, ld_u)) || sage_product_any_rows(m, n, k, 1, 0)) &&
+                   ld_x >= 0 && ld_g >= 0 && ld_u >= 0 && ld_out >= n, SAGE_EINVAL, "sage_int8_gated_linear: rows are whole pieces of 16 bytes (sage_pad_rows) and outputs do not overlap");
   Product p{};
   p.a = reinterpret_cast<const char*>(x); p.lda = ld_x;
   p.b0 = reinterpret_cast<const char*>(w_gate); p.ldb0 = ld_g;
@@ -1106,7 +1145,8 @@ extern "C" int sage_gated_linear_fwd(const void* x, sage_i64 ld_x, const void* w
   if (m == 0) return SAGE_OK;
   SAGE_REQUIRE(x && w_gate && w_up && out, SAGE_EINVAL, "sage_gated_linear_fwd: NULL pointer");
   const int size = size_of(dtype);
-  SAGE_REQUIRE(k * size % 16 == 0 && rows16(x, ld_x * size) && rows16(w_gate, ld_g * size) && rows16(w_up, ld_u * size) && ld_out >= h,
+  SAGE_REQUIRE(((k * size % 16 == 0 && rows16(x, ld_x * size) && rows16(w_gate, ld_g * size) && rows16(w_up, ld_u * size)) ||
+                sage_product_any_rows(m, h, k * size, 1, dtype == SAGE_F32)) && ld_x >= 0 && ld_g >= 0 && ld_u >= 0 && ld_out >= h,
                SAGE_EINVAL, "sage_gated_linear_fwd: rows are whole pieces of 16 bytes (sage_pad_rows) and outputs do not overlap");
   Product p{};
   p.a = static_cast<const char*>(x); p.lda = ld_x * size;

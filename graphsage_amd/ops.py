@@ -1527,6 +1527,19 @@ def _pieces(t, p, ld, copy=False):
     return out.data_ptr(), wide, wide, out
 
 
+def _product_rows(m, n, k, size, fp32, *mats):
+    """The operands (tensor, pointer, row stride) of a product of rows of k elements as its kernel takes them:
+    (k, [(pointer, row stride)], what must stay alive).  A product with few rows takes any rows."""
+    bits, far = k * size, False
+    for _, p, ld in mats:
+        bits |= p | ld * size
+        far |= ld * size >= 1 << 23
+    if not far and (bits & 15 == 0 or m <= 512 and _lib.load().sage_product_any_rows(m, n, k * size, len(mats) - 2, fp32)):
+        return k, [(p, ld) for _, p, ld in mats], None
+    done = [_pieces(*mat) for mat in mats]
+    return done[0][2], [d[:2] for d in done], done
+
+
 def _product_workspace(m, n, row_bytes, gated, fp32, device):
     """(pointer, bytes, owner) of what a product of few tiles splits k into; the fewest rows take none."""
     size = _lib.load().sage_product_workspace_bytes(m, n, row_bytes, gated, fp32) if m > 16 else 0
@@ -1572,8 +1585,7 @@ def _int8_weight(w, scale, k, device):
     n, wk = w.shape
     if wk != k or n == 0:
         raise RuntimeError(f"8-bit product: weight of shape {[n, wk]} for rows of {k} elements")
-    ps = _vector(scale, "8-bit product: weight scale", n, device)
-    return (*_pieces(w, pw, ldw), ps, n)
+    return pw, ldw, _vector(scale, "8-bit product: weight scale", n, device), n
 
 
 def _int8_rows_in(x, x_scale, out_dtype):
@@ -1591,11 +1603,11 @@ def int8_linear(x, x_scale, weight, w_scale, bias=None, out_dtype=torch.float32,
     """out[m, n] = x_scale[m] * w_scale[n] * (x @ weight^T)[m, n] + bias[n] for int8 x [m, k] and weight
     [n, k] (k <= 131056: the integer sum is exact), fp32 scales and bias."""
     px, ldx, psx, m, k, dev = _int8_rows_in(x, x_scale, out_dtype)
-    pw, ldw, _, keep_w, psw, n = _int8_weight(weight, w_scale, k, dev)
+    pw, ldw, psw, n = _int8_weight(weight, w_scale, k, dev)
     pb = None if bias is None else _vector(bias, "int8_linear: bias", n, dev)
     out, po, ldo = _product_output(out, "int8_linear: out", (m, n), out_dtype, dev, (x, x_scale, weight, w_scale, bias))
     if m > 0:
-        px, ldx, wide, keep_x = _pieces(x, px, ldx)
+        wide, ((px, ldx), (pw, ldw)), kept = _product_rows(m, n, k, 1, 0, (x, px, ldx), (weight, pw, ldw))
         ws, ws_bytes, keep = _product_workspace(m, n, wide, 0, 0, dev)
         _call("sage_int8_linear", dev, px, ldx, psx, pw, ldw, psw, pb, m, n, wide, ROW_DTYPES[out_dtype], po, ldo,
               ws, ws_bytes)
@@ -1607,14 +1619,14 @@ def int8_gated_linear(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation
     act = _activation(activation)
     act = _activation(activation)
     px, ldx, psx, m, k, dev = _int8_rows_in(x, x_scale, out_dtype)
-    pg, ldg, _, keep_g, psg, n = _int8_weight(w_gate, gate_scale, k, dev)
-    pu, ldu, _, keep_u, psu, nu = _int8_weight(w_up, up_scale, k, dev)
+    pg, ldg, psg, n = _int8_weight(w_gate, gate_scale, k, dev)
+    pu, ldu, psu, nu = _int8_weight(w_up, up_scale, k, dev)
     if n != nu:
         raise RuntimeError(f"int8_gated_linear: weights of {n} and {nu} rows")
     out, po, ldo = _product_output(out, "int8_gated_linear: out", (m, n), out_dtype, dev,
                                    (x, x_scale, w_gate, gate_scale, w_up, up_scale))
     if m > 0:
-        px, ldx, wide, keep_x = _pieces(x, px, ldx)
+        wide, ((px, ldx), (pg, ldg), (pu, ldu)), kept = _product_rows(m, n, k, 1, 0, (x, px, ldx), (w_gate, pg, ldg), (w_up, pu, ldu))
         ws, ws_bytes, keep = _product_workspace(m, n, wide, 1, 0, dev)
         _call("sage_int8_gated_linear", dev, px, ldx, psx, pg, ldg, psg, pu, ldu, psu, act, m, n, wide,
               ROW_DTYPES[out_dtype], po, ldo, ws, ws_bytes)
@@ -1642,10 +1654,9 @@ def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
     saved = torch.empty((2, m, h), dtype=torch.float32, device=dev) if save else None
     if m == 0:
         return out, saved
-    px, ldx, wide, keep_x = _pieces(x, px, ldx)
-    pg, ldg, _, keep_g = _pieces(w_gate, pg, ldg)
-    pu, ldu, _, keep_u = _pieces(w_up, pu, ldu)
-    ws, ws_bytes, keep = _product_workspace(m, h, wide * x.element_size(), 1, x.dtype is torch.float32, dev)
+    size, fp32 = x.element_size(), x.dtype is torch.float32
+    wide, ((px, ldx), (pg, ldg), (pu, ldu)), kept = _product_rows(m, h, k, size, fp32, (x, px, ldx), (w_gate, pg, ldg), (w_up, pu, ldu))
+    ws, ws_bytes, keep = _product_workspace(m, h, wide * size, 1, fp32, dev)
     _call("sage_gated_linear_fwd", dev, px, ldx, pg, ldg, pu, ldu, act, m, h, wide, ROW_DTYPES[x.dtype], po, ldo,
           saved.data_ptr() if save else None, ws, ws_bytes)
     return out, saved

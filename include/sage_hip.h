@@ -789,9 +789,13 @@ int sage_rms_norm_bwd(const void* dy, sage_i64 ld_dy, const void* sum, sage_i64 
                       void* stream);
 
 /* Rows of row_bytes bytes into rows that start on 16 bytes and end, zero-filled, on 16 bytes:
- * what the products below take (both operands' rows, and k, in whole pieces of 16 bytes). */
+ * what the products below take (both operands' rows, and k, in whole pieces of 16 bytes) where
+ * sage_product_any_rows does not say that they take any. */
 int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows, sage_i64 row_bytes, void* out,
                   sage_i64 ld_out_bytes, void* stream);
+/* 1 where a product below (row_bytes >= 16) takes rows of any alignment and length as they are: those
+ * with few rows, whose weights a padded copy would cost more than the product. */
+int sage_product_any_rows(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32);
 /* Workspace of a product below (starts on 16 bytes; 0 bytes: none, NULL): where an output has too few
  * tiles to fill the chip, k is split and the slices' sums meet there.  row_bytes is k times the
  * element's size; gated: two weights; fp32: fp32 operands.  The operands' rows are less than 2^23 bytes

@@ -77,10 +77,10 @@ def test_product_refusals():
                          (ELIMIT, dict(ldx=1 << 23)), (EWORKSPACE, dict(wn=size - 1)), (EWORKSPACE, dict(wk=ODD))):
         refused(code, "sage_int8_linear", *{**ok, **change}.values())
     ok = dict(x=P, ldx=64, xs=P, g=P, ldg=64, gs=P, u=P, ldu=64, us=P, act=0, m=2, n=8, k=64, dt=0, out=P, ldo=8, wk=None, wn=0, st=None)
-    for code, change in ((EINVAL, dict(u=None)), (EINVAL, dict(us=None)), (EINVAL, dict(act=3)), (EINVAL, dict(ldu=24)), (EINVAL, dict(k=24)), (ELIMIT, dict(k=131072))):
+    for code, change in ((EINVAL, dict(u=None)), (EINVAL, dict(us=None)), (EINVAL, dict(act=3)), (EINVAL, dict(ldu=24, m=600)), (EINVAL, dict(k=24, m=600)), (EINVAL, dict(k=15)), (ELIMIT, dict(k=131072))):
         refused(code, "sage_int8_gated_linear", *{**ok, **change}.values())
     ok = dict(x=P, ldx=16, g=P, ldg=16, u=P, ldu=16, act=1, m=2, h=8, k=16, dt=1, out=P, ldo=8, saved=None, wk=None, wn=0, st=None)
-    for change in (dict(x=None), dict(g=ODD), dict(act=-1), dict(dt=5), dict(k=12), dict(ldx=12), dict(ldo=4), dict(h=0)):
+    for change in (dict(x=None), dict(g=ODD, m=600), dict(act=-1), dict(dt=5), dict(k=12, m=600), dict(k=7), dict(ldx=20, m=600), dict(ldo=4), dict(h=0)):
         refused(EINVAL, "sage_gated_linear_fwd", *{**ok, **change}.values())
     size = lib.sage_gated_linear_bwd_workspace_bytes(20, 8, 16, 1)
     ok = dict(dh=P, ldh=8, x=P, ldx=16, g=P, ldg=16, u=P, ldu=16, saved=P, act=0, m=20, h=8, k=16, dt=1, dx=P, lddx=16, dw=P, ws=P, n=size, st=None)

@@ -328,6 +328,33 @@ def test_products_take_any_rows(dev, dtype):
             assert bool((hold == 5.0).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES + [torch.int8])
+@pytest.mark.parametrize("m,n,k", [(1, 9, 17), (4, 4100, 37), (16, 700, 1999), (20, 4099, 1023), (24, 50, 4111), (40, 33, 517), (200, 300, 65)])
+def test_few_rows_of_odd_lengths(dev, dtype, m, n, k):
+    """Rows of any length and start, with NaN (8 bits: 127) around them, give what whole pieces give."""
+    rng = gen(dev, m + n + k)
+    one = 127 if dtype == torch.int8 else float("nan")
+
+    def inside(rows):
+        hold = torch.full((rows + 2, k + 6), one, dtype=dtype, device=dev)
+        hold[1:-1, 3:-3] = normal(rng, rows, k, scale=40.0 if dtype == torch.int8 else 1.0).clamp(-127, 127).to(dtype)
+        view = hold[1:-1, 3:-3]
+        return view, torch.nn.functional.pad(view, (0, 16 - k % 16))
+
+    (x, x16), (wg, wg16), (wu, wu16) = inside(m), inside(n), inside(n)
+    if dtype == torch.int8:
+        s, t = torch.rand(m, generator=rng, device=dev) * 1e-2, torch.rand(n, generator=rng, device=dev) * 1e-2
+        assert torch.equal(ops.int8_linear(x, s, wg, t), ops.int8_linear(x16, s, wg16, t))
+        assert torch.equal(ops.int8_gated_linear(x, s, wg, t, wu, t), ops.int8_gated_linear(x16, s, wg16, t, wu16, t))
+        return
+    got, saved = ops.gated_linear_fwd(x, wg, wu, save=True)
+    g, u, dg, du = gated_ref(x, wg, wu, "silu")
+    within(saved[0], g, dg + g.abs() * E, "gate")
+    within(saved[1], u, du + u.abs() * E, "up")
+    want = act64(g, "silu") * u
+    within(got, want, gated_bound(g, u, dg, du, "silu") * (1 + 2 ** -7) + want.abs() * U[dtype] + TINY[dtype], "out")
+
+
 def test_not_a_number_stays_in_its_row(dev):
     """A NaN in a row of x reaches that row's outputs and no others, also through rows that fill a tile."""
     for m in (3, 70, 300):
