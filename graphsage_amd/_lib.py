@@ -5,6 +5,7 @@ RuntimeError is raised (the convention of the natives the reference binds throug
 torch.ops, e.g. samplers/uniform_loader.py:64).
 """
 import ctypes
+import gc
 import os
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
@@ -209,6 +210,10 @@ def load():
         fn = getattr(lib, name)  # AttributeError -> a symbol the header declares is missing
         fn.restype = restype
         fn.argtypes = argtypes
+    # What this process leaves in reference cycles (an engine and the calls it recorded hold each other) is not
+    # collected by a forked child: destroying its events, streams and graphs there calls into a HIP runtime that
+    # the child does not have, and ends it.
+    os.register_at_fork(after_in_child=gc.freeze)
     _lib = lib
     return _Recorder(_lib) if _tape is not None else _lib
 

@@ -1617,7 +1617,6 @@ def int8_linear(x, x_scale, weight, w_scale, bias=None, out_dtype=torch.float32,
 def int8_gated_linear(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation="silu", out_dtype=torch.float32, out=None):
     """activation(x @ w_gate^T) * (x @ w_up^T), both 8-bit products with token and channel scales."""
     act = _activation(activation)
-    act = _activation(activation)
     px, ldx, psx, m, k, dev = _int8_rows_in(x, x_scale, out_dtype)
     pg, ldg, psg, n = _int8_weight(w_gate, gate_scale, k, dev)
     pu, ldu, psu, nu = _int8_weight(w_up, up_scale, k, dev)
