@@ -30,6 +30,15 @@ __device__ inline float wave_max(float v) {
   return v;
 }
 
+// sum + <a, b>, and (g - y dot) inv: the same fused steps wherever a row's sums are taken again, so that the passes from
+// y and from z give the same bits
+__device__ inline float add_dot(float sum, const float4& a, const float4& b) {
+  return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, sum))));
+}
+__device__ inline float4 project_out(const float4& g, const float4& y, float dot, float inv) {
+  return make_float4(fmaf(-y.x, dot, g.x) * inv, fmaf(-y.y, dot, g.y) * inv, fmaf(-y.z, dot, g.z) * inv, fmaf(-y.w, dot, g.w) * inv);
+}
+
 // V4: n and every row stride are multiples of 4 and the bases 16-byte aligned — each lane moves
 // 16-byte vectors (one per lane covers n = 256), twice the bytes per instruction of the scalar form
 template <bool V4>
@@ -47,7 +56,7 @@ l2norm_relu_fwd_kernel(float* __restrict__ z, int64_t ld_z, int64_t m,
   if constexpr (V4) {
     for (int f = lane * 4; f < n; f += kWave * 4) {
       const float4 v = *reinterpret_cast<const float4*>(zr + f);
-      ss += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+      ss = add_dot(ss, v, v);
     }
   } else {
     for (int f = lane; f < n; f += kWave) {
@@ -105,7 +114,7 @@ l2norm_relu_bwd_kernel(float* __restrict__ dh, int64_t ld_dh, const float* __res
         if (!(yv.z > 0.f)) g.z = 0.f;
         if (!(yv.w > 0.f)) g.w = 0.f;
       }
-      dot += yv.x * g.x + yv.y * g.y + yv.z * g.z + yv.w * g.w;
+      dot = add_dot(dot, yv, g);
     }
   } else {
     for (int f = lane; f < n; f += kWave) {
@@ -126,9 +135,7 @@ l2norm_relu_bwd_kernel(float* __restrict__ dh, int64_t ld_dh, const float* __res
         if (!(yv.z > 0.f)) g.z = 0.f;
         if (!(yv.w > 0.f)) g.w = 0.f;
       }
-      *reinterpret_cast<float4*>(dz + r * ld_dz + f) =
-          make_float4((g.x - yv.x * dot) * inv, (g.y - yv.y * dot) * inv, (g.z - yv.z * dot) * inv,
-                      (g.w - yv.w * dot) * inv);
+      *reinterpret_cast<float4*>(dz + r * ld_dz + f) = project_out(g, yv, dot, inv);
       // consume-and-clear: the next step's scatter-add starts from zeros without a fill kernel
       if (clear_dh) *reinterpret_cast<float4*>(gr + f) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -171,7 +178,7 @@ l2norm_relu_bwd_z_body(int64_t block, float* __restrict__ dh, int64_t ld_dh, flo
       zv[v] = zr[q];
       g[v] = gr[q];
     }
-    ss += zv[v].x * zv[v].x + zv[v].y * zv[v].y + zv[v].z * zv[v].z + zv[v].w * zv[v].w;
+    ss = add_dot(ss, zv[v], zv[v]);
   }
   ss = wave_sum(ss);
   const float denom = fmaxf(sqrtf(ss), kNormEps);
@@ -187,15 +194,14 @@ l2norm_relu_bwd_z_body(int64_t block, float* __restrict__ dh, int64_t ld_dh, flo
       if (!(zv[v].z > 0.f)) g[v].z = 0.f;
       if (!(zv[v].w > 0.f)) g[v].w = 0.f;
     }
-    dot += zv[v].x * g[v].x + zv[v].y * g[v].y + zv[v].z * g[v].z + zv[v].w * g[v].w;
+    dot = add_dot(dot, zv[v], g[v]);
   }
   dot = clamped ? 0.f : wave_sum(dot);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int q = lane + kWave * v;
     if (q < nq) {
-      or_[q] = make_float4((g[v].x - zv[v].x * dot) * inv, (g[v].y - zv[v].y * dot) * inv,
-                           (g[v].z - zv[v].z * dot) * inv, (g[v].w - zv[v].w * dot) * inv);
+      or_[q] = project_out(g[v], zv[v], dot, inv);
       zr[q] = zero4;
       if (clear_dh) gr[q] = zero4;
     }
