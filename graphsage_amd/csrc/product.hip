@@ -888,7 +888,7 @@ int launch_planned(Product p, const Plan& plan, void* ws, size_t ws_bytes, hipSt
   SAGE_REQUIRE(plan.workspace <= ws_bytes && (plan.workspace == 0 || rows16(ws, 0)), SAGE_EWORKSPACE,
                "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, plan.workspace);
   const int64_t tm = cdiv(p.m, plan.tile), tn = cdiv(p.n, kGated ? plan.tile / 2 : plan.tile);
-  SAGE_REQUIRE(tm * tn < (int64_t{1} << 24), SAGE_ELIMIT, "%s: %ld output tiles", what, (long)(tm * tn));
+  SAGE_REQUIRE(tm * tn < (int64_t{1} << 23), SAGE_ELIMIT, "%s: %ld output tiles", what, (long)(tm * tn));
   p.slice_runs = plan.slice_runs;
   p.partial = plan.slices > 1 ? static_cast<i32x4*>(ws) : nullptr;
   if (plan.tile == 256) launch_tiles<T, 256, kGated, kAT, kBT>(p, plan, tm, tn, stream);
@@ -928,6 +928,7 @@ int launch_product(Product p, void* ws, size_t ws_bytes, hipStream_t stream, con
   p.part_runs = p.runs;
   p.whole_runs = p.kbytes / 64;
   if (plan.tile != 0) return launch_planned<T, kGated, false, false>(p, plan, ws, ws_bytes, stream, what);
+  SAGE_REQUIRE(p.n < (int64_t{1} << 26), SAGE_ELIMIT, "%s: %ld columns", what, (long)p.n);
   const bool whole = p.kbytes % 16 == 0 && rows16(p.a, p.lda) && rows16(p.b0, p.ldb0) && rows16(p.b1, p.ldb1);
   if (whole) launch_few_rows<T, kGated, false>(p, stream);
   else launch_few_rows<T, kGated, true>(p, stream);
@@ -992,20 +993,20 @@ __global__ void __launch_bounds__(256) gate_bwd_kernel(const T* dh, int64_t ld_d
 
 __global__ void __launch_bounds__(256) pad_rows_kernel(const uint8_t* in, int64_t ld_in, int64_t row_bytes, uint8_t* out,
                                                        int64_t ld_out, int64_t pieces, int64_t total) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= total) return;
-  const int64_t row = i / pieces, at = (i - row * pieces) * 16;
-  const uint8_t* p = in + row * ld_in + at;
-  struct __attribute__((packed, aligned(1))) P {
-    uint8_t v[16];
-  } k;
-  if (at + 16 <= row_bytes) {
-    k = *reinterpret_cast<const P*>(p);
-  } else {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / pieces, at = (i - row * pieces) * 16;
+    const uint8_t* p = in + row * ld_in + at;
+    struct __attribute__((packed, aligned(1))) P {
+      uint8_t v[16];
+    } k;
+    if (at + 16 <= row_bytes) {
+      k = *reinterpret_cast<const P*>(p);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) k.v[e] = at + e < row_bytes ? p[e] : 0;
+      for (int e = 0; e < 16; ++e) k.v[e] = at + e < row_bytes ? p[e] : 0;
+    }
+    *reinterpret_cast<i32x4*>(out + row * ld_out + at) = __builtin_bit_cast(i32x4, k);
   }
-  *reinterpret_cast<i32x4*>(out + row * ld_out + at) = __builtin_bit_cast(i32x4, k);
 }
 
 // The backward pass's workspace: [m, 2 wide] of dg and du, and the room for slices, which its two products, one
@@ -1078,8 +1079,8 @@ extern "C" int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows
   SAGE_REQUIRE(rows16(out, ld_out_bytes) && ld_out_bytes >= row_bytes && ld_in_bytes >= 0, SAGE_EINVAL,
                "sage_pad_rows: output rows start on 16 bytes and hold the input's");
   const int64_t pieces = cdiv(row_bytes, 16), total = rows * pieces;
-  SAGE_REQUIRE(cdiv(total, 256) < (int64_t{1} << 31), SAGE_ELIMIT, "sage_pad_rows: %ld rows of %ld bytes", (long)rows, (long)row_bytes);
-  hipLaunchKernelGGL(pad_rows_kernel, dim3(static_cast<unsigned>(cdiv(total, 256))), dim3(256), 0, static_cast<hipStream_t>(stream),
+  const int64_t blocks = cdiv(total, 256) < (1 << 20) ? cdiv(total, 256) : 1 << 20;
+  hipLaunchKernelGGL(pad_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream),
                      static_cast<const uint8_t*>(in), ld_in_bytes, row_bytes, static_cast<uint8_t*>(out), ld_out_bytes, pieces, total);
   SAGE_CHECK_LAUNCH("sage_pad_rows");
   return SAGE_OK;

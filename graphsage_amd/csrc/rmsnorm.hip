@@ -9,8 +9,14 @@
 //
 // Bound by HBM: every array is read or written once.  A row stays in registers between the
 // reduction and the output (kNV vectors of 16 bytes a thread), so there is no second pass over
-// memory; rows longer than the registers hold are read twice (row_loop kernels, the second time
-// mostly from L2).  Sums, maxima and rstd are fp32 whatever the type of the rows.
+// memory; rows longer than the registers hold are read twice (the long kernels, the second time
+// mostly from L2).  Sums, maxima and rstd are fp32 whatever the type of the rows, and the forward
+// pass norms the fp32 sum s; the s that is stored, and that the backward pass reads, is rounded once
+// to the rows' type, as a residual stream in that type is.
+//
+// Measured (a large copy runs at 5.16 TB/s): forward to 8 bits, 8192 x 5120 bf16 with a residual 87 us
+// = 4.8 TB/s; forward and backward, 16381 x 2047 bf16 134 us = 3.5 TB/s, of which the backward pass
+// 71 us = 3.8 TB/s.
 //
 // Rows start at any address: vectors are loaded and stored with the element's alignment (gfx950
 // splits a misaligned 16-byte access itself), so odd widths need no other kernel; a row's last
@@ -190,6 +196,13 @@ struct NormArgs {
   int normalise;        // 0: rstd = 1 (quantisation alone)
 };
 
+// Which of a launch's blocks this is: their number may pass what one dimension of a grid takes (2^32 threads).
+inline dim3 block_grid(int64_t blocks) {
+  const int64_t x = blocks < (1 << 20) ? blocks : 1 << 20;
+  return dim3(static_cast<unsigned>(x), static_cast<unsigned>(cdiv(blocks, x)));
+}
+__device__ inline int64_t block_index() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 // A row to a wave (four rows a block) or to the block; kNV vectors of 16 bytes a thread hold it.
 template <typename T, bool kInt8, bool kWaveRow, int kNV>
 __global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024) rms_norm_kernel(NormArgs a) {
@@ -198,7 +211,7 @@ __global__ void __launch_bounds__(kWaveRow ? kRowBlock : 1024) rms_norm_kernel(N
   __shared__ uint32_t lds_top[16];
   const int threads = kWaveRow ? kWave : blockDim.x;       // of a row
   const int t = kWaveRow ? threadIdx.x % kWave : threadIdx.x;
-  const int64_t row = kWaveRow ? static_cast<int64_t>(blockIdx.x) * (kRowBlock / kWave) + threadIdx.x / kWave : blockIdx.x;
+  const int64_t row = kWaveRow ? block_index() * (kRowBlock / kWave) + threadIdx.x / kWave : block_index();
   if (row >= a.rows) return;     // whole waves, and never part of a block that meets at a barrier
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ld_r : nullptr;
@@ -273,7 +286,8 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(NormArgs a) {
   constexpr int n = VecOf<T>::n;
   __shared__ float lds_sum[16];
   __shared__ uint32_t lds_top[16];
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_index();
+  if (row >= a.rows) return;
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ld_r : nullptr;
   float ss = 0.f;
@@ -632,12 +646,12 @@ void launch_norm(const NormArgs& a, hipStream_t stream) {
   const RowShape shape = row_shape(kInt8 ? a.q_cols : a.dim, VecOf<T>::n, a.rows);
   const bool held = with_row_shape(shape, [&](auto wave, auto nv) {
     constexpr bool kWaveRow = decltype(wave)::value;
-    const dim3 grid(static_cast<unsigned>(kWaveRow ? cdiv(a.rows, kRowBlock / kWave) : a.rows));
+    const dim3 grid = block_grid(kWaveRow ? cdiv(a.rows, kRowBlock / kWave) : a.rows);
     hipLaunchKernelGGL((rms_norm_kernel<T, kInt8, kWaveRow, decltype(nv)::value>), grid,
                        dim3(kWaveRow ? kRowBlock : shape.threads), 0, stream, a);
   });
   if (!held)
-    hipLaunchKernelGGL((rms_norm_long_kernel<T, kInt8>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((rms_norm_long_kernel<T, kInt8>), block_grid(a.rows), dim3(1024), 0, stream, a);
 }
 
 template <bool kInt8>

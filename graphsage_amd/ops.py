@@ -1420,10 +1420,18 @@ def _output(out, name, shape, dtype, device):
     return out
 
 
-def _like(t, out, name):
-    """`out`, checked against t's shape and dtype, or a new tensor: (tensor, pointer, row stride)."""
+def _like(t, out, name, inputs=(), apart=()):
+    """`out`, checked against t's shape and dtype, or a new tensor: (tensor, pointer, row stride).  It may be one of
+    the inputs, or apart from all of them: a row that is another's as well would be read behind its change."""
     if out is not None:
-        return (out, *_row_matrix(out, name, t.dtype, t.shape, t.device, output=True))
+        p, ld = _row_matrix(out, name, t.dtype, t.shape, t.device, output=True)
+        for other in apart:
+            if _overlap(out, other):
+                raise RuntimeError(f"{name}: shares memory with another operand")
+        for other in inputs:
+            if other is not None and _overlap(out, other) and (p, ld) != _row_matrix(other, name, t.dtype):
+                raise RuntimeError(f"{name}: shares memory with an input, at other places of its rows")
+        return out, p, ld
     out = torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
     return out, out.data_ptr(), t.shape[1]
 
@@ -1435,10 +1443,10 @@ def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out=None, sum_out=None):
     px, ldx, pr, ldr, pw, wd, shape, dev = _norm_inputs(x, weight, residual)
     if weight is None:
         raise RuntimeError("rms_norm_fwd: weight: tensor required")
-    y, py, ldy = _like(x, out, "rms_norm_fwd: out")
+    y, py, ldy = _like(x, out, "rms_norm_fwd: out", (x, residual), (weight,))
     s, ps, lds = x, None, 0
     if residual is not None:
-        s, ps, lds = _like(x, sum_out, "rms_norm_fwd: sum_out")
+        s, ps, lds = _like(x, sum_out, "rms_norm_fwd: sum_out", (x, residual), (weight, y))
     elif sum_out is not None:
         raise RuntimeError("rms_norm_fwd: sum_out without a residual")
     _call("sage_rms_norm_fwd", dev, px, ldx, pr, ldr, pw, wd, shape[0], shape[1], ROW_DTYPES[x.dtype], eps,
@@ -1454,7 +1462,7 @@ def _int8_rows(x, weight, residual, eps, normalise, padded, sum_out):
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
     s, ps, lds = x, None, 0
     if residual is not None:
-        s, ps, lds = _like(x, sum_out, "rms_norm_int8: sum_out")
+        s, ps, lds = _like(x, sum_out, "rms_norm_int8: sum_out", (x, residual), () if weight is None else (weight,))
     elif sum_out is not None:
         raise RuntimeError("rms_norm_int8: sum_out without a residual")
     _call("sage_rms_norm_int8", dev, px, ldx, pr, ldr, pw, wd, rows, dim, ROW_DTYPES[x.dtype], eps, normalise,
@@ -1518,7 +1526,7 @@ def _pieces(t, p, ld, copy=False):
     """The matrix itself if its rows are whole pieces of 16 bytes that start on 16 bytes, else a
     zero-filled copy that is: (pointer, row stride in elements, columns, what must stay alive)."""
     size, (rows, cols) = t.element_size(), t.shape
-    if not copy and p % 16 == 0 and ld * size % 16 == 0 and cols * size % 16 == 0 and ld * size < 1 << 23:
+    if not copy and p % 16 == 0 and ld * size % 16 == 0 and cols * size % 16 == 0 and cols <= ld < (1 << 23) // size:
         return p, ld, cols, t
     each = 16 // size
     wide = (cols + each - 1) // each * each

@@ -13,7 +13,8 @@
  *   - All pointers are DEVICE pointers (hipMalloc'ed / torch CUDA tensors) unless the
  *     parameter name ends in `_host`.
  *   - Index tensors are int64 (`sage_i64`), as in the reference's torch.LongTensor
- *     (samplers/uniform_loader.py:60-61).  Features/weights/gradients are IEEE fp32.
+ *     (samplers/uniform_loader.py:60-61).  Features/weights/gradients are IEEE fp32,
+ *     but for the feed-forward block's entry points (the last section), which name their types.
  *   - `stream` is a hipStream_t passed as void* (NULL = the default stream).  All work is
  *     enqueued on it; no entry point synchronises, allocates or frees device memory or
  *     retains a pointer after it returns, so every call may be captured in a HIP graph.
@@ -763,7 +764,8 @@ int sage_adam_step_parts(float* param, float* grad, float* exp_avg, float* exp_a
 /* s = x + residual (fp32 sum; residual may be NULL), rstd = 1 / sqrt(mean(s^2) + eps),
  * y = s * rstd * weight, each output rounded once to the rows' type.  sum (may be NULL) is s.
  * The weight is in the rows' type or in fp32.  Rows may start at any element; stride 0 repeats
- * a row.  sum may be the residual's own buffer. */
+ * a row.  y and sum may each be the buffer of x or of the residual (row for row), else they share no
+ * memory with an input or with each other. */
 int sage_rms_norm_fwd(const void* x, sage_i64 ld_x, const void* residual, sage_i64 ld_r, const void* weight,
                       int weight_dtype, sage_i64 rows, sage_i64 dim, int dtype, float eps, void* y, sage_i64 ld_y,
                       void* sum, sage_i64 ld_sum, void* stream);

@@ -355,6 +355,51 @@ def test_few_rows_of_odd_lengths(dev, dtype, m, n, k):
     within(got, want, gated_bound(g, u, dg, du, "silu") * (1 + 2 ** -7) + want.abs() * U[dtype] + TINY[dtype], "out")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_backward_takes_repeated_rows(dev, dtype):
+    """x and both weights as one row repeated (stride 0), and weights that are every other row of a buffer."""
+    rng = gen(dev, 5)
+    x, w = normal(rng, 1, 64, dtype=dtype).expand(40, 64), normal(rng, 1, 64, dtype=dtype).expand(24, 64)
+    v = normal(rng, 48, 64, dtype=dtype)[::2]
+    for args in ((x, w, w), (x, v, w), (x.contiguous(), v, v)):
+        dh = normal(rng, 40, 24, dtype=dtype)
+        full = [t.contiguous() for t in args]
+        saved = ops.gated_linear_fwd(*args, save=True)[1]
+        assert torch.equal(saved, ops.gated_linear_fwd(*full, save=True)[1])
+        for got, want in zip(ops.gated_linear_bwd(dh, *args, saved), ops.gated_linear_bwd(dh, *full, saved)):
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows,dim,dtype", [(2 ** 26 + 5, 8, torch.bfloat16), (2 ** 22 + 3, 2056, torch.bfloat16), (2 ** 22 + 3, 1032, torch.float32)])
+def test_rms_norm_of_very_many_rows(dev, rows, dim, dtype):
+    """More rows than one dimension of a grid takes threads for, as one row repeated and its last rows others."""
+    rng = gen(dev, dim)
+    row, w = normal(rng, 1, dim, dtype=dtype), normal(rng, dim, dtype=dtype)
+    y, _ = ops.rms_norm_fwd(row.expand(rows, dim), w)
+    want = ops.rms_norm_fwd(row.expand(2048, dim), w)[0][:1]
+    for at in (0, 2 ** 20 - 1, 2 ** 20, 2 ** 22, rows - 1):
+        assert torch.equal(y[at:at + 1], want), at
+    q, scale = ops.quantize_rows(row.expand(rows, dim))
+    want, one = ops.quantize_rows(row.expand(2048, dim))
+    for at in (0, 2 ** 20, 2 ** 22, rows - 1):
+        assert torch.equal(q[at], want[0]) and torch.equal(scale[at], one[0]), at
+
+
+def test_norm_outputs_that_share_memory(dev):
+    """An output may be an input, row for row; shifted against one, or both outputs in one buffer, is refused."""
+    rng = gen(dev, 3)
+    hold, w = normal(rng, 41, 96), normal(rng, 96)
+    x, r = hold[:20], hold[20:40]
+    y, s = ops.rms_norm_fwd(x, w, r)
+    for kw in (dict(out=hold[1:21]), dict(sum_out=hold[21:41]), dict(out=r, sum_out=r), dict(sum_out=hold.view(-1)[8:8 + 1920].view(20, 96))):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            ops.rms_norm_fwd(x, w, r, **kw)
+    with pytest.raises(RuntimeError, match="shares memory"):
+        ops.rms_norm_int8(x, w, r, sum_out=hold[21:41])
+    y2, s2 = ops.rms_norm_fwd(x, w, r, out=x, sum_out=r)
+    assert torch.equal(y, y2) and torch.equal(s, s2)
+
+
 def test_not_a_number_stays_in_its_row(dev):
     """A NaN in a row of x reaches that row's outputs and no others, also through rows that fill a tile."""
     for m in (3, 70, 300):
