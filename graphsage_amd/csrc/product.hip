@@ -4,7 +4,16 @@
 // All of them are C[m, n] = sum_k A[m, k] B[n, k] with both operands' rows contiguous in k, and one
 // kernel body serves every type because it works on 16-byte pieces of rows: a lane's operand of an
 // MFMA is 16 bytes of one row whatever the type (16 int8, 8 bf16 / fp16, 4 fp32), and the order in
-// which the k of a product are summed over lanes is free as long as A and B agree on it.
+// which the k of a product are summed over lanes is free as long as A and B agree on it.  (The backward
+// pass's products read operands whose rows are rows of k across, see below.)
+//
+// Large products are bound by the MFMAs and, as closely, by LDS: a 256 x 256 tile reads 96 KB a run of 64
+// bytes of k and is handed 32, which takes as long as its MFMAs; they are busy 59 % of the time at about
+// 2.0 GHz.  Small ones are bound by the weights' bytes (few_rows) or by a launch's start and its one burst of
+// stores.  Measured: 8 bits 8192^3 to bf16 450 us = 2.44 PTOP/s; bf16 forward 8192 x 8192 (two weights)
+// over 2048 430 us of products and, with g and u kept, 165 of stores; dx and dw 475 each = 1.15 PFLOP/s;
+// fp32 13312 x 1024 over 256 157, 156 and 130 us for three times 14 GFLOP; 8 bits 1 x 4096 over 4096
+// 5.3 us = 3.2 TB/s of weights; 4 rows against a bf16 pair of 5632 x 2048 4.1 TB/s.
 #include "common.h"
 
 #include <type_traits>
