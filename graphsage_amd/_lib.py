@@ -124,7 +124,7 @@ SIGNATURES = {
     "sage_rms_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
     "sage_rms_norm_bwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, _P, c_int64, c_int64, c_int64, c_int, c_float,
                                   _P, c_int64, _P, _P, c_size_t, _P]),
-    "sage_pad_rows": (c_int, [_P, c_int64, c_int64, c_int64, _P, c_int64, _P]),
+    "sage_pad_rows": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int64, _P, c_int64, _P]),
     "sage_int8_linear": (c_int, [_P, c_int64, _P, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int, _P, c_int64,
                                  _P, c_size_t, _P]),
     "sage_product_any_rows": (c_int, [c_int64, c_int64, c_int64, c_int, c_int]),

@@ -856,7 +856,8 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool 
   }
   for (int tile : {128, 256}) {
     const int64_t tiles = cdiv(m, tile) * cdiv(n, gated ? tile / 2 : tile);
-    for (int64_t slices = 1; slices <= 32 && 2 * slices <= steps + 1; slices *= 2) {
+    for (const int slices : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32}) {
+      if (2 * slices > steps + 1) break;
       const int64_t each = cdiv(steps, slices), blocks = tiles * slices;
       if (cdiv(steps, each) != slices) continue;
       double time;
@@ -872,7 +873,7 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool 
       if (slices > 1) time += 4.2 + 2.0 * bytes / 7.5e6;
       if (time < least) {
         least = time;
-        best = Plan{tile, static_cast<int>(slices), each * 2, slices > 1 ? static_cast<size_t>(bytes) : 0};
+        best = Plan{tile, slices, each * 2, slices > 1 ? static_cast<size_t>(bytes) : 0};
       }
     }
   }
@@ -1000,11 +1001,20 @@ __global__ void __launch_bounds__(256) gate_bwd_kernel(const T* dh, int64_t ld_d
   }
 }
 
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint8_t* in, int64_t ld_in, int64_t row_bytes, uint8_t* out,
-                                                       int64_t ld_out, int64_t pieces, int64_t total) {
+struct PadArgs {
+  const uint8_t* in[3];
+  int64_t ld[3];          // bytes
+  int64_t first[3];       // output row of the first row
+};
+// A piece of 16 bytes a thread.  The matrices of a product come in one launch: most are small, and a call's launches cost
+// more than the bytes (8 bits, 1411 x 470 over 634: a launch and an output for each 24.0 us a call, one for both 18.7).
+__global__ void __launch_bounds__(256) pad_rows_kernel(PadArgs a, int64_t row_bytes, uint8_t* out, int64_t ld_out, int64_t pieces,
+                                                       int64_t total) {
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t row = i / pieces, at = (i - row * pieces) * 16;
-    const uint8_t* p = in + row * ld_in + at;
+    const int of = row >= a.first[2] ? 2 : row >= a.first[1] ? 1 : 0;
+    const uint8_t* p = (of == 2 ? a.in[2] : of == 1 ? a.in[1] : a.in[0]) +
+                       (row - (of == 2 ? a.first[2] : of == 1 ? a.first[1] : 0)) * (of == 2 ? a.ld[2] : of == 1 ? a.ld[1] : a.ld[0]) + at;
     struct __attribute__((packed, aligned(1))) P {
       uint8_t v[16];
     } k;
@@ -1080,17 +1090,22 @@ int gated_bwd(const void* dh, int64_t ld_dh, const void* x, int64_t ld_x, const 
 
 using namespace sage;
 
-extern "C" int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows, sage_i64 row_bytes, void* out,
+extern "C" int sage_pad_rows(const void* in0, sage_i64 ld0_bytes, sage_i64 rows0, const void* in1, sage_i64 ld1_bytes, sage_i64 rows1,
+                             const void* in2, sage_i64 ld2_bytes, sage_i64 rows2, sage_i64 row_bytes, void* out,
                              sage_i64 ld_out_bytes, void* stream) {
-  SAGE_REQUIRE(rows >= 0 && row_bytes > 0, SAGE_EINVAL, "sage_pad_rows: bad shape [%ld, %ld]", (long)rows, (long)row_bytes);
+  SAGE_REQUIRE(rows0 >= 0 && rows1 >= 0 && rows2 >= 0 && row_bytes > 0, SAGE_EINVAL, "sage_pad_rows: bad shape [%ld + %ld + %ld, %ld]",
+               (long)rows0, (long)rows1, (long)rows2, (long)row_bytes);
+  const int64_t rows = rows0 + rows1 + rows2;
   if (rows == 0) return SAGE_OK;
-  SAGE_REQUIRE(in != nullptr && out != nullptr, SAGE_EINVAL, "sage_pad_rows: NULL pointer");
-  SAGE_REQUIRE(rows16(out, ld_out_bytes) && ld_out_bytes >= row_bytes && ld_in_bytes >= 0, SAGE_EINVAL,
+  SAGE_REQUIRE((in0 || rows0 == 0) && (in1 || rows1 == 0) && (in2 || rows2 == 0) && out, SAGE_EINVAL, "sage_pad_rows: NULL pointer");
+  SAGE_REQUIRE(rows16(out, ld_out_bytes) && ld_out_bytes >= row_bytes && ld0_bytes >= 0 && ld1_bytes >= 0 && ld2_bytes >= 0, SAGE_EINVAL,
                "sage_pad_rows: output rows start on 16 bytes and hold the input's");
+  const PadArgs a = {{static_cast<const uint8_t*>(in0), static_cast<const uint8_t*>(in1), static_cast<const uint8_t*>(in2)},
+                     {ld0_bytes, ld1_bytes, ld2_bytes}, {0, rows0, rows0 + rows1}};
   const int64_t pieces = cdiv(row_bytes, 16), total = rows * pieces;
   const int64_t blocks = cdiv(total, 256) < (1 << 20) ? cdiv(total, 256) : 1 << 20;
   hipLaunchKernelGGL(pad_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                     static_cast<const uint8_t*>(in), ld_in_bytes, row_bytes, static_cast<uint8_t*>(out), ld_out_bytes, pieces, total);
+                     a, row_bytes, static_cast<uint8_t*>(out), ld_out_bytes, pieces, total);
   SAGE_CHECK_LAUNCH("sage_pad_rows");
   return SAGE_OK;
 }

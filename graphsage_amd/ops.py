@@ -1522,17 +1522,33 @@ def rms_norm_bwd(dy, s, weight, eps=1e-6, dsum=None, need_dx=True, need_dw=True)
     return dx, dw
 
 
-def _pieces(t, p, ld, copy=False):
-    """The matrix itself if its rows are whole pieces of 16 bytes that start on 16 bytes, else a
-    zero-filled copy that is: (pointer, row stride in elements, columns, what must stay alive)."""
-    size, (rows, cols) = t.element_size(), t.shape
-    if not copy and p % 16 == 0 and ld * size % 16 == 0 and cols * size % 16 == 0 and cols <= ld < (1 << 23) // size:
-        return p, ld, cols, t
+def _pieces(k, size, mats, same=()):
+    """The matrices (tensor, pointer, row stride) of rows of k elements as ones whose rows are whole pieces of 16
+    bytes that start on 16 bytes: themselves, or zero-filled copies, all of them in one buffer.  same: matrices
+    whose row strides have to be equal.  Returns (columns, [(pointer, row stride)], what must stay alive)."""
     each = 16 // size
-    wide = (cols + each - 1) // each * each
-    out = torch.empty((rows, wide), dtype=t.dtype, device=t.device)
-    _call("sage_pad_rows", t.device, p, ld * size, rows, cols * size, out.data_ptr(), wide * size)
-    return out.data_ptr(), wide, wide, out
+    wide = (k + each - 1) // each * each
+    uneven = len({mats[i][2] for i in same}) > 1
+    copied = [i for i, (_, p, ld) in enumerate(mats) if k != wide or p % 16 or ld % each or not k <= ld < (1 << 23) // size or
+              (uneven and i in same)]
+    done = [(p, ld) for _, p, ld in mats]
+    if not copied:
+        return wide, done, None
+    if not set(copied).isdisjoint(same):
+        copied = sorted({*copied, *same})
+    args, rows = [], 0
+    for i in copied:
+        t, p, ld = mats[i]
+        args += [p, ld * size, t.size(0)]
+        rows += t.size(0)
+    first = mats[0][0]
+    out = torch.empty((rows, wide), dtype=first.dtype, device=first.device)
+    at = out.data_ptr()
+    _call("sage_pad_rows", first.device, *args, *(None, 0, 0) * (3 - len(copied)), k * size, at, wide * size)
+    for i in copied:
+        done[i] = (at, wide)
+        at += mats[i][0].size(0) * wide * size
+    return wide, done, out
 
 
 def _product_rows(m, n, k, size, fp32, *mats):
@@ -1544,8 +1560,7 @@ def _product_rows(m, n, k, size, fp32, *mats):
         far |= ld * size >= 1 << 23
     if not far and (bits & 15 == 0 or m <= 512 and _lib.load().sage_product_any_rows(m, n, k * size, len(mats) - 2, fp32)):
         return k, [(p, ld) for _, p, ld in mats], None
-    done = [_pieces(*mat) for mat in mats]
-    return done[0][2], [d[:2] for d in done], done
+    return _pieces(k, size, mats)
 
 
 def _product_workspace(m, n, row_bytes, gated, fp32, device):
@@ -1685,12 +1700,8 @@ def gated_linear_bwd(dh, x, w_gate, w_up, saved, activation="silu", need_dx=True
         dw = torch.zeros((2 * h, k), dtype=x.dtype, device=dev) if need_dw else None
     else:
         dw = torch.empty((2 * h, k), dtype=x.dtype, device=dev) if need_dw else None
-        px, ldx, _, keep_x = _pieces(x, px, ldx)
-        pg, ldg, _, keep_g = _pieces(w_gate, pg, ldg)
-        pu, ldu, _, keep_u = _pieces(w_up, pu, ldu)
-        if ldg != ldu:                       # the weights' rows go on from one to the other at one stride
-            pg, ldg, _, keep_g = _pieces(keep_g, pg, ldg, copy=True)
-            pu, ldu, _, keep_u = _pieces(keep_u, pu, ldu, copy=True)
+        # the weights' rows go on from one to the other at one stride
+        _, ((px, ldx), (pg, ldg), (pu, ldu)), kept = _pieces(k, x.element_size(), ((x, px, ldx), (w_gate, pg, ldg), (w_up, pu, ldu)), (1, 2))
         ws_bytes = _lib.load().sage_gated_linear_bwd_workspace_bytes(m, h, k, ROW_DTYPES[x.dtype])
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         _call("sage_gated_linear_bwd", dev, pd, ldd, px, ldx, pg, ldg, pu, ldu, saved.data_ptr(), act, m, h, k,

@@ -791,9 +791,11 @@ int sage_rms_norm_bwd(const void* dy, sage_i64 ld_dy, const void* sum, sage_i64 
                       void* stream);
 
 /* Rows of row_bytes bytes into rows that start on 16 bytes and end, zero-filled, on 16 bytes:
- * what the products below take (both operands' rows, and k, in whole pieces of 16 bytes) where
- * sage_product_any_rows does not say that they take any. */
-int sage_pad_rows(const void* in, sage_i64 ld_in_bytes, sage_i64 rows, sage_i64 row_bytes, void* out,
+ * what the products below take (their operands' rows, and k, in whole pieces of 16 bytes) where
+ * sage_product_any_rows does not say that they take any.  Up to three matrices, below each other in
+ * out (those with no rows may be NULL). */
+int sage_pad_rows(const void* in0, sage_i64 ld0_bytes, sage_i64 rows0, const void* in1, sage_i64 ld1_bytes, sage_i64 rows1,
+                  const void* in2, sage_i64 ld2_bytes, sage_i64 rows2, sage_i64 row_bytes, void* out,
                   sage_i64 ld_out_bytes, void* stream);
 /* 1 where a product below (row_bytes >= 16) takes rows of any alignment and length as they are: those
  * with few rows, whose weights a padded copy would cost more than the product. */

@@ -87,8 +87,8 @@ def test_product_refusals():
     for code, change in ((EINVAL, dict(dh=None)), (EINVAL, dict(saved=None)), (EINVAL, dict(dx=None, dw=None)), (EINVAL, dict(m=0)), (EINVAL, dict(act=7)),
                          (EINVAL, dict(lddx=15)), (EWORKSPACE, dict(n=size - 1)), (EWORKSPACE, dict(ws=ODD))):
         refused(code, "sage_gated_linear_bwd", *{**ok, **change}.values())
-    for change in (dict(i=None), dict(o=ODD), dict(ldo=24), dict(ldo=16), dict(b=0)):
-        refused(EINVAL, "sage_pad_rows", *{**dict(i=P, ldi=20, r=3, b=20, o=P, ldo=32, st=None), **change}.values())
+    for change in (dict(i=None), dict(j=None), dict(l=None), dict(o=ODD), dict(ldo=24), dict(ldo=16), dict(b=0), dict(r=-1)):
+        refused(EINVAL, "sage_pad_rows", *{**dict(i=P, ldi=20, r=3, j=P, ldj=20, rj=1, l=P, ldl=0, rl=2, b=20, o=P, ldo=32, st=None), **change}.values())
 
 
 def test_empty_inputs_launch_nothing():
@@ -96,7 +96,7 @@ def test_empty_inputs_launch_nothing():
     assert lib.sage_rms_norm_fwd(*norm(rows=0, x=None, y=None)) == 0
     assert lib.sage_int8_linear(None, 64, None, P, 64, P, None, 0, 8, 64, 0, None, 8, None, 0, None) == 0
     assert lib.sage_gated_linear_fwd(None, 16, P, 16, P, 16, 0, 0, 8, 16, 0, None, 8, None, None, 0, None) == 0
-    assert lib.sage_pad_rows(None, 20, 0, 20, None, 32, None) == 0
+    assert lib.sage_pad_rows(None, 20, 0, None, 0, 0, None, 0, 0, 20, None, 32, None) == 0
 
 
 def test_not_recordable_on_a_tape():
