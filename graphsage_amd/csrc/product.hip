@@ -11,7 +11,7 @@
 // bytes of k and is handed 32, which takes as long as its MFMAs; they are busy 59 % of the time at about
 // 2.0 GHz.  Small ones are bound by the weights' bytes (few_rows) or by a launch's start and its one burst of
 // stores.  Measured: 8 bits 8192^3 to bf16 450 us = 2.44 PTOP/s; bf16 forward 8192 x 8192 (two weights)
-// over 2048 430 us of products and, with g and u kept, 165 of stores; dx and dw 475 each = 1.15 PFLOP/s;
+// over 2048 490 us, 590 with g and u kept (537 MB of stores more); dx and dw 475 each = 1.15 PFLOP/s;
 // fp32 13312 x 1024 over 256 157, 156 and 130 us for three times 14 GFLOP; 8 bits 1 x 4096 over 4096
 // 5.3 us = 3.2 TB/s of weights; 4 rows against a bf16 pair of 5632 x 2048 4.1 TB/s.
 #include "common.h"
@@ -665,10 +665,22 @@ __global__ void __launch_bounds__(256) join_kernel(Product p, int tiles_m, int t
   Acc acc[1][S::kNI];
 #pragma unroll
   for (int j = 0; j < S::kNI; ++j) acc[0][j] = __builtin_bit_cast(Acc, from[j * kWave]);
-  for (int s = 1; s < slices; ++s) {
-    from += stride;
+  constexpr int kAhead = 4;      // slices under way at once (48 slices 17 -> 11 us; with 8, whose places behind the last load it again, 2 or 3 slices cost a microsecond more)
+  for (int s = 1; s < slices; s += kAhead) {
+    i32x4 part[kAhead][S::kNI];
 #pragma unroll
-    for (int j = 0; j < S::kNI; ++j) acc[0][j] += __builtin_bit_cast(Acc, from[j * kWave]);
+    for (int t = 0; t < kAhead; ++t) {
+      const int of = s + t < slices ? s + t : s;
+#pragma unroll
+      for (int j = 0; j < S::kNI; ++j) part[t][j] = from[of * stride + j * kWave];
+    }
+    asm volatile("" ::: "memory");      // the loads stay in front of the first sum
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      if (s + t >= slices) break;
+#pragma unroll
+      for (int j = 0; j < S::kNI; ++j) acc[0][j] += __builtin_bit_cast(Acc, part[t][j]);
+    }
   }
   const int64_t m0 = static_cast<int64_t>(tm) * kTile, n0 = static_cast<int64_t>(tn) * S::kColsOut;
   finish_rows<T, kGated, kBT, 1>(p, m0, n0, (wave / S::WN * S::kMI + i) * 16, wave % S::WN, lane,
@@ -856,7 +868,7 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t kbytes, bool gated, bool 
   }
   for (int tile : {128, 256}) {
     const int64_t tiles = cdiv(m, tile) * cdiv(n, gated ? tile / 2 : tile);
-    for (const int slices : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32}) {
+    for (const int slices : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64}) {
       if (2 * slices > steps + 1) break;
       const int64_t each = cdiv(steps, slices), blocks = tiles * slices;
       if (cdiv(steps, each) != slices) continue;
