@@ -11,6 +11,10 @@ quantize_() lays the three weights out in 8 bits, one scale a channel, for infer
 writes 8 bits with a scale a row, and every product is an 8-bit one.  The 8-bit weights are those of the
 call's moment: train() and load_state_dict() drop them, any other change of the weights needs quantize_()
 again.  They serve calls in eval mode without gradients; every other call takes the fp32 weights.
+
+A training step of the block can be captured into a graph.  As with any module, no eager output of the same
+parameters may be alive then: torch keeps the stream of a parameter's gradient with the first of them, and
+a captured backward pass cannot wait for that stream.
 """
 import torch
 
