@@ -850,9 +850,9 @@ struct Plan {
   size_t workspace;
 };
 
-// The cut with the least estimated time.  The estimate, in microseconds, is fitted to measurements of every cut at m
-// 24 to 8000 against weights of 256 x 256 to 8192 x 2048 and 2048 x 8192 in 8 bits, bf16 pairs and fp32 pairs: its
-// choice is 0.4 % slower than the best cut there in the geometric mean, and 18 % at most.
+// The cut with the least estimated time.  The estimate, in microseconds, is fitted to measurements of every cut (slices
+// in powers of two, up to 32) at m 24 to 8000 against weights of 256 x 256 to 8192 x 2048 and 2048 x 8192 in 8 bits, bf16
+// pairs and fp32 pairs: its choice is 0.4 % slower than the best cut there in the geometric mean, and 18 % at most.
 //   few rows: a block's bytes of k at 2.2 us a thousand (more with two Bs), blocks in turns of one a CU;
 //   tiles: a step of 128 bytes of k takes a CU 1.5 us at 256 x 256 (1.4 while half of the chip is idle), at
 //     128 x 128 0.57 us alone and 1.2 us for the two that share a CU; fp32 is bound by its MFMAs (8, 2.15, 4.4 us);

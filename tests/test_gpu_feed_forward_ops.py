@@ -385,6 +385,40 @@ def test_rms_norm_of_very_many_rows(dev, rows, dim, dtype):
         assert torch.equal(q[at], want[0]) and torch.equal(scale[at], one[0]), at
 
 
+def test_products_behind_32_bit_offsets(dev):
+    """More than 2^31 outputs, saved sums and weight bytes: the last rows against calls of their own.  Small whole
+    numbers, so that every sum is exact and the order of its terms is free."""
+    rng = gen(dev, 31)
+    m, h, k, last = 66000, 33000, 32, 5
+
+    def whole(rows, cols, dtype):
+        return torch.randint(-1, 2, (rows, cols), generator=rng, device=dev, dtype=torch.int8).to(dtype)
+
+    x, w, v = (whole(n, k, torch.int8) for n in (m, h, h))
+    sx, sw = torch.rand(m, generator=rng, device=dev), torch.rand(h, generator=rng, device=dev)
+    out = ops.int8_linear(x, sx, w, sw, out_dtype=torch.bfloat16)
+    assert out.numel() > 2 ** 31
+    assert torch.equal(out[-last:], ops.int8_linear(x[-last:], sx[-last:], w, sw, out_dtype=torch.bfloat16))
+    del out
+    x, w, v = x.bfloat16(), w.bfloat16(), v.bfloat16()
+    out, saved = ops.gated_linear_fwd(x, w, v, "relu", save=True)
+    end, end_saved = ops.gated_linear_fwd(x[-last:], w, v, "relu", save=True)
+    assert torch.equal(out[-last:], end) and torch.equal(saved[:, -last:], end_saved)
+    dh = out.zero_()
+    dh[-last:] = whole(last, h, torch.bfloat16)
+    got = ops.gated_linear_bwd(dh, x, w, v, saved, "relu")
+    want = ops.gated_linear_bwd(dh[-last:], x[-last:], w, v, end_saved, "relu")
+    assert torch.equal(got[0][-last:], want[0]) and not got[0][:-last].any()
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    del out, saved, dh
+    n, k = 2 ** 24 + 21, 130           # weights of more than 2^31 bytes, few rows
+    w = torch.randint(-2, 3, (n, k), generator=rng, device=dev, dtype=torch.int8)
+    x, sx, sw = whole(3, k, torch.int8), torch.ones(3, device=dev), torch.ones(n, device=dev)
+    out = ops.int8_linear(x, sx, w, sw)
+    for at in (0, 2 ** 24 - 1, n - 40):
+        assert torch.equal(out[:, at:at + 40].double(), x.double() @ w[at:at + 40].double().t()), at
+
+
 def test_norm_outputs_that_share_memory(dev):
     """An output may be an input, row for row; shifted against one, or both outputs in one buffer, is refused."""
     rng = gen(dev, 3)
