@@ -842,6 +842,43 @@ inline bool rows16(const void* p, int64_t ld_bytes) {
 }
 constexpr int64_t kMaxRowBytes = int64_t{1} << 23;     // the tile loads' offsets: 256 rows in 31 bits
 
+// Up to 8 rows against one B in blocks of 8 columns: an MFMA operand's slots 8 to 15 are the rows and columns of slots 0
+// to 7 again, at later bytes of k, so that C's two diagonal quarters add up to the 8 x 8 outputs.
+template <typename T, int U, bool kRagged>
+__global__ void __launch_bounds__(kFewWaves* kWave) few_rows_half_kernel(Product p) {
+  using Acc = typename Mma<T>::Acc;
+  __shared__ Acc lds[kFewWaves][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int l15 = lane & 15, q = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 8;
+  const int64_t col = n0 + (l15 & 7) < p.n ? n0 + (l15 & 7) : p.n - 1, row = (l15 & 7) < p.m ? l15 & 7 : p.m - 1;
+  const char* b = p.b0 + col * p.ldb0;
+  const char* a = p.a + row * p.lda;
+  const int64_t from = (l15 >> 3) * (U * 64) + q * 16;
+  Acc acc = Acc{};
+  for (int64_t k = wave * (2 * U * 64); k < p.kbytes; k += kFewWaves * 2 * U * 64) {
+    const bool last = k + 2 * U * 64 > p.kbytes;
+    i32x4 bv[U], av[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) bv[u] = load_piece<T, kRagged>(b, k + from + u * 64, p.kbytes, last);
+#pragma unroll
+    for (int u = 0; u < U; ++u) av[u] = load_piece<T, kRagged>(a, k + from + u * 64, p.kbytes, last);
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc = Mma<T>::mma(bv[u], av[u], acc);
+  }
+  lds[wave][lane] = acc;
+  __syncthreads();
+  if (threadIdx.x >= 32 || l15 >= 8) return;      // lane: row l15, columns 4 q + 0..3; 40 lanes on those of the later k
+  Acc sum = lds[0][lane] + lds[0][lane + 40];
+#pragma unroll
+  for (int w = 1; w < kFewWaves; ++w) sum += lds[w][lane] + lds[w][lane + 40];
+  using E = std::conditional_t<std::is_same<T, int8_t>::value, int, float>;
+  E c[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] = sum[e];
+  finish<T, 4>(p, l15, n0 + q * 4, c);
+}
+
 // How a product is cut: blocks of 64 rows and 16 columns (tile 0: few_rows_kernel), or tiles of `tile` x `tile`
 // (gated: `tile` / 2 columns), k in `slices`.
 struct Plan {
@@ -929,6 +966,14 @@ void launch_few_rows(const Product& p, hipStream_t stream) {
       const dim3 eight(static_cast<unsigned>(cdiv(p.n, 8)));
       if (p.kbytes >= kFewWaves * 512) hipLaunchKernelGGL((few_rows_pair_kernel<T, 8, kRagged>), eight, threads, 0, stream, p);
       else hipLaunchKernelGGL((few_rows_pair_kernel<T, 4, kRagged>), eight, threads, 0, stream, p);
+      return;
+    }
+  }
+  if constexpr (!kGated) {
+    // the same, for up to 8 rows (8 bits, 1 row: 2048 x 8192 8.0 -> 6.5 us, 5120 x 13824 22.0 -> 18.4, 64 x 65536 36.6 -> 19.5)
+    if (p.m <= 8 && cdiv(cdiv(p.n, 8), 256) < 2 * cdiv(cdiv(p.n, 16), 256)) {
+      const dim3 eight(static_cast<unsigned>(cdiv(p.n, 8)));
+      hipLaunchKernelGGL((few_rows_half_kernel<T, 4, kRagged>), eight, threads, 0, stream, p);
       return;
     }
   }
