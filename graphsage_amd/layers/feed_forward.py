@@ -9,8 +9,11 @@ functional.gated_linear).
 
 quantize_() lays the three weights out in 8 bits, one scale a channel, for inference: the norm then
 writes 8 bits with a scale a row, and every product is an 8-bit one.  The 8-bit weights are those of the
-call's moment: train() and load_state_dict() drop them, any other change of the weights needs quantize_()
-again.  They serve calls in eval mode without gradients; every other call takes the fp32 weights.
+call's moment: train() and load_state_dict() drop them, and so does the next call after any change of a weight
+that torch counts (an optimizer's step, copy_, another Parameter in its place; a write through .data or through
+a raw pointer is not counted and needs quantize_() again).  They serve calls in eval mode without gradients;
+every other call takes the fp32 weights.  A graph captured while they served reads them where they lay: keep
+the weights as they are, and the block in eval mode, for as long as it is replayed.
 
 A training step of the block can be captured into a graph.  As with any module, no eager output of the same
 parameters may be alive then: torch keeps the stream of a parameter's gradient with the first of them, and
@@ -33,9 +36,10 @@ class GatedFeedForward(torch.nn.Module):
         self.up = torch.nn.Linear(channels, hidden_channels, bias=False)
         self.down = torch.nn.Linear(hidden_channels, channels, bias=False)
         self._eight = None
+        self._eight_of = None            # the weights that the 8 bits were made from, and how far torch had counted
 
     def reset_parameters(self):
-        self._eight = None
+        self._eight = self._eight_of = None
         with torch.no_grad():
             self.norm_weight.fill_(1.0)
         for layer in (self.gate, self.up, self.down):
@@ -45,32 +49,53 @@ class GatedFeedForward(torch.nn.Module):
     @torch.no_grad()
     def quantize_(self):
         self._eight = tuple(ops.quantize_rows(layer.weight, padded=True) for layer in (self.gate, self.up, self.down))
+        self._eight_of = self._weights_now()
         return self
 
+    def _weights_now(self):
+        weights = (self.gate.weight, self.up.weight, self.down.weight)
+        return tuple((w, w.data_ptr(), None if w.is_inference() else w._version) for w in weights)
+
+    def _current(self):
+        """The 8-bit weights are there and still those of the weights; if not, they are dropped."""
+        if self._eight is not None and not all(a[0] is b[0] and a[1:] == b[1:]
+                                               for a, b in zip(self._eight_of, self._weights_now())):
+            self._eight = self._eight_of = None
+        return self._eight is not None
+
+    def __getstate__(self):              # copies and pickles take the 8-bit weights along where they are current
+        self._current()
+        return dict(self.__dict__)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if self._eight is not None:
+            self._eight_of = self._weights_now()
+
     def dequantize_(self):
-        self._eight = None
+        self._eight = self._eight_of = None
         return self
 
     @property
     def quantized(self):
-        return self._eight is not None
+        return self._current()
 
     def train(self, mode=True):
         if mode:
-            self._eight = None
+            self._eight = self._eight_of = None
         return super().train(mode)
 
     def _apply(self, fn, *args, **kwargs):      # .to() and the like: the 8-bit copies stay behind
-        self._eight = None
+        self._eight = self._eight_of = None
         return super()._apply(fn, *args, **kwargs)
 
     def _load_from_state_dict(self, *args, **kwargs):
-        self._eight = None
+        self._eight = self._eight_of = None
         return super()._load_from_state_dict(*args, **kwargs)
 
     # ------------------------------------------------------------------ forward
     def forward(self, x, residual=None):
-        if self._eight is not None and not self.training and not torch.is_grad_enabled():
+        if not self.training and not torch.is_grad_enabled() and self._current():
             return self._serve(x, residual)
         if residual is None:
             y, s = SF.rms_norm(x, self.norm_weight, eps=self.eps), x

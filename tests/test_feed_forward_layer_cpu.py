@@ -1,0 +1,85 @@
+"""GatedFeedForward's and the autograd forms' choices, with recorders in place of the kernels: which form a call takes,
+and which weights it serves."""
+import copy
+import io
+
+import pytest
+import torch
+
+from graphsage_amd import functional as SF
+from graphsage_amd import ops
+from graphsage_amd.layers import GatedFeedForward
+
+
+@pytest.fixture
+def served(monkeypatch):
+    """An 8-bit layout that is a copy of its weight, and a block that says which weights a call was served from."""
+    monkeypatch.setattr(ops, "quantize_rows", lambda w, padded=False: (w.detach().clone(), torch.ones(w.size(0))))
+    monkeypatch.setattr(SF, "rms_norm", lambda *a, **k: a[0])
+    monkeypatch.setattr(SF, "gated_linear", lambda x, *a: x)
+    monkeypatch.setattr(SF, "linear_concat", lambda h, w: "fp32")
+    monkeypatch.setattr(GatedFeedForward, "_serve", lambda self, x, r: self._eight)
+    monkeypatch.setattr(torch.Tensor, "__add__", lambda a, b: b)
+
+    def call(block):
+        with torch.no_grad():
+            return block(torch.zeros(1, 8))
+    return call
+
+
+CHANGES = {
+    "copy_": lambda b: b.up.weight.detach().copy_(torch.zeros(12, 8)),
+    "in place": lambda b: b.gate.weight.detach().mul_(0.5),
+    "another parameter": lambda b: setattr(b.down, "weight", torch.nn.Parameter(torch.zeros(8, 12))),
+    "other data": lambda b: setattr(b.gate.weight, "data", torch.zeros(12, 8)),
+    "a layer's load_state_dict": lambda b: b.up.load_state_dict({"weight": torch.zeros(12, 8)}),
+    "a layer's reset": lambda b: b.up.reset_parameters(),
+    "a step": lambda b: torch.optim.SGD(b.parameters(), lr=0.1).step(),
+}
+
+
+@pytest.mark.parametrize("change", CHANGES)
+@pytest.mark.parametrize("training", [False, True])
+def test_changed_weights_are_not_served_from_old_8_bits(served, change, training):
+    """In eval mode, and where the 8 bits were laid out in training mode."""
+    block = GatedFeedForward(8, 12).train(training)
+    block.quantize_()
+    block.eval()
+    assert served(block) is block._eight and block.quantized
+    for p in block.parameters():
+        p.grad = torch.ones_like(p)
+    CHANGES[change](block)
+    assert served(block) == "fp32" and not block.quantized
+    block.quantize_()
+    eight = served(block)
+    for (q, _), layer in zip(eight, (block.gate, block.up, block.down)):
+        assert torch.equal(q, layer.weight)
+
+
+def test_the_norms_weight_is_not_quantised(served):
+    block = GatedFeedForward(8, 12).eval().quantize_()
+    with torch.no_grad():
+        block.norm_weight.mul_(2)
+    assert served(block) is block._eight
+
+
+def test_copies_keep_current_8_bits_and_no_others(served):
+    block = GatedFeedForward(8, 12).eval().quantize_()
+    stored = io.BytesIO()
+    torch.save(block, stored)
+    stored.seek(0)
+    for other in (copy.deepcopy(block), torch.load(stored, weights_only=False)):
+        assert other.quantized and served(other) is other._eight
+        with torch.no_grad():
+            other.gate.weight.zero_()
+        assert not other.quantized and block.quantized
+    with torch.no_grad():
+        block.gate.weight.zero_()
+    assert not copy.deepcopy(block).quantized
+
+
+def test_inference_tensors_as_weights(served):
+    """Weights made under inference_mode have no count of their changes; they are served."""
+    with torch.inference_mode():
+        block = GatedFeedForward(8, 12).eval().quantize_()
+        assert served(block) is block._eight
