@@ -226,13 +226,12 @@ class RmsNormFn(Function):
 
 
 class GatedLinearFn(Function):
-    """activation(x w_gate^T) * (x w_up^T); both products are kept in fp32 for the backward pass when a
-    gradient will be asked for."""
+    """activation(x w_gate^T) * (x w_up^T); save: both products are kept in fp32 for the backward pass.  The
+    caller decides: forward runs with the gradient mode off, and ctx.needs_input_grad does not know the mode."""
 
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, activation):
+    def forward(ctx, x, w_gate, w_up, activation, save):
         x2, w_gate, w_up = _rows(x), _rows(w_gate), _rows(w_up)
-        save = any(ctx.needs_input_grad)
         out, saved = ops.gated_linear_fwd(x2, w_gate, w_up, activation, save=save)
         if save:
             ctx.save_for_backward(x2, w_gate, w_up, saved)
@@ -247,7 +246,7 @@ class GatedLinearFn(Function):
         dx, dwg, dwu = ops.gated_linear_bwd(_rows(dout), x, w_gate, w_up, saved, ctx.activation,
                                             need_dx=ctx.needs_input_grad[0], need_dw=need_dw)
         return (None if dx is None else dx.view(ctx.shape), dwg if ctx.needs_input_grad[1] else None,
-                dwu if ctx.needs_input_grad[2] else None, None)
+                dwu if ctx.needs_input_grad[2] else None, None, None)
 
 
 def _rows(t):
@@ -267,8 +266,10 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 def gated_linear(x, w_gate, w_up, activation="silu"):
     """activation(x @ w_gate^T) * (x @ w_up^T): the two projections of a gated feed-forward block, their
     activation and product in one kernel.  x [..., k], weights [h, k], all of one dtype (fp32, bf16,
-    fp16); activation 'silu', 'gelu' (erf) or 'relu'."""
-    return GatedLinearFn.apply(x, w_gate, w_up, activation)
+    fp16); activation 'silu', 'gelu' (erf) or 'relu'.  Where a gradient will be asked for, both products are
+    kept in fp32 (8 bytes an output) for the backward pass; without gradients nothing is."""
+    save = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
+    return GatedLinearFn.apply(x, w_gate, w_up, activation, save)
 
 
 def gather_reduce(x, plan_or_ptr, src=None, num_targets=None, reduce="mean", node_map=None):

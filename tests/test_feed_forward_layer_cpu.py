@@ -83,3 +83,48 @@ def test_inference_tensors_as_weights(served):
     with torch.inference_mode():
         block = GatedFeedForward(8, 12).eval().quantize_()
         assert served(block) is block._eight
+
+
+# ------------------------------------------------------------------------------- what the backward pass keeps
+@pytest.fixture
+def kept(monkeypatch):
+    """ops.gated_linear_fwd on the CPU; the list of what `save` was at each call."""
+    calls = []
+
+    def forward(x, w_gate, w_up, activation="silu", save=False, out=None):
+        calls.append(save)
+        g, u = x @ w_gate.t(), x @ w_up.t()
+        return g.sigmoid() * g * u, (torch.stack((g, u)) if save else None)
+    monkeypatch.setattr(ops, "gated_linear_fwd", forward)
+    return calls
+
+
+def test_products_are_kept_for_a_gradient_only(kept):
+    plain, leaf = torch.randn(3, 8), torch.nn.Parameter(torch.randn(5, 8))
+    w = torch.randn(5, 8)
+    for args in ((plain, leaf, w), (plain, w, leaf), (plain.clone().requires_grad_(), w, w), (plain, leaf, leaf)):
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode():
+                want = SF.gated_linear(*args)
+            assert kept.pop() is False and not want.requires_grad
+        got = SF.gated_linear(*args)
+        assert kept.pop() is True and got.requires_grad and torch.equal(got, want)
+        with torch.no_grad(), torch.enable_grad():
+            SF.gated_linear(*args)
+        assert kept.pop() is True
+    SF.gated_linear(plain, w, w)
+    assert kept == [False]
+
+
+def test_blocks_evaluation_keeps_no_products(kept, monkeypatch):
+    monkeypatch.setattr(ops, "rms_norm_fwd", lambda x, w, residual=None, eps=1e-6: (x * w, x if residual is None else x + residual))
+    monkeypatch.setattr(ops, "linear_concat_fwd", lambda a1, w1, *a, **k: a1 @ w1.t())
+    monkeypatch.setattr(ops, "aligned_rows", lambda t: t)
+    block = GatedFeedForward(8, 12)
+    for mode in (block.train, block.eval):
+        mode()
+        with torch.no_grad():
+            block(torch.randn(2, 8), torch.randn(2, 8))
+        assert kept.pop() is False
+        block(torch.randn(2, 8))
+        assert kept.pop() is True
