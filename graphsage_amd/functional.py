@@ -258,7 +258,9 @@ def _rows(t):
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """s / sqrt(mean(s^2) + eps) * weight over the last dimension of x [..., n] (fp32, bf16, fp16; the weight
     in x's dtype or fp32), s = x + residual.  Returns y, or (y, s) with a residual: s goes on as the next
-    residual."""
+    residual.  The residual has x's shape."""
+    if residual is not None and residual.shape != x.shape:      # as rows they could still agree, in another order
+        raise RuntimeError(f"rms_norm: residual: expected shape {list(x.shape)}, got {list(residual.shape)}")
     y, s = RmsNormFn.apply(x, weight, residual, eps)
     return y if residual is None else (y, s)
 

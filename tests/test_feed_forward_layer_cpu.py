@@ -128,3 +128,12 @@ def test_blocks_evaluation_keeps_no_products(kept, monkeypatch):
         assert kept.pop() is False
         block(torch.randn(2, 8))
         assert kept.pop() is True
+
+
+# ------------------------------------------------------------------------------- shapes
+@pytest.mark.parametrize("shape", [(3, 2, 8), (6, 8), (1, 6, 8), (2, 3, 1, 8), (8,), (2, 3, 4)])
+def test_a_residual_of_another_shape_is_refused(monkeypatch, shape):
+    """Also where it has as many rows: they would be other rows."""
+    monkeypatch.setattr(ops, "rms_norm_fwd", lambda x, w, residual=None, eps=1e-6: (x * w, x + residual))
+    with pytest.raises(RuntimeError, match="residual: expected shape"):
+        SF.rms_norm(torch.zeros(2, 3, 8), torch.ones(8), torch.zeros(shape))
