@@ -198,16 +198,17 @@ class L2NormReLUFn(Function):
 
 
 class RmsNormFn(Function):
-    """(y, s): s = x + residual, y = s / rms(s) * weight.  Backward from the stored s, so nothing but it
-    and the weight is kept."""
+    """(y, s) of matrices: s = x + residual, y = s / rms(s) * weight.  Backward from the stored s, so nothing but
+    it and the weight is kept.  The outputs are the operator's own tensors, no views, so that a caller may change
+    y in place."""
 
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         ctx.set_materialize_grads(False)
-        y, s = ops.rms_norm_fwd(_rows(x), weight.contiguous(), None if residual is None else _rows(residual), eps)
+        y, s = ops.rms_norm_fwd(x, weight.contiguous(), residual, eps)
         ctx.save_for_backward(s, weight)
-        ctx.eps, ctx.shape, ctx.has_residual = eps, x.shape, residual is not None
-        return y.view(x.shape), (s.view(x.shape) if residual is not None else None)
+        ctx.eps, ctx.has_residual = eps, residual is not None
+        return y, (s if residual is not None else None)
 
     @staticmethod
     @once_differentiable
@@ -221,22 +222,22 @@ class RmsNormFn(Function):
         elif need_dx or need_dw:
             dx, dw = ops.rms_norm_bwd(_rows(dy), s, weight.contiguous(), ctx.eps, None if ds is None else _rows(ds),
                                       need_dx=need_dx, need_dw=need_dw)
-            dx = None if dx is None else dx.view(ctx.shape)
         return dx, dw, (dx if ctx.has_residual else None), None
 
 
 class GatedLinearFn(Function):
-    """activation(x w_gate^T) * (x w_up^T); save: both products are kept in fp32 for the backward pass.  The
-    caller decides: forward runs with the gradient mode off, and ctx.needs_input_grad does not know the mode."""
+    """activation(x w_gate^T) * (x w_up^T) of matrices; save: both products are kept in fp32 for the backward
+    pass.  The caller decides: forward runs with the gradient mode off, and ctx.needs_input_grad does not know
+    the mode."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, activation, save):
-        x2, w_gate, w_up = _rows(x), _rows(w_gate), _rows(w_up)
-        out, saved = ops.gated_linear_fwd(x2, w_gate, w_up, activation, save=save)
+        w_gate, w_up = _rows(w_gate), _rows(w_up)
+        out, saved = ops.gated_linear_fwd(x, w_gate, w_up, activation, save=save)
         if save:
-            ctx.save_for_backward(x2, w_gate, w_up, saved)
-        ctx.activation, ctx.shape = activation, x.shape
-        return out.view(*x.shape[:-1], out.size(1))
+            ctx.save_for_backward(x, w_gate, w_up, saved)
+        ctx.activation = activation
+        return out
 
     @staticmethod
     @once_differentiable
@@ -245,8 +246,7 @@ class GatedLinearFn(Function):
         need_dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dx, dwg, dwu = ops.gated_linear_bwd(_rows(dout), x, w_gate, w_up, saved, ctx.activation,
                                             need_dx=ctx.needs_input_grad[0], need_dw=need_dw)
-        return (None if dx is None else dx.view(ctx.shape), dwg if ctx.needs_input_grad[1] else None,
-                dwu if ctx.needs_input_grad[2] else None, None, None)
+        return (dx, dwg if ctx.needs_input_grad[1] else None, dwu if ctx.needs_input_grad[2] else None, None, None)
 
 
 def _rows(t):
@@ -255,14 +255,19 @@ def _rows(t):
     return t if t.stride(1) == 1 or t.size(1) <= 1 else t.contiguous()
 
 
+def _shaped(rows, like):
+    """A matrix with the leading dimensions of `like` (itself where that is a matrix)."""
+    return rows if like.dim() == 2 else rows.view(*like.shape[:-1], rows.size(1))
+
+
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """s / sqrt(mean(s^2) + eps) * weight over the last dimension of x [..., n] (fp32, bf16, fp16; the weight
     in x's dtype or fp32), s = x + residual.  Returns y, or (y, s) with a residual: s goes on as the next
     residual.  The residual has x's shape."""
     if residual is not None and residual.shape != x.shape:      # as rows they could still agree, in another order
         raise RuntimeError(f"rms_norm: residual: expected shape {list(x.shape)}, got {list(residual.shape)}")
-    y, s = RmsNormFn.apply(x, weight, residual, eps)
-    return y if residual is None else (y, s)
+    y, s = RmsNormFn.apply(_rows(x), weight, None if residual is None else _rows(residual), eps)
+    return _shaped(y, x) if residual is None else (_shaped(y, x), _shaped(s, x))
 
 
 def gated_linear(x, w_gate, w_up, activation="silu"):
@@ -271,7 +276,7 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
     fp16); activation 'silu', 'gelu' (erf) or 'relu'.  Where a gradient will be asked for, both products are
     kept in fp32 (8 bytes an output) for the backward pass; without gradients nothing is."""
     save = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
-    return GatedLinearFn.apply(x, w_gate, w_up, activation, save)
+    return _shaped(GatedLinearFn.apply(_rows(x), w_gate, w_up, activation, save), x)
 
 
 def gather_reduce(x, plan_or_ptr, src=None, num_targets=None, reduce="mean", node_map=None):

@@ -137,3 +137,27 @@ def test_a_residual_of_another_shape_is_refused(monkeypatch, shape):
     monkeypatch.setattr(ops, "rms_norm_fwd", lambda x, w, residual=None, eps=1e-6: (x * w, x + residual))
     with pytest.raises(RuntimeError, match="residual: expected shape"):
         SF.rms_norm(torch.zeros(2, 3, 8), torch.ones(8), torch.zeros(shape))
+
+
+# ------------------------------------------------------------------------------- outputs
+@pytest.mark.parametrize("shape", [(4, 8), (2, 3, 8), (8,)])
+def test_outputs_may_be_changed_in_place(kept, monkeypatch, shape):
+    """y and the gated product are not kept for the backward pass; s is, and torch says so."""
+    monkeypatch.setattr(ops, "rms_norm_fwd", lambda x, w, residual=None, eps=1e-6: (x * w, x if residual is None else x + residual))
+    monkeypatch.setattr(ops, "rms_norm_bwd", lambda dy, s, w, eps, ds, need_dx, need_dw: (dy * w, (dy * s).sum(0)))
+    monkeypatch.setattr(ops, "gated_linear_bwd", lambda d, x, g, u, saved, act, need_dx, need_dw: (d @ u, d.t() @ x, d.t() @ x))
+    x, r, w = torch.randn(shape, requires_grad=True), torch.randn(shape), torch.ones(8, requires_grad=True)
+    wg, wu = torch.randn(5, 8, requires_grad=True), torch.randn(5, 8)
+    for y in (SF.rms_norm(x, w), SF.rms_norm(x, w, r)[0]):
+        assert y.shape == x.shape
+        y.mul_(3.0).sum().backward()
+        assert bool((x.grad == 3).all())
+        x.grad = None
+    h = SF.gated_linear(x, wg, wu)
+    assert h.shape == (*shape[:-1], 5)
+    h.mul_(2.0).sum().backward()
+    assert x.grad.shape == x.shape and wg.grad.shape == wg.shape
+    y, s = SF.rms_norm(x, w, r)
+    s.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
