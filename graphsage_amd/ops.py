@@ -1439,7 +1439,8 @@ def _like(t, out, name, inputs=(), apart=()):
 def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out=None, sum_out=None):
     """s = x + residual; y = s / sqrt(mean(s^2) + eps) * weight over each row of x [rows, dim]
     (fp32 / bf16 / fp16; weight in x's dtype or fp32).  Returns (y, s); without a residual s is x
-    itself.  sum_out may be `residual` (the residual stream updated in place)."""
+    itself, or None where out is x (y has taken its place, and rms_norm_bwd has no sum to start from).
+    sum_out may be `residual` (the residual stream updated in place)."""
     px, ldx, pr, ldr, pw, wd, shape, dev = _norm_inputs(x, weight, residual)
     if weight is None:
         raise RuntimeError("rms_norm_fwd: weight: tensor required")
@@ -1449,6 +1450,8 @@ def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out=None, sum_out=None):
         s, ps, lds = _like(x, sum_out, "rms_norm_fwd: sum_out", (x, residual), (weight, y))
     elif sum_out is not None:
         raise RuntimeError("rms_norm_fwd: sum_out without a residual")
+    elif out is not None and _overlap(out, x):
+        s = None
     _call("sage_rms_norm_fwd", dev, px, ldx, pr, ldr, pw, wd, shape[0], shape[1], ROW_DTYPES[x.dtype], eps,
           py, ldy, ps, lds)
     return y, s
