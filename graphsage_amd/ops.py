@@ -1414,12 +1414,6 @@ def _norm_inputs(x, weight, residual):
     return px, ldx, pr, ldr, pw, ROW_DTYPES[wd], shape, dev
 
 
-def _output(out, name, shape, dtype, device):
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    return out
-
-
 def _like(t, out, name, inputs=(), apart=()):
     """`out`, checked against t's shape and dtype, or a new tensor: (tensor, pointer, row stride).  It may be one of
     the inputs, or apart from all of them: a row that is another's as well would be read behind its change."""
@@ -1497,8 +1491,7 @@ def dequantize_rows(q, scale, dtype=torch.float32, out=None):
     if shape[1] == 0:
         raise RuntimeError("dequantize_rows: rows of no elements")
     ps = _vector(scale, "dequantize_rows: scale", shape[0], dev)
-    out = _output(out, "out", shape, dtype, dev)
-    po, ldo = _row_matrix(out, "dequantize_rows: out", dtype, shape, dev, output=True)
+    out, po, ldo = _apart_output(out, "dequantize_rows: out", shape, dtype, dev, (q, scale))
     _call("sage_dequantize_rows", dev, pq, ldq, ps, shape[0], shape[1], ROW_DTYPES[dtype], po, ldo)
     return out
 
@@ -1575,7 +1568,7 @@ def _product_workspace(m, n, row_bytes, gated, fp32, device):
     return ws.data_ptr(), size, ws
 
 
-def _product_output(out, name, shape, dtype, device, operands):
+def _apart_output(out, name, shape, dtype, device, operands):
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=device)
         return out, out.data_ptr(), shape[1]
@@ -1631,7 +1624,7 @@ def int8_linear(x, x_scale, weight, w_scale, bias=None, out_dtype=torch.float32,
     px, ldx, psx, m, k, dev = _int8_rows_in(x, x_scale, out_dtype)
     pw, ldw, psw, n = _int8_weight(weight, w_scale, k, dev)
     pb = None if bias is None else _vector(bias, "int8_linear: bias", n, dev)
-    out, po, ldo = _product_output(out, "int8_linear: out", (m, n), out_dtype, dev, (x, x_scale, weight, w_scale, bias))
+    out, po, ldo = _apart_output(out, "int8_linear: out", (m, n), out_dtype, dev, (x, x_scale, weight, w_scale, bias))
     if m > 0:
         wide, ((px, ldx), (pw, ldw)), kept = _product_rows(m, n, k, 1, 0, (x, px, ldx), (weight, pw, ldw))
         ws, ws_bytes, keep = _product_workspace(m, n, wide, 0, 0, dev)
@@ -1648,7 +1641,7 @@ def int8_gated_linear(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation
     pu, ldu, psu, nu = _int8_weight(w_up, up_scale, k, dev)
     if n != nu:
         raise RuntimeError(f"int8_gated_linear: weights of {n} and {nu} rows")
-    out, po, ldo = _product_output(out, "int8_gated_linear: out", (m, n), out_dtype, dev,
+    out, po, ldo = _apart_output(out, "int8_gated_linear: out", (m, n), out_dtype, dev,
                                    (x, x_scale, w_gate, gate_scale, w_up, up_scale))
     if m > 0:
         wide, ((px, ldx), (pg, ldg), (pu, ldu)), kept = _product_rows(m, n, k, 1, 0, (x, px, ldx), (w_gate, pg, ldg), (w_up, pu, ldu))
@@ -1675,7 +1668,7 @@ def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
     fp32 for gated_linear_bwd, else None."""
     px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up)
     act = _activation(activation)
-    out, po, ldo = _product_output(out, "gated_linear_fwd: out", (m, h), x.dtype, dev, (x, w_gate, w_up))
+    out, po, ldo = _apart_output(out, "gated_linear_fwd: out", (m, h), x.dtype, dev, (x, w_gate, w_up))
     saved = torch.empty((2, m, h), dtype=torch.float32, device=dev) if save else None
     if m == 0:
         return out, saved

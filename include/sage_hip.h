@@ -777,7 +777,7 @@ int sage_rms_norm_fwd(const void* x, sage_i64 ld_x, const void* residual, sage_i
 int sage_rms_norm_int8(const void* x, sage_i64 ld_x, const void* residual, sage_i64 ld_r, const void* weight,
                        int weight_dtype, sage_i64 rows, sage_i64 dim, int dtype, float eps, int normalise, int8_t* q,
                        sage_i64 ld_q, sage_i64 q_cols, float* scale, void* sum, sage_i64 ld_sum, void* stream);
-/* out[r, c] = q[r, c] * scale[r], rounded once */
+/* out[r, c] = q[r, c] * scale[r], rounded once; out shares no memory with q or scale */
 int sage_dequantize_rows(const int8_t* q, sage_i64 ld_q, const float* scale, sage_i64 rows, sage_i64 dim, int dtype,
                          void* out, sage_i64 ld_out, void* stream);
 /* Backward of sage_rms_norm_fwd from the stored sum: xh = sum * rstd, c = mean(dy * weight * xh),

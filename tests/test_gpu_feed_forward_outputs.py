@@ -25,3 +25,24 @@ def test_norm_in_place_of_its_rows(dev, dtype, rows, dim):
     assert y is other and s is x
     with pytest.raises(RuntimeError):
         ops.rms_norm_bwd(x, None, w)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dequantised_rows_apart_from_their_inputs(dev, dtype):
+    q, scale = ops.quantize_rows(torch.randn(6, 64, device=dev))
+    size = torch.empty((), dtype=dtype).element_size()
+    hold = torch.zeros(6 * 64 * (size + 1) + 64, dtype=torch.int8, device=dev)
+    rows = hold[:6 * 64].view(6, 64)
+    rows.copy_(q)
+    for start in (0, 64, 5 * 64):
+        out = hold[start:start + 6 * 64 * size].view(dtype).view(6, 64)
+        with pytest.raises(RuntimeError, match="shares memory"):
+            ops.dequantize_rows(rows, scale, dtype, out=out)
+    if dtype == torch.float32:
+        both = torch.zeros(6 * 64, device=dev)
+        both[:6] = scale
+        with pytest.raises(RuntimeError, match="shares memory"):
+            ops.dequantize_rows(q, both[:6], dtype, out=both.view(6, 64))
+    out = hold[6 * 64:6 * 64 * (size + 1)].view(dtype).view(6, 64)       # behind the last row
+    assert torch.equal(ops.dequantize_rows(rows, scale, dtype, out=out), ops.dequantize_rows(q, scale, dtype))
+    assert torch.equal(rows, q)
