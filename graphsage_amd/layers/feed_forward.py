@@ -15,6 +15,9 @@ a raw pointer is not counted and needs quantize_() again).  They serve calls in 
 every other call takes the fp32 weights.  A graph captured while they served reads them where they lay: keep
 the weights as they are, and the block in eval mode, for as long as it is replayed.
 
+x and the residual are matrices [rows, channels].  With the fp32 weights they are fp32 too; the 8-bit weights serve
+fp32, bf16 and fp16 rows.
+
 A training step of the block can be captured into a graph.  As with any module, no eager output of the same
 parameters may be alive then: torch keeps the stream of a parameter's gradient with the first of them, and
 a captured backward pass cannot wait for that stream.
@@ -97,6 +100,9 @@ class GatedFeedForward(torch.nn.Module):
     def forward(self, x, residual=None):
         if not self.training and not torch.is_grad_enabled() and self._current():
             return self._serve(x, residual)
+        if x.dtype != torch.float32 or self.down.weight.dtype != torch.float32:
+            raise RuntimeError(f"GatedFeedForward: expected fp32 rows and weights, got {x.dtype} and {self.down.weight.dtype} "
+                               "(16-bit rows are served by the 8-bit weights, see quantize_)")
         if residual is None:
             y, s = SF.rms_norm(x, self.norm_weight, eps=self.eps), x
         else:

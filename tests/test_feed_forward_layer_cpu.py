@@ -161,3 +161,15 @@ def test_outputs_may_be_changed_in_place(kept, monkeypatch, shape):
     s.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_16_bit_blocks_are_refused_before_any_work(monkeypatch):
+    """The down projection is an fp32 product."""
+    monkeypatch.setattr(SF, "rms_norm", lambda *a, **k: pytest.fail("launched"))
+    block = GatedFeedForward(8, 12)
+    with pytest.raises(RuntimeError, match="expected fp32 rows"):
+        block(torch.zeros(2, 8, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="expected fp32 rows"):
+        block.half()(torch.zeros(2, 8, dtype=torch.float16))
+    with pytest.raises(RuntimeError, match="expected fp32 rows"):
+        block.eval()(torch.zeros(2, 8))
