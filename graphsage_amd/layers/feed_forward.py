@@ -112,6 +112,7 @@ class GatedFeedForward(torch.nn.Module):
 
     def _serve(self, x, residual):
         (gate, gate_scale), (up, up_scale), (down, down_scale) = self._eight
+        x, residual = (t if t is None or t.dim() != 2 else SF._rows(t) for t in (x, residual))
         y, y_scale, s = ops.rms_norm_int8(x, self.norm_weight, residual, self.eps, padded=True)
         # bf16 between the two products: its rounding is a 128th of the 8-bit step that follows at the row's
         # largest values, and halves the bytes

@@ -66,3 +66,19 @@ def test_served_block_rounds_its_sum_once(dev, dtype, rows):
         with torch.no_grad():
             got = block(x, residual)
         assert got.dtype == dtype and torch.equal(got, want) and torch.equal(x, kept)
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_served_block_takes_rows_of_any_strides(dev, rows):
+    """As the block does with its fp32 weights: transposed, every other column, one row repeated."""
+    torch.manual_seed(rows)
+    block = GatedFeedForward(96, 130).to(dev).eval()
+    wide, row = torch.randn(192, rows, device=dev), torch.randn(1, 96, device=dev)
+    for x, r in ((wide[:96].t(), wide[96:].t()), (wide[::2].t(), None), (wide[:96].t(), row.expand(rows, 96))):
+        full = x.contiguous(), None if r is None else r.contiguous()
+        for layout in (block.dequantize_, block.quantize_):
+            layout()
+            with torch.no_grad():
+                assert torch.equal(block(x, r), block(*full))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="2-D"):
+        block(torch.randn(2, 3, 96, device=dev))
