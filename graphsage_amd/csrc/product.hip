@@ -186,21 +186,17 @@ __device__ inline void load_run(const float* p, int64_t left, float (&v)[n]) {
   }
 }
 
-// n consecutive columns of one row, from the sums of one B
+// n consecutive columns of one row, from the sums of one B (8 bits: the other types' products with few rows are pairs)
 template <typename T, int n, typename S>
 __device__ inline void finish(const Product& p, int64_t row, int64_t col, const S (&c)[n]) {
+  static_assert(std::is_same<T, int8_t>::value, "the form that is used");
   if (row >= p.m || col >= p.n) return;
   float v[n];
-  if constexpr (std::is_same<T, int8_t>::value) {
-    const float sa = p.sa[row];
+  const float sa = p.sa[row];
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const int64_t at = col + i < p.n ? col + i : p.n - 1;
-      v[i] = static_cast<float>(c[i]) * (sa * p.sb0[at]) + (p.bias != nullptr ? p.bias[at] : 0.f);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < n; ++i) v[i] = c[i];
+  for (int i = 0; i < n; ++i) {
+    const int64_t at = col + i < p.n ? col + i : p.n - 1;
+    v[i] = static_cast<float>(c[i]) * (sa * p.sb0[at]) + (p.bias != nullptr ? p.bias[at] : 0.f);
   }
   store_out<n>(p, row, col, v);
 }
@@ -861,12 +857,6 @@ __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_pair_kernel(Product
   finish_gated<T, 4>(p, l15, n0 + q * 4, c, d);
 }
 
-// ------------------------------------------------------------------------------- launch
-inline bool rows16(const void* p, int64_t ld_bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld_bytes & 15) == 0 && ld_bytes >= 0;
-}
-constexpr int64_t kMaxRowBytes = int64_t{1} << 23;     // the tile loads' offsets: 256 rows in 31 bits
-
 // Up to 8 rows against one B in blocks of 8 columns: an MFMA operand's slots 8 to 15 are the rows and columns of slots 0
 // to 7 again, at later bytes of k, so that C's two diagonal quarters add up to the 8 x 8 outputs.
 template <typename T, int U, bool kRagged>
@@ -903,6 +893,12 @@ __global__ void __launch_bounds__(kFewWaves* kWave) few_rows_half_kernel(Product
   for (int e = 0; e < 4; ++e) c[e] = sum[e];
   finish<T, 4>(p, l15, n0 + q * 4, c);
 }
+
+// ------------------------------------------------------------------------------- launch
+inline bool rows16(const void* p, int64_t ld_bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld_bytes & 15) == 0 && ld_bytes >= 0;
+}
+constexpr int64_t kMaxRowBytes = int64_t{1} << 23;     // the tile loads' offsets: 256 rows in 31 bits
 
 // How a product is cut: blocks of 64 rows and 16 columns (tile 0: few_rows_kernel), or tiles of `tile` x `tile`
 // (gated: `tile` / 2 columns), k in `slices`.
