@@ -129,6 +129,7 @@ SIGNATURES = {
                                  _P, c_size_t, _P]),
     "sage_product_any_rows": (c_int, [c_int64, c_int64, c_int64, c_int, c_int]),
     "sage_product_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "sage_product_cut": (c_int, [c_int64, c_int64, c_int64, c_int, c_int, c_int, _P, _P]),
     "sage_int8_gated_linear": (c_int, [_P, c_int64, _P, _P, c_int64, _P, _P, c_int64, _P, c_int, c_int64, c_int64,
                                        c_int64, c_int, _P, c_int64, _P, c_size_t, _P]),
     "sage_gated_linear_fwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int, c_int64, c_int64, c_int64, c_int,

@@ -1197,6 +1197,17 @@ extern "C" size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 
   return plan_product(m, n, row_bytes, gated != 0, fp32 != 0, true).workspace;
 }
 
+extern "C" int sage_product_cut(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32, int few_rows, int* tile_host,
+                                int* slices_host) {
+  SAGE_REQUIRE(m > 0 && n > 0 && row_bytes > 0, SAGE_EINVAL, "sage_product_cut: bad shape m %ld n %ld, rows of %ld bytes", (long)m,
+               (long)n, (long)row_bytes);
+  SAGE_REQUIRE(tile_host != nullptr && slices_host != nullptr, SAGE_EINVAL, "sage_product_cut: NULL pointer");
+  const Plan plan = plan_product(m, n, row_bytes, gated != 0, fp32 != 0, few_rows != 0);
+  *tile_host = plan.tile;
+  *slices_host = plan.slices;
+  return SAGE_OK;
+}
+
 #define SAGE_INT8_CHECKS(what)                                                                                          \
   SAGE_REQUIRE(known_dtype(out_dtype), SAGE_EINVAL, what ": unknown output dtype %d", out_dtype);                       \
   SAGE_REQUIRE(m >= 0 && n > 0 && k > 0, SAGE_EINVAL, what ": bad shape m %ld n %ld k %ld", (long)m, (long)n, (long)k); \

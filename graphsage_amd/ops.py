@@ -1559,6 +1559,15 @@ def _product_rows(m, n, k, size, fp32, *mats):
     return _pieces(k, size, mats)
 
 
+def product_cut(m, n, row_bytes, gated=False, fp32=False, few_rows=True):
+    """(tile, slices of k) that a product of these sizes takes on the GPU: tile 256, 128 or 0 (the kernels for few
+    rows).  few_rows=False: of the backward pass, whose products do not take those."""
+    tile, slices = ctypes.c_int(), ctypes.c_int()
+    rc = _lib.load().sage_product_cut(m, n, row_bytes, gated, fp32, few_rows, ctypes.byref(tile), ctypes.byref(slices))
+    _lib.check(rc, "sage_product_cut")
+    return tile.value, slices.value
+
+
 def _product_workspace(m, n, row_bytes, gated, fp32, device):
     """(pointer, bytes, owner) of what a product of few tiles splits k into; the fewest rows take none."""
     size = _lib.load().sage_product_workspace_bytes(m, n, row_bytes, gated, fp32) if m > 16 else 0

@@ -805,6 +805,12 @@ int sage_product_any_rows(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated,
  * element's size; gated: two weights; fp32: fp32 operands.  The operands' rows are less than 2^23 bytes
  * apart. */
 size_t sage_product_workspace_bytes(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32);
+/* The cut that a product takes: tile_host 256 or 128 (outputs of a block along a side; gated: half as many columns),
+ * 0 the kernels for few rows; slices_host: of k.  few_rows = 0: a product that does not take those, as the
+ * backward pass's (sage_gated_linear_bwd: dx is m x k over 2 w, dw w + h x k over m, w = h in whole runs of 64
+ * bytes).  Work only on the host; tests hold the sizes to the kernels they mean with it. */
+int sage_product_cut(sage_i64 m, sage_i64 n, sage_i64 row_bytes, int gated, int fp32, int few_rows, int* tile_host,
+                     int* slices_host);
 /* out[m, n] = x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]; the sum is exact (32-bit
  * integers, k <= SAGE_INT8_MAX_K), the rest fp32, rounded once to out_dtype.  bias may be NULL. */
 int sage_int8_linear(const int8_t* x, sage_i64 ld_x, const float* x_scale, const int8_t* w, sage_i64 ld_w,

@@ -2,12 +2,13 @@
 and which weights it serves."""
 import copy
 import io
+import itertools
 
 import pytest
 import torch
 
 from graphsage_amd import functional as SF
-from graphsage_amd import ops
+from graphsage_amd import _lib, ops
 from graphsage_amd.layers import GatedFeedForward
 
 
@@ -173,3 +174,27 @@ def test_16_bit_blocks_are_refused_before_any_work(monkeypatch):
         block.half()(torch.zeros(2, 8, dtype=torch.float16))
     with pytest.raises(RuntimeError, match="expected fp32 rows"):
         block.eval()(torch.zeros(2, 8))
+
+
+# ------------------------------------------------------------------------------- the products' cuts
+def test_product_cut_agrees_with_what_the_products_ask_for():
+    """Its slices with the workspace (a tile's sums in 32 bits for each), its 0 with the sizes that take any rows."""
+    lib = _lib.load()
+    seen = set()
+    for m, n, k, gated, fp32 in itertools.product((1, 16, 17, 300, 512, 513, 2049, 8192), (1, 64, 700, 4099, 8192), (16, 64, 1040, 4112, 40000),
+                                                  (False, True), (False, True)):
+        tile, slices = ops.product_cut(m, n, k, gated, fp32)
+        seen.add((tile, slices > 1))
+        assert lib.sage_product_any_rows(m, n, k, gated, fp32) == (tile == 0)
+        across = tile // 2 if gated else tile
+        want = 0 if slices == 1 else -(-m // tile) * -(-n // across) * tile * tile * 4 * slices
+        assert lib.sage_product_workspace_bytes(m, n, k, gated, fp32) == want
+        assert ops.product_cut(m, n, k, gated, fp32, few_rows=False)[0] in (128, 256)
+    assert seen == {(0, False), (128, False), (128, True), (256, False), (256, True)}
+
+
+def test_product_cut_refusals():
+    for bad in ((0, 8, 64), (8, 0, 64), (8, 8, 0), (-1, 8, 64)):
+        with pytest.raises(RuntimeError, match="sage_product_cut"):
+            ops.product_cut(*bad)
+    assert _lib.load().sage_product_cut(8, 8, 64, 0, 0, 1, None, None) == -1
