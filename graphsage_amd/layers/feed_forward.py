@@ -118,8 +118,9 @@ class GatedFeedForward(torch.nn.Module):
         # largest values, and halves the bytes
         h = ops.int8_gated_linear(y, y_scale, gate, gate_scale, up, up_scale, self.activation, torch.bfloat16)
         h, h_scale = ops.quantize_rows(h, padded=True)
-        z = ops.int8_linear(h, h_scale, down, down_scale)      # fp32: the sum is rounded once
-        return z.add_(s) if s.dtype == z.dtype else torch.add(z, s, out=torch.empty_like(s))
+        # 16-bit rows: the product is rounded before the sum is.  Its own rounding is a small part of what 8-bit operands
+        # leave of it, and an fp32 product costs 8 us of 60 (8192 rows of 256 channels, 1024 hidden)
+        return ops.int8_linear(h, h_scale, down, down_scale, out_dtype=s.dtype).add_(s)
 
     def __repr__(self):
         return f'{self.__class__.__name__}({self.channels}, {self.hidden_channels}, activation={self.activation})'
