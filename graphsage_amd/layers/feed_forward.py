@@ -55,16 +55,32 @@ class GatedFeedForward(torch.nn.Module):
         self._eight_of = self._weights_now()
         return self
 
+    def _sources(self):
+        """What the three weights are made of: the layers' own parameters, or a parametrization's."""
+        m = self._modules
+        found = []
+        for layer in (m["gate"], m["up"], m["down"]):
+            found += layer.parameters() if layer._modules else layer._parameters.values()
+        return found
+
     def _weights_now(self):
-        weights = (self.gate.weight, self.up.weight, self.down.weight)
-        return tuple((w, w.data_ptr(), None if w.is_inference() else w._version) for w in weights)
+        return [p if p is None else (p, p.data_ptr(), None if p.is_inference() else p._version) for p in self._sources()]
 
     def _current(self):
         """The 8-bit weights are there and still those of the weights; if not, they are dropped."""
-        if self._eight is not None and not all(a[0] is b[0] and a[1:] == b[1:]
-                                               for a, b in zip(self._eight_of, self._weights_now())):
+        if self._eight is None:
+            return False
+        now = self._sources()
+        same = len(now) == len(self._eight_of)
+        for p, of in zip(now, self._eight_of):
+            if p is not None and of is not None:
+                was, at, count = of
+                same = same and p is was and (count is None or p._version == count) and p.data_ptr() == at
+            elif p is not of:
+                same = False
+        if not same:
             self._eight = self._eight_of = None
-        return self._eight is not None
+        return same
 
     def __getstate__(self):              # copies and pickles take the 8-bit weights along where they are current
         self._current()
@@ -112,7 +128,10 @@ class GatedFeedForward(torch.nn.Module):
 
     def _serve(self, x, residual):
         (gate, gate_scale), (up, up_scale), (down, down_scale) = self._eight
-        x, residual = (t if t is None or t.dim() != 2 else SF._rows(t) for t in (x, residual))
+        if x.dim() == 2 and x.stride(1) != 1:
+            x = SF._rows(x)
+        if residual is not None and residual.dim() == 2 and residual.stride(1) != 1:
+            residual = SF._rows(residual)
         y, y_scale, s = ops.rms_norm_int8(x, self.norm_weight, residual, self.eps, padded=True)
         # bf16 between the two products: its rounding is a 128th of the 8-bit step that follows at the row's
         # largest values, and halves the bytes

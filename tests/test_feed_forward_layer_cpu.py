@@ -64,6 +64,16 @@ def test_the_norms_weight_is_not_quantised(served):
     assert served(block) is block._eight
 
 
+def test_parametrized_weights_are_served_until_they_change(served):
+    block = GatedFeedForward(8, 12).eval()
+    torch.nn.utils.parametrizations.weight_norm(block.up)
+    block.quantize_()
+    assert served(block) is block._eight and served(block) is block._eight
+    with torch.no_grad():
+        block.up.parametrizations.weight.original0.mul_(2)
+    assert served(block) == "fp32"
+
+
 def test_copies_keep_current_8_bits_and_no_others(served):
     block = GatedFeedForward(8, 12).eval().quantize_()
     stored = io.BytesIO()
