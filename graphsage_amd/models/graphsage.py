@@ -46,6 +46,11 @@ class GraphSAGE(torch.nn.Module):
             self.blocks = torch.nn.ModuleList([GatedFeedForward(hidden_channels, ffn_channels, ffn_activation)
                                                for _ in range(len(self.layers) - 1)])
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if not hasattr(self, 'blocks'):          # a whole model stored before there were any
+            self.blocks = None
+
     def quantize_(self):
         """8-bit weights for the feed-forward blocks (see GatedFeedForward.quantize_); call in eval mode."""
         if self.blocks is None:

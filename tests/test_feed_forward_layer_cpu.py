@@ -10,6 +10,7 @@ import torch
 from graphsage_amd import functional as SF
 from graphsage_amd import _lib, ops
 from graphsage_amd.layers import GatedFeedForward
+from graphsage_amd.models import GraphSAGE
 
 
 @pytest.fixture
@@ -208,3 +209,18 @@ def test_product_cut_refusals():
         with pytest.raises(RuntimeError, match="sage_product_cut"):
             ops.product_cut(*bad)
     assert _lib.load().sage_product_cut(8, 8, 64, 0, 0, 1, None, None) == -1
+
+
+# ------------------------------------------------------------------------------- stored models
+def test_models_stored_before_there_were_blocks(served):
+    """A whole model without the attribute loads as one without blocks; one with blocks keeps them."""
+    old = GraphSAGE(8, 8)
+    del old.blocks
+    for model, count in ((old, None), (GraphSAGE(8, 8, num_layers=3, ffn_channels=12), 2)):
+        stored = io.BytesIO()
+        torch.save(model, stored)
+        stored.seek(0)
+        back = torch.load(stored, weights_only=False)
+        assert (back.blocks if count is None else len(back.blocks)) == count
+        x = torch.zeros(2, 8)
+        assert back._feed_forward(0, x, x) is x if count is None else len(list(back.blocks.parameters())) == 8
