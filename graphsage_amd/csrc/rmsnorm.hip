@@ -14,9 +14,9 @@
 // pass norms the fp32 sum s; the s that is stored, and that the backward pass reads, is rounded once
 // to the rows' type, as a residual stream in that type is.
 //
-// Measured (a large copy runs at 5.16 TB/s): forward to 8 bits, 8192 x 5120 bf16 with a residual 87 us
-// = 4.8 TB/s; forward and backward, 16381 x 2047 bf16 134 us = 3.5 TB/s, of which the backward pass
-// 71 us = 3.8 TB/s.
+// Measured (a large copy runs at 5.16 TB/s): forward to 8 bits, 8192 x 5120 bf16 with a residual 70 us
+// = 4.2 TB/s; forward, 16381 x 2047 bf16 59 us = 4.5 TB/s; its backward pass 64 us = 4.2 TB/s and 7 us
+// for dw's join.
 //
 // Rows start at any address: vectors are loaded and stored with the element's alignment (gfx950
 // splits a misaligned 16-byte access itself), so odd widths need no other kernel; a row's last

@@ -1691,7 +1691,8 @@ def gated_linear_fwd(x, w_gate, w_up, activation="silu", save=False, out=None):
 
 def gated_linear_bwd(dh, x, w_gate, w_up, saved, activation="silu", need_dx=True, need_dw=True):
     """Gradients of gated_linear_fwd: (dx, dw_gate, dw_up); the two weight gradients are the halves of
-    one [2 h, k] buffer."""
+    one [2 h, k] buffer.  The gradients of the two products are rounded to x's dtype on the way, in fp16 to its
+    range as well (a loss scale has to leave them below 65504)."""
     px, ldx, pg, ldg, pu, ldu, m, h, k, dev = _gated_inputs(x, w_gate, w_up)
     act = _activation(activation)
     pd, ldd = _row_matrix(dh, "gated_linear_bwd: dh", x.dtype, (m, h), dev)

@@ -827,7 +827,7 @@ int sage_gated_linear_fwd(const void* x, sage_i64 ld_x, const void* w_gate, sage
                           sage_i64 ld_u, int activation, sage_i64 m, sage_i64 h, sage_i64 k, int dtype, void* out,
                           sage_i64 ld_out, float* saved, void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients: dg = dh * u * activation'(g), du = dh * activation(g) (rounded to dtype: the products'
- * operands), dx = dg w_gate + du w_up, dw = [dg^T x ; du^T x] as one [2 h, k] matrix.  dx or dw may
+ * operands; fp16: to its range as well), dx = dg w_gate + du w_up, dw = [dg^T x ; du^T x] as one [2 h, k] matrix.  dx or dw may
  * be NULL.  x's and the weights' rows start on 16 bytes and can be read to whole pieces of 16 bytes; the
  * weights' row strides are the same.  The workspace starts on 256 bytes. */
 size_t sage_gated_linear_bwd_workspace_bytes(sage_i64 m, sage_i64 h, sage_i64 k, int dtype);
